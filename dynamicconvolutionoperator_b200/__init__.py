@@ -5,10 +5,16 @@ Public surface:
   * ``DDPM`` — the module (reference ``triton_impl.py:247-392``).
   * ``fused_dynamic_cat`` / ``fused_generator_dynamic_cat`` — the differentiable
     kernel-level ops (reference ``_triton_kernels.py:869``, ``:1056``).
+  * ``group_norm_act`` / ``dropout`` — differentiable channel-last operators
+    around the module: group norm with an activation, dropout from a
+    counter-based generator.
   * ``data_parallel`` — batch-sharded training helpers over NCCL.
 """
 
+from ._dropout import dropout
 from ._kernels import fused_dynamic_cat, fused_generator_dynamic_cat
+from ._norm import group_norm_act
 from .ddpm import DDPM
 
-__all__ = ["DDPM", "fused_dynamic_cat", "fused_generator_dynamic_cat"]
+__all__ = ["DDPM", "dropout", "fused_dynamic_cat", "fused_generator_dynamic_cat",
+           "group_norm_act"]

@@ -21,6 +21,9 @@ DTYPE_CODE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _c_int = ctypes.c_int
 _c_ptr = ctypes.c_void_p
 _c_size = ctypes.c_size_t
+_c_i64 = ctypes.c_longlong
+_c_u64 = ctypes.c_ulonglong
+_c_float = ctypes.c_float
 
 # name -> (restype, argtypes); mirrors include/ddpm_b200.h
 _SIGNATURES: dict[str, tuple[object, list[object]]] = {
@@ -111,6 +114,20 @@ _SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "ddpm_fuseconv_bwd_weight": (
         _c_int, [_c_ptr] * 5 + [_c_size] + [_c_int] * 6 + [_c_ptr]
     ),
+    "ddpm_group_norm_workspace_bytes": (_c_size, [_c_i64] * 2 + [_c_int] * 4),
+    "ddpm_group_norm_fwd": (
+        _c_int,
+        [_c_ptr] * 6 + [_c_size] + [_c_i64] * 2 + [_c_int] * 2 + [_c_float] + [_c_int] * 3
+        + [_c_ptr],
+    ),
+    "ddpm_group_norm_bwd": (
+        _c_int,
+        [_c_ptr] * 9 + [_c_size] + [_c_i64] * 2 + [_c_int] * 5 + [_c_ptr],
+    ),
+    "ddpm_dropout": (
+        _c_int,
+        [_c_ptr] * 3 + [_c_i64, ctypes.c_double, _c_u64, _c_ptr, _c_u64, _c_int, _c_ptr],
+    ),
     "ddpm_test_skip_arrive": (_c_int, [_c_int]),
     "ddpm_test_disable_tma": (_c_int, [_c_int]),
     "ddpm_umma_selftest": (
@@ -156,6 +173,17 @@ def call(name: str, *args) -> None:
     if rc != 0:
         msg = lib.ddpm_last_error().decode(errors="replace")
         raise RuntimeError(f"{name} failed (code {rc}): {msg}")
+
+
+def call_on(device: torch.device, name: str, *args) -> None:
+    """``call`` with ``device`` current and torch's current stream on it as the
+    last argument."""
+    stream = torch.cuda.current_stream(device).cuda_stream
+    if torch.cuda.current_device() == device.index:
+        call(name, *args, stream)
+    else:
+        with torch.cuda.device(device):
+            call(name, *args, stream)
 
 
 def device_status(reset: bool = True) -> int:

@@ -89,6 +89,16 @@ int read_status(int reset, int* code);
 size_t fuseconv_wgrad_workspace_bytes(int n, int cin, int cout, int h, int w);
 int fuseconv_wgrad(const void* cat, const void* gout, void* gw, void* gb, void* ws, size_t ws_bytes,
                    int n, int cin, int cout, int h, int w, int dt, cudaStream_t st);
+size_t group_norm_workspace_bytes(long long n, long long P, int C, int G, int dt, int bwd);
+int group_norm_fwd(const void* x, const void* w, const void* b, void* out, void* stats, void* ws,
+                   size_t ws_bytes, long long n, long long P, int C, int G, float eps, int act,
+                   int dt, int pdt, cudaStream_t st);
+int group_norm_bwd(const void* x, const void* dy, const void* w, const void* b, const void* stats,
+                   void* gx, void* gw, void* gb, void* ws, size_t ws_bytes, long long n,
+                   long long P, int C, int G, int act, int dt, int pdt, cudaStream_t st);
+int dropout(const void* x, const void* residual, void* out, long long n, double p,
+            unsigned long long seed, const void* seed_ptr, unsigned long long offset, int dt,
+            cudaStream_t st);
 }  // namespace ddpm
 
 extern "C" {
@@ -346,6 +356,40 @@ int ddpm_fuseconv_bwd_weight(const void* x, const void* grad_out, void* grad_wei
   ddpm::clear_error();
   return ddpm::fuseconv_wgrad(x, grad_out, grad_weight, grad_bias, workspace, workspace_bytes, n,
                               cin, cout, h, w, dtype, static_cast<cudaStream_t>(stream));
+}
+
+size_t ddpm_group_norm_workspace_bytes(long long n, long long pixels, int channels, int groups,
+                                       int dtype, int bwd) {
+  return ddpm::group_norm_workspace_bytes(n, pixels, channels, groups, dtype, bwd);
+}
+
+int ddpm_group_norm_fwd(const void* x, const void* weight, const void* bias, void* out, void* stats,
+                        void* workspace, size_t workspace_bytes, long long n, long long pixels,
+                        int channels, int groups, float eps, int act, int dtype, int param_dtype,
+                        void* stream) {
+  ddpm::clear_error();
+  return ddpm::group_norm_fwd(x, weight, bias, out, stats, workspace, workspace_bytes, n, pixels,
+                              channels, groups, eps, act, dtype, param_dtype,
+                              static_cast<cudaStream_t>(stream));
+}
+
+int ddpm_group_norm_bwd(const void* x, const void* grad_out, const void* weight, const void* bias,
+                        const void* stats, void* grad_x, void* grad_weight, void* grad_bias,
+                        void* workspace, size_t workspace_bytes, long long n, long long pixels,
+                        int channels, int groups, int act, int dtype, int param_dtype,
+                        void* stream) {
+  ddpm::clear_error();
+  return ddpm::group_norm_bwd(x, grad_out, weight, bias, stats, grad_x, grad_weight, grad_bias,
+                              workspace, workspace_bytes, n, pixels, channels, groups, act, dtype,
+                              param_dtype, static_cast<cudaStream_t>(stream));
+}
+
+int ddpm_dropout(const void* x, const void* residual, void* out, long long size, double p,
+                 unsigned long long seed, const void* seed_ptr, unsigned long long offset,
+                 int dtype, void* stream) {
+  ddpm::clear_error();
+  return ddpm::dropout(x, residual, out, size, p, seed, seed_ptr, offset, dtype,
+                       static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

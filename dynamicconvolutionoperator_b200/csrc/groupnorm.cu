@@ -1,0 +1,669 @@
+// Group norm with an activation over channel-last data, forward and backward.
+//
+//   x [N][P][C] (P pixels, channels innermost), G groups of cg = C / G channels
+//   mean, rstd   per (n, g) over cnt = P * cg values, biased variance
+//   z    = (x - mean) * rstd * weight[c] + bias[c],   out = act(z)
+// backward, with dz = dy * act'(z) and xhat = (x - mean) * rstd:
+//   dbias = sum dz, dweight = sum dz * xhat          (over n, pixels)
+//   A = sum_group weight * dz / cnt, B = sum_group weight * dz * xhat / cnt
+//   dx = rstd * (weight * dz - A - xhat * B)
+//
+// Bound: HBM. Both directions need their group's sums before the first value
+// can be written, so the data is needed twice; the point of the design is that
+// the second time comes from L2. One persistent launch walks chunks (R pixels
+// of one sample) in order: a block sums chunk t (phase 1), and L steps later,
+// when every block has passed the end of that chunk's sample, writes it
+// (phase 2). L = ceil((chunks of a sample - 1) / grid), 0 or 1 for samples up
+// to 16 MB, so what lies between the two phases is a few tens of MB.
+//
+// The blocks of a sample meet through a counter: the last one to add its
+// partial sums folds the sample's partials in their fixed order (no floating
+// point atomics: results do not depend on the order of arrival) and raises the
+// sample's flag; phase 2 waits for the flag. No block waits for a phase 1
+// that lies behind a wait of the same step, and the cooperative launch keeps
+// all blocks resident, so the waits end; they are bounded all the same.
+//
+// Variance: every thread sums x - s and (x - s)^2 for its own channel about
+// its first value s, then (count, mean, squared deviations) triples are merged
+// exactly, so a mean far from zero costs no precision.
+#include "act.cuh"
+#include "common.cuh"
+#include "tc.cuh"
+
+namespace ddpm {
+
+namespace gencat {
+int status_ptr(int** out);
+int num_sms();
+}  // namespace gencat
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kWarps = kThreads / 32;
+constexpr int kMaxChannels = 65536;  // at one channel a thread: 256 tiles, fewer than the blocks
+constexpr uint64_t kWaitLimitNs = 2000000000ull;
+
+struct NormParams {
+  const void* x;
+  const void* dy;      // backward only
+  const void* weight;  // nullable (ones)
+  const void* bias;    // nullable (zeros)
+  void* out;           // out, or dx (nullable in the backward)
+  float2* stats;       // [N][G] mean, rstd (written by the forward)
+  float2* part;        // [N * S][U] partial sums of a chunk
+  float2* grp;         // backward: [N][G] A, B
+  float2* wsum;        // backward: [grid / CT][C] sums of dz, dz * xhat; nullable
+  unsigned* count;     // [N] arrivals, then [N] flags; zeroed before the launch
+  int* status;
+  long long P;
+  int N, C, G, cg;
+  int R, S, CT, TX, TY, U, uw;  // uw: channels of a unit (partials are kept per unit)
+  long long chunks;
+  int lag, act, param_f32;
+  float eps;
+};
+
+template <typename T, int V> struct alignas(sizeof(T) * V) Vec { T e[V]; };
+
+template <typename T> __device__ __forceinline__ float load_param(const void* p, int c, int f32) {
+  return f32 ? __ldg(static_cast<const float*>(p) + c) : ldg_f32<T>(static_cast<const T*>(p) + c);
+}
+
+// Sum over the warp, the same in every lane.
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+// What a block's threads keep for the whole launch.
+template <int V> struct Column {
+  int c0;        // first channel
+  bool live;
+  float w[V], b[V];
+};
+
+// Chunk t -> sample, first pixel, pixels.
+struct Chunk {
+  int n, rows;
+  long long at;  // index of the first pixel over all samples
+};
+__device__ __forceinline__ Chunk chunk_of(const NormParams& p, long long t) {
+  const long long ns = t / p.CT;
+  Chunk k;
+  k.n = (int)(ns / p.S);
+  const int s = (int)(ns - (long long)k.n * p.S);
+  const long long first = (long long)s * p.R;
+  k.at = (long long)k.n * p.P + first;
+  k.rows = (int)(p.P - first < p.R ? p.P - first : p.R);
+  return k;
+}
+
+__device__ __forceinline__ unsigned add_acq_rel(unsigned* p) {
+  unsigned old;
+  asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(old) : "l"(p) : "memory");
+  return old;
+}
+__device__ __forceinline__ unsigned load_acquire(const unsigned* p) {
+  unsigned v;
+  asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
+  return v;
+}
+__device__ __forceinline__ void store_release(unsigned* p, unsigned v) {
+  asm volatile("st.release.gpu.global.u32 [%0], %1;" ::"l"(p), "r"(v) : "memory");
+}
+
+// (mean, squared deviations) of unit u of the tile from the per-thread pairs
+// in shared memory; every lane of the warp gets the result.
+__device__ __forceinline__ float2 merge_unit(const NormParams& p, const float2* sh, int u,
+                                             int width, int rows, int lane) {
+  const int items = p.TY * p.uw;
+  const int full = rows / p.TY, rest = rows - full * p.TY;
+  const float m0 = sh[u * p.uw].x;  // sums about the first mean: no digits lost to a large one
+  float s = 0.f;
+  for (int i = lane; i < items; i += 32) {
+    const int ty = i / p.uw;
+    const float k = (float)(full + (ty < rest));
+    if (k > 0.f) s += k * (sh[ty * width + u * p.uw + (i - ty * p.uw)].x - m0);
+  }
+  const float cnt = (float)rows * (float)p.uw;
+  const float mean = m0 + warp_sum(s) / cnt;
+  float m2 = 0.f;
+  for (int i = lane; i < items; i += 32) {
+    const int ty = i / p.uw;
+    const float k = (float)(full + (ty < rest));
+    const float2 v = sh[ty * width + u * p.uw + (i - ty * p.uw)];
+    const float d = v.x - mean;
+    if (k > 0.f) m2 += v.y + k * d * d;
+  }
+  return make_float2(mean, warp_sum(m2));
+}
+
+// Forward statistics of sample n from its chunks' partials (one block).
+__device__ void fold_stats(const NormParams& p, int n, int warp, int lane) {
+  const int upg = p.U / p.G;
+  const int items = p.S * upg;
+  const float total = (float)((double)p.P * p.cg);
+  const int last = (int)(p.P - (long long)(p.S - 1) * p.R);
+  for (int g = warp; g < p.G; g += kWarps) {
+    const float2* base = p.part + (long long)n * p.S * p.U + (long long)g * upg;
+    const float m0 = __ldcg(&base[0].x);
+    float s = 0.f;
+    for (int i = lane; i < items; i += 32) {
+      const int k = i / upg;
+      const float cnt = (float)(k == p.S - 1 ? last : p.R) * (float)p.uw;
+      s += cnt * (__ldcg(&base[(long long)k * p.U + (i - k * upg)].x) - m0);
+    }
+    const float mean = m0 + warp_sum(s) / total;
+    float m2 = 0.f;
+    for (int i = lane; i < items; i += 32) {
+      const int k = i / upg;
+      const float cnt = (float)(k == p.S - 1 ? last : p.R) * (float)p.uw;
+      const float2 v = __ldcg(&base[(long long)k * p.U + (i - k * upg)]);
+      const float d = v.x - mean;
+      m2 += v.y + cnt * d * d;
+    }
+    m2 = warp_sum(m2);
+    if (lane == 0)
+      p.stats[(long long)n * p.G + g] = make_float2(mean, 1.f / sqrtf(m2 / total + p.eps));
+  }
+}
+
+// Backward group sums of sample n.
+__device__ void fold_sums(const NormParams& p, int n, int warp, int lane) {
+  const int upg = p.U / p.G;
+  const int items = p.S * upg;
+  const float total = (float)((double)p.P * p.cg);
+  for (int g = warp; g < p.G; g += kWarps) {
+    const float2* base = p.part + (long long)n * p.S * p.U + (long long)g * upg;
+    float a = 0.f, b = 0.f;
+    for (int i = lane; i < items; i += 32) {
+      const int k = i / upg;
+      const float2 v = __ldcg(&base[(long long)k * p.U + (i - k * upg)]);
+      a += v.x;
+      b += v.y;
+    }
+    a = warp_sum(a);
+    b = warp_sum(b);
+    if (lane == 0) p.grp[(long long)n * p.G + g] = make_float2(a / total, b / total);
+  }
+}
+
+template <typename T, int V, bool kBwd>
+__global__ void __launch_bounds__(kThreads, kBwd ? 2 : 3) norm_kernel(const NormParams p) {
+  constexpr bool kFast = sizeof(T) == 2;
+  constexpr int kUnroll = 4;
+  using Vt = Vec<T, V>;
+  __shared__ float2 sh[kThreads * V];
+  __shared__ float2 run[kBwd ? kThreads * V : 1];  // the block's own sums of dz, dz * xhat
+  __shared__ int sh_last, sh_abort;
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int ct = (int)(blockIdx.x % p.CT);
+  const int tx = tid % p.TX, ty = tid / p.TX;
+  const int width = p.TX * V;  // channels of the tile (the last tile may hold fewer)
+  const int tile_c = (p.C - ct * width) < width ? p.C - ct * width : width;
+  Column<V> col;
+  col.c0 = ct * width + tx * V;
+  col.live = ty < p.TY && col.c0 < p.C;
+#pragma unroll
+  for (int e = 0; e < V; ++e) {
+    col.w[e] = col.live && p.weight ? load_param<T>(p.weight, col.c0 + e, p.param_f32) : 1.f;
+    col.b[e] = col.live && p.bias ? load_param<T>(p.bias, col.c0 + e, p.param_f32) : 0.f;
+  }
+  if (tid == 0) sh_abort = 0;
+  if constexpr (kBwd) {
+#pragma unroll
+    for (int e = 0; e < V; ++e) run[tid * V + e] = make_float2(0.f, 0.f);
+  }
+  const T* x = static_cast<const T*>(p.x);
+  const T* dy = static_cast<const T*>(p.dy);
+  T* out = static_cast<T*>(p.out);
+  unsigned* flags = p.count + p.N;
+  __syncthreads();
+
+  const long long steps = (p.chunks + gridDim.x - 1) / gridDim.x;
+  for (long long i = 0; i < steps + p.lag; ++i) {
+    // ---- phase 1: partial sums of chunk t1 ----
+    const long long t1 = i * gridDim.x + blockIdx.x;
+    if (i < steps && t1 < p.chunks) {
+      const Chunk k = chunk_of(p, t1);
+      if (col.live) {
+        const long long base = (k.at + ty) * p.C + col.c0;
+        const long long pitch = (long long)p.TY * p.C;
+        const int mine = (k.rows - ty + p.TY - 1) / p.TY;  // <= 0: none
+        if constexpr (!kBwd) {
+          float s0[V], a1[V], a2[V];
+#pragma unroll
+          for (int e = 0; e < V; ++e) s0[e] = a1[e] = a2[e] = 0.f;
+          if (mine > 0) {
+            const Vt v = *reinterpret_cast<const Vt*>(x + base);
+#pragma unroll
+            for (int e = 0; e < V; ++e) s0[e] = to_f32<T>(v.e[e]);
+          }
+          for (int r = 0; r < mine; r += kUnroll) {
+            Vt v[kUnroll];
+#pragma unroll
+            for (int j = 0; j < kUnroll; ++j)
+              if (r + j < mine) v[j] = *reinterpret_cast<const Vt*>(x + base + (r + j) * pitch);
+#pragma unroll
+            for (int j = 0; j < kUnroll; ++j)
+              if (r + j < mine) {
+#pragma unroll
+                for (int e = 0; e < V; ++e) {
+                  const float d = to_f32<T>(v[j].e[e]) - s0[e];
+                  a1[e] += d;
+                  a2[e] += d * d;
+                }
+              }
+          }
+          const float cnt = (float)(mine > 0 ? mine : 1);
+#pragma unroll
+          for (int e = 0; e < V; ++e) {
+            const float m = a1[e] / cnt;
+            sh[ty * width + tx * V + e] = make_float2(s0[e] + m, fmaxf(a2[e] - a1[e] * m, 0.f));
+          }
+        } else {
+          float mean[V], rstd[V], s1[V], s2[V];
+#pragma unroll
+          for (int e = 0; e < V; ++e) {
+            const float2 st = __ldg(&p.stats[(long long)k.n * p.G + (col.c0 + e) / p.cg]);
+            mean[e] = st.x;
+            rstd[e] = st.y;
+            s1[e] = s2[e] = 0.f;
+          }
+          for (int r = 0; r < mine; r += kUnroll) {
+            Vt v[kUnroll], g[kUnroll];
+#pragma unroll
+            for (int j = 0; j < kUnroll; ++j)
+              if (r + j < mine) {
+                v[j] = *reinterpret_cast<const Vt*>(x + base + (r + j) * pitch);
+                g[j] = *reinterpret_cast<const Vt*>(dy + base + (r + j) * pitch);
+              }
+#pragma unroll
+            for (int j = 0; j < kUnroll; ++j)
+              if (r + j < mine) {
+                float xh[V], sl[V];
+#pragma unroll
+                for (int e = 0; e < V; ++e) {
+                  xh[e] = (to_f32<T>(v[j].e[e]) - mean[e]) * rstd[e];
+                  sl[e] = xh[e] * col.w[e] + col.b[e];
+                }
+                act_slopes<kFast, V>(p.act, sl);
+#pragma unroll
+                for (int e = 0; e < V; ++e) {
+                  const float dz = to_f32<T>(g[j].e[e]) * sl[e];
+                  s1[e] += dz;
+                  s2[e] += dz * xh[e];
+                }
+              }
+          }
+#pragma unroll
+          for (int e = 0; e < V; ++e) {
+            sh[ty * width + tx * V + e] = make_float2(s1[e] * col.w[e], s2[e] * col.w[e]);
+            float2& q = run[tid * V + e];
+            q.x += s1[e];
+            q.y += s2[e];
+          }
+        }
+      }
+      __syncthreads();
+      // units of this tile: groups, or single channels when the channels do
+      // not fit one tile
+      const int units = tile_c / p.uw;
+      const int u0 = ct * width / p.uw;
+      for (int u = warp; u < units; u += kWarps) {
+        float2 r;
+        if constexpr (!kBwd) {
+          r = merge_unit(p, sh, u, width, k.rows, lane);
+        } else {
+          float a = 0.f, b = 0.f;
+          for (int j = lane; j < p.TY * p.uw; j += 32) {
+            const int yy = j / p.uw;
+            const float2 v = sh[yy * width + u * p.uw + (j - yy * p.uw)];
+            a += v.x;
+            b += v.y;
+          }
+          r = make_float2(warp_sum(a), warp_sum(b));
+        }
+        if (lane == 0) p.part[(t1 / p.CT) * p.U + u0 + u] = r;
+      }
+      __syncthreads();
+      if (tid == 0) {
+        __threadfence();
+        sh_last = add_acq_rel(&p.count[k.n]) == (unsigned)(p.S * p.CT - 1);
+      }
+      __syncthreads();
+      if (sh_last) {  // the sample's last chunk: fold its partials
+        if constexpr (kBwd) fold_sums(p, k.n, warp, lane);
+        else fold_stats(p, k.n, warp, lane);
+        __threadfence();
+        __syncthreads();
+        if (tid == 0) store_release(&flags[k.n], 1u);
+      }
+    }
+    // ---- phase 2: write chunk t2 ----
+    const long long t2 = (i - p.lag) * gridDim.x + blockIdx.x;
+    if (i >= p.lag && t2 < p.chunks && (!kBwd || p.out != nullptr)) {
+      const Chunk k = chunk_of(p, t2);
+      if (tid == 0 && load_acquire(&flags[k.n]) == 0u) {
+        const uint64_t began = tc::globaltimer_ns();
+        while (load_acquire(&flags[k.n]) == 0u) {
+          __nanosleep(32);
+          if (tc::globaltimer_ns() - began > kWaitLimitNs) {
+            sh_abort = 1;
+            atomicExch(p.status, 90);
+            break;
+          }
+        }
+      }
+      __syncthreads();
+      if (sh_abort) return;
+      if (col.live) {
+        const long long base = (k.at + ty) * p.C + col.c0;
+        const long long pitch = (long long)p.TY * p.C;
+        const int mine = (k.rows - ty + p.TY - 1) / p.TY;
+        float mean[V], rstd[V], ga[V], gb[V];
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          const long long g = (long long)k.n * p.G + (col.c0 + e) / p.cg;
+          const float2 st = __ldcg(&p.stats[g]);
+          mean[e] = st.x;
+          rstd[e] = st.y;
+          if constexpr (kBwd) {
+            const float2 ab = __ldcg(&p.grp[g]);
+            ga[e] = ab.x;
+            gb[e] = ab.y;
+          }
+        }
+        for (int r = 0; r < mine; r += kUnroll) {
+          Vt v[kUnroll], d[kUnroll];
+#pragma unroll
+          for (int j = 0; j < kUnroll; ++j)
+            if (r + j < mine) {
+              v[j] = *reinterpret_cast<const Vt*>(x + base + (r + j) * pitch);
+              if constexpr (kBwd) d[j] = *reinterpret_cast<const Vt*>(dy + base + (r + j) * pitch);
+            }
+#pragma unroll
+          for (int j = 0; j < kUnroll; ++j)
+            if (r + j < mine) {
+              float xh[V], z[V];
+#pragma unroll
+              for (int e = 0; e < V; ++e) {
+                xh[e] = (to_f32<T>(v[j].e[e]) - mean[e]) * rstd[e];
+                z[e] = xh[e] * col.w[e] + col.b[e];
+              }
+              Vt o;
+              if constexpr (!kBwd) {
+                act_values<kFast, V>(p.act, z);
+#pragma unroll
+                for (int e = 0; e < V; ++e) o.e[e] = from_f32<T>(z[e]);
+              } else {
+                act_slopes<kFast, V>(p.act, z);
+#pragma unroll
+                for (int e = 0; e < V; ++e) {
+                  const float dz = to_f32<T>(d[j].e[e]) * z[e];
+                  o.e[e] = from_f32<T>(rstd[e] * (col.w[e] * dz - ga[e] - xh[e] * gb[e]));
+                }
+              }
+              *reinterpret_cast<Vt*>(out + base + (r + j) * pitch) = o;
+            }
+        }
+      }
+    }
+  }
+  if constexpr (kBwd) {
+    if (p.wsum != nullptr) {
+      __syncthreads();
+      // rows of the block folded in order; one channel a thread at a time
+      for (int c = tid; c < tile_c; c += kThreads) {
+        float2 a = make_float2(0.f, 0.f);
+        for (int yy = 0; yy < p.TY; ++yy) {
+          const float2 v = run[yy * width + c];
+          a.x += v.x;
+          a.y += v.y;
+        }
+        p.wsum[(long long)(blockIdx.x / p.CT) * p.C + ct * width + c] = a;
+      }
+    }
+  }
+}
+
+// dbias and dweight from the blocks' sums: 32 channels a block, its 8 warps
+// share the rows, folded in a fixed order.
+template <typename PT>
+__global__ void __launch_bounds__(256) norm_param_kernel(const float2* __restrict__ sums, int rows,
+                                                         int C, PT* gw, PT* gb) {
+  __shared__ float2 sh[8][32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int c = blockIdx.x * 32 + lane;
+  float2 a = make_float2(0.f, 0.f);
+  if (c < C)
+    for (int r = warp; r < rows; r += 8) {
+      const float2 v = sums[(long long)r * C + c];
+      a.x += v.x;
+      a.y += v.y;
+    }
+  sh[warp][lane] = a;
+  __syncthreads();
+  if (warp == 0 && c < C) {
+    for (int w = 1; w < 8; ++w) {
+      a.x += sh[w][lane].x;
+      a.y += sh[w][lane].y;
+    }
+    if (gb) gb[c] = from_f32<PT>(a.x);
+    if (gw) gw[c] = from_f32<PT>(a.y);
+  }
+}
+
+// ------------------------------------------------------------------ plan ----
+struct Plan {
+  int V, CT, TX, TY, U, uw, R, S, grid, lag;
+  long long chunks;
+  size_t part_off, grp_off, wsum_off, count_off, total;
+};
+
+int gcd_pow2(long long v, int most) {  // largest power of two <= most that divides v
+  int r = most;
+  while (v % r) r >>= 1;
+  return r;
+}
+
+// `align`: the largest power of two (in elements, at most 16 bytes' worth)
+// that divides every tensor's address.
+int make_plan(Plan* q, long long n, long long P, int C, int G, int dt, bool bwd, int align) {
+  const int es = dtype_size(dt);
+  q->V = gcd_pow2(C, align);
+  const int cols = C / q->V;
+  q->CT = (cols + kThreads - 1) / kThreads;
+  q->TX = (cols + q->CT - 1) / q->CT;
+  q->CT = (cols + q->TX - 1) / q->TX;
+  q->TY = kThreads / q->TX;
+  q->U = q->CT == 1 ? G : C;
+  q->uw = q->CT == 1 ? C / G : 1;
+  // Two (backward) or three (forward) blocks an SM are resident by the launch
+  // bounds; the launch checks it.
+  const int most = gencat::num_sms() * (bwd ? 2 : 3) / q->CT * q->CT;
+  // Pixels of a chunk: about 48 KB of x (24 KB in the backward, which moves
+  // twice as much), fewer when that leaves blocks without work, at least two
+  // a thread.
+  const long long row_bytes = (long long)q->TX * q->V * es;
+  const long long big = (bwd ? 24576 : 49152) / row_bytes;
+  long long even = (n * P * q->CT + most - 1) / most;
+  long long r = even < big ? even : big;
+  if (r < 2 * q->TY) r = 2 * q->TY;
+  r = (r + q->TY - 1) / q->TY * q->TY;
+  if (r > P) r = P;
+  q->R = (int)r;
+  const long long s = (P + r - 1) / r;
+  q->chunks = n * s * q->CT;
+  if (q->chunks >= (1LL << 31) || s * q->CT >= (1LL << 31))
+    return set_error(DDPM_ERR_UNSUPPORTED, "group norm: too many chunks");
+  q->S = (int)s;
+  q->grid = (int)(q->chunks < most ? q->chunks : most);
+  q->lag = (int)((s * q->CT - 1 + q->grid - 1) / q->grid);
+  auto up = [](size_t v) { return (v + 255) / 256 * 256; };
+  q->count_off = 0;
+  q->part_off = up((size_t)n * 8);
+  q->grp_off = q->part_off + up((size_t)n * s * q->U * 8);
+  q->wsum_off = q->grp_off + (bwd ? up((size_t)n * G * 8) : 0);
+  q->total = q->wsum_off + (bwd ? up((size_t)(q->grid / q->CT) * C * 8) : 0);
+  return DDPM_OK;
+}
+
+int check_norm(long long n, long long P, int C, int G, int dt, int pdt, int act) {
+  DDPM_CHECK_ARG(n >= 0 && P >= 0 && C >= 1, "sizes must not be negative, channels positive");
+  DDPM_CHECK_ARG(G >= 1 && C % G == 0, "num_groups %d does not divide %d channels", G, C);
+  DDPM_CHECK_ARG(dtype_size(dt) > 0, "unknown dtype code %d", dt);
+  DDPM_CHECK_ARG(pdt == dt || pdt == DDPM_F32, "weight and bias must have x's dtype or be fp32");
+  DDPM_CHECK_ARG(act_known(act), "unknown activation code %d", act);
+  DDPM_CHECK_ARG(n < (1LL << 31) && P < (1LL << 31) && (double)n * P * C < 4e18,
+                 "too many samples or pixels");
+  if (C > kMaxChannels)
+    return set_error(DDPM_ERR_UNSUPPORTED, "group norm supports C <= %d (got %d)", kMaxChannels, C);
+  return DDPM_OK;
+}
+
+template <typename T, int V, bool kBwd>
+int launch_norm(const NormParams& p, const Plan& q, cudaStream_t st) {
+  auto fn = norm_kernel<T, V, kBwd>;
+  if (q.S * q.CT > 1 && q.grid > 1) {
+    // blocks wait for one another: all of them have to be resident
+    NormParams arg = p;
+    void* args[] = {&arg};
+    DDPM_CUDA_TRY(cudaLaunchCooperativeKernel(reinterpret_cast<const void*>(fn), dim3(q.grid),
+                                              dim3(kThreads), args, 0, st));
+  } else {
+    fn<<<q.grid, kThreads, 0, st>>>(p);
+  }
+  DDPM_CHECK_LAUNCH(kBwd ? "group_norm_bwd_kernel" : "group_norm_fwd_kernel");
+  return DDPM_OK;
+}
+
+template <typename T, bool kBwd>
+int dispatch_norm(const NormParams& p, const Plan& q, cudaStream_t st) {
+  if constexpr (sizeof(T) == 2) {
+    if (q.V == 8) return launch_norm<T, 8, kBwd>(p, q, st);
+  }
+  switch (q.V) {
+    case 4: return launch_norm<T, 4, kBwd>(p, q, st);
+    case 2: return launch_norm<T, 2, kBwd>(p, q, st);
+    default: return launch_norm<T, 1, kBwd>(p, q, st);
+  }
+}
+
+int alignment(uintptr_t at, int es) {
+  int v = 16 / es;
+  while (at % ((uintptr_t)v * es)) v >>= 1;
+  return v;
+}
+
+int run_norm(bool bwd, const void* x, const void* dy, const void* w, const void* b, void* out,
+             void* stats, void* gw, void* gb, void* ws, size_t ws_bytes, long long n, long long P,
+             int C, int G, float eps, int act, int dt, int pdt, cudaStream_t st) {
+  int rc = check_norm(n, P, C, G, dt, pdt, act);
+  if (rc) return rc;
+  if (n == 0 || P == 0) return DDPM_OK;
+  DDPM_CHECK_ARG(x && stats && ws && (bwd ? dy != nullptr : out != nullptr), "null pointer");
+  const int es = dtype_size(dt);
+  const uintptr_t at = (uintptr_t)x | (uintptr_t)dy | (uintptr_t)out;
+  DDPM_CHECK_ARG(at % es == 0 && (uintptr_t)stats % 8 == 0 && (uintptr_t)ws % 256 == 0,
+                 "misaligned pointer");
+  Plan q;
+  rc = make_plan(&q, n, P, C, G, dt, bwd, alignment(at, es));
+  if (rc) return rc;
+  if (ws_bytes < q.total)
+    return set_error(DDPM_ERR_WORKSPACE, "group norm workspace: %zu bytes needed, %zu given",
+                     q.total, ws_bytes);
+  uint8_t* base = static_cast<uint8_t*>(ws);
+  NormParams p{};
+  p.x = x;
+  p.dy = dy;
+  p.weight = w;
+  p.bias = b;
+  p.out = out;
+  p.stats = static_cast<float2*>(stats);
+  p.part = reinterpret_cast<float2*>(base + q.part_off);
+  p.grp = reinterpret_cast<float2*>(base + q.grp_off);
+  p.wsum = bwd && (gw || gb) ? reinterpret_cast<float2*>(base + q.wsum_off) : nullptr;
+  p.count = reinterpret_cast<unsigned*>(base + q.count_off);
+  rc = gencat::status_ptr(&p.status);
+  if (rc) return rc;
+  p.P = P;
+  p.N = (int)n;
+  p.C = C;
+  p.G = G;
+  p.cg = C / G;
+  p.R = q.R;
+  p.S = q.S;
+  p.CT = q.CT;
+  p.TX = q.TX;
+  p.TY = q.TY;
+  p.U = q.U;
+  p.uw = q.uw;
+  p.chunks = q.chunks;
+  p.lag = q.lag;
+  p.act = act;
+  p.param_f32 = pdt == DDPM_F32;
+  p.eps = eps;
+  DDPM_CUDA_TRY(cudaMemsetAsync(p.count, 0, (size_t)n * 8, st));
+  switch (dt) {
+    case DDPM_F32:
+      rc = bwd ? dispatch_norm<float, true>(p, q, st) : dispatch_norm<float, false>(p, q, st);
+      break;
+    case DDPM_BF16:
+      rc = bwd ? dispatch_norm<__nv_bfloat16, true>(p, q, st)
+               : dispatch_norm<__nv_bfloat16, false>(p, q, st);
+      break;
+    default:
+      rc = bwd ? dispatch_norm<__half, true>(p, q, st) : dispatch_norm<__half, false>(p, q, st);
+  }
+  if (rc || !p.wsum) return rc;
+  const int blocks = (C + 31) / 32, rows = q.grid / q.CT;
+  switch (pdt) {
+    case DDPM_F32:
+      norm_param_kernel<<<blocks, 256, 0, st>>>(p.wsum, rows, C, (float*)gw, (float*)gb);
+      break;
+    case DDPM_BF16:
+      norm_param_kernel<<<blocks, 256, 0, st>>>(p.wsum, rows, C, (__nv_bfloat16*)gw,
+                                                (__nv_bfloat16*)gb);
+      break;
+    default:
+      norm_param_kernel<<<blocks, 256, 0, st>>>(p.wsum, rows, C, (__half*)gw, (__half*)gb);
+  }
+  DDPM_CHECK_LAUNCH("group_norm_param_kernel");
+  return DDPM_OK;
+}
+
+}  // namespace
+
+// The largest workspace any alignment of the tensors asks for.
+size_t group_norm_workspace_bytes(long long n, long long P, int C, int G, int dt, int bwd) {
+  if (n <= 0 || P <= 0 || C < 1 || G < 1 || C % G || C > kMaxChannels ||
+      dtype_size(dt) == 0 || n >= (1LL << 31) || P >= (1LL << 31))
+    return 0;
+  size_t most = 0;
+  for (int align = 16 / dtype_size(dt); align >= 1; align >>= 1) {
+    Plan q;
+    if (make_plan(&q, n, P, C, G, dt, bwd != 0, align) == DDPM_OK && q.total > most)
+      most = q.total;
+  }
+  return most;
+}
+
+int group_norm_fwd(const void* x, const void* w, const void* b, void* out, void* stats, void* ws,
+                   size_t ws_bytes, long long n, long long P, int C, int G, float eps, int act,
+                   int dt, int pdt, cudaStream_t st) {
+  return run_norm(false, x, nullptr, w, b, out, stats, nullptr, nullptr, ws, ws_bytes, n, P, C, G,
+                  eps, act, dt, pdt, st);
+}
+
+int group_norm_bwd(const void* x, const void* dy, const void* w, const void* b, const void* stats,
+                   void* gx, void* gw, void* gb, void* ws, size_t ws_bytes, long long n,
+                   long long P, int C, int G, int act, int dt, int pdt, cudaStream_t st) {
+  return run_norm(true, x, dy, w, b, gx, const_cast<void*>(stats), gw, gb, ws, ws_bytes, n, P, C,
+                  G, 0.f, act, dt, pdt, st);
+}
+
+}  // namespace ddpm

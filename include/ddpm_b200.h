@@ -368,6 +368,57 @@ DDPM_API int ddpm_gencat_bwd_yw_static(const void* x, const void* y, const void*
                                        void* stream);
 
 /* ---------------------------------------------------------------------------
+ * Channel-last operators around the module (no reference counterpart): group
+ * norm with an activation, matrix product with bias, activation and residual,
+ * dropout. Row-major tensors, channels innermost.
+ * ------------------------------------------------------------------------- */
+
+/* Activations: none, max(z, 0), z * sigmoid(z), z * Phi(z), and the tanh form
+ * of the latter. */
+#define DDPM_ACT_NONE      0
+#define DDPM_ACT_RELU      1
+#define DDPM_ACT_SILU      2
+#define DDPM_ACT_GELU      3
+#define DDPM_ACT_GELU_TANH 4
+
+/*
+ * Group norm with an activation over x [n][pixels][channels]:
+ *   z = (x - mean) * rstd * weight[c] + bias[c],  out = act(z)
+ * with mean and rstd = 1 / sqrt(var + eps) per sample and group of
+ * channels / groups channels over all pixels (biased variance, FP32).
+ * weight and bias [channels] may be NULL (ones, zeros); `param_dtype` is
+ * `dtype` or DDPM_F32. `stats` [n][groups][2] FP32 receives (mean, rstd) and is
+ * what the backward reads. Workspace: `bwd` 0 / 1 selects the entry point;
+ * 256-byte aligned, 0 bytes for an empty x. n or pixels of 0: nothing runs.
+ */
+DDPM_API size_t ddpm_group_norm_workspace_bytes(long long n, long long pixels, int channels,
+                                                int groups, int dtype, int bwd);
+DDPM_API int ddpm_group_norm_fwd(const void* x, const void* weight, const void* bias, void* out,
+                                 void* stats, void* workspace, size_t workspace_bytes,
+                                 long long n, long long pixels, int channels, int groups,
+                                 float eps, int act, int dtype, int param_dtype, void* stream);
+/* Gradients of the above; grad_x, grad_weight, grad_bias may each be NULL.
+ * Sums in a fixed order: the same call gives the same bits. */
+DDPM_API int ddpm_group_norm_bwd(const void* x, const void* grad_out, const void* weight,
+                                 const void* bias, const void* stats, void* grad_x,
+                                 void* grad_weight, void* grad_bias, void* workspace,
+                                 size_t workspace_bytes, long long n, long long pixels,
+                                 int channels, int groups, int act, int dtype, int param_dtype,
+                                 void* stream);
+
+/*
+ * Dropout: out[i] = x[i] / (1 - p) if the value at position offset + i is kept,
+ * else 0; plus residual[i] where `residual` is not NULL. Position q is kept iff
+ * word q % 4 of Philox-4x32-10 with counter (q / 4, 0) and key `seed` is at
+ * least round(p * 2^32). `seed_ptr` (device, 8-byte aligned) replaces `seed`
+ * when not NULL and is read when the kernel runs. The gradient of x is the same
+ * call on the gradient. `out` may be `x` or `residual`.
+ */
+DDPM_API int ddpm_dropout(const void* x, const void* residual, void* out, long long size, double p,
+                          unsigned long long seed, const void* seed_ptr,
+                          unsigned long long offset, int dtype, void* stream);
+
+/* ---------------------------------------------------------------------------
  * Test-only exports (no reference counterpart). They exist for this
  * library's own tests; production callers never need them.
  * ------------------------------------------------------------------------- */

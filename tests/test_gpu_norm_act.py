@@ -1,0 +1,237 @@
+"""group_norm_act against a float64 form: values, gradients, layouts, streams,
+graphs, empty inputs."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from tests import _operators as ops
+
+pytestmark = pytest.mark.gpu
+
+# FP32 roundings on the way to a value: the statistics are folded in three
+# levels (a thread's, a block's, a sample's partial sums; at most 64 + 12 + 20
+# roundings of a running sum each), the value itself takes about ten more.
+STEPS = 128
+
+
+def _case(shape, dtype, groups, seed=0, mean=0.5, channels_last=True):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    c = shape[1]
+    x = torch.randn(shape, generator=g, device="cuda") * 1.5 + mean
+    x = x.to(dtype)
+    if channels_last and x.ndim > 2:
+        x = x.movedim(1, -1).contiguous().movedim(-1, 1)
+    w = (1 + 0.2 * torch.randn(c, generator=g, device="cuda")).to(dtype)
+    b = (0.2 * torch.randn(c, generator=g, device="cuda")).to(dtype)
+    dy = torch.randn(shape, generator=g, device="cuda").to(dtype)
+    return x, w, b, dy
+
+
+def _run(x, groups, w, b, dy, name, eps=1e-5, steps=STEPS):
+    from dynamicconvolutionoperator_b200 import _lib, group_norm_act
+
+    leaves = [t.detach().requires_grad_() for t in (x, w, b) if t is not None]
+    it = iter(leaves)
+    xa = next(it)
+    wa = next(it) if w is not None else None
+    ba = next(it) if b is not None else None
+    out = group_norm_act(xa, groups, wa, ba, eps, activation=name)
+    grads = torch.autograd.grad(out, leaves, dy)
+    with torch.no_grad():
+        again = group_norm_act(x, groups, w, b, eps, activation=name)
+    assert torch.equal(out, again)
+    ref, scale, gref = ops.group_norm(x, groups, w, b, eps, name, dy)
+    ops.check("out", out.detach(), ref, ops.bound(ref, scale, steps, x.dtype))
+    names = ["x"] + ["weight"] * (w is not None) + ["bias"] * (b is not None)
+    want = [gref[0]] + [gref[1]] * (w is not None) + [gref[2]] * (b is not None)
+    for nm, got, (r, s) in zip(names, grads, want):
+        ops.check(nm, got, r, ops.bound(r, s, steps, got.dtype))
+    assert _lib.device_status() == 0
+    return out, grads
+
+
+SHAPES = [
+    ((1, 8, 1), 1),               # one pixel
+    ((1, 64, 16, 16), 8),
+    ((3, 60, 37, 53), 5),         # 4-channel loads, ragged rows
+    ((2, 18, 9, 7), 3),           # 2-channel loads
+    ((5, 7, 11, 3), 7),           # one channel a load, one channel a group
+    ((2, 33, 130), 1),            # one group, odd channels
+    ((4, 96), 4),                 # rows without pixels
+    ((1, 64, 256, 256), 8),       # one sample over the whole grid
+    ((300, 16, 5, 3), 2),         # more samples than blocks
+    ((2, 2304, 6, 5), 9),         # channels of several tiles, groups across them
+    ((2, 515, 17), 5),            # several tiles of single channels
+    ((1, 8, 3, 4, 5), 4),         # three spatial dimensions
+]
+
+
+@pytest.mark.parametrize("dtype", ops.DTYPES)
+@pytest.mark.parametrize("shape,groups", SHAPES)
+def test_matches_float64(shape, groups, dtype):
+    x, w, b, dy = _case(shape, dtype, groups)
+    _run(x, groups, w, b, dy, "silu")
+
+
+@pytest.mark.parametrize("dtype", ops.DTYPES)
+@pytest.mark.parametrize("name", ops.ACTS)
+def test_activations(name, dtype):
+    x, w, b, dy = _case((2, 32, 19, 23), dtype, 4, seed=3)
+    if name == "relu":
+        # away from the kink, where a rounding turns the slope on or off
+        z = ops.group_norm(x, 4, w, b, 1e-5, None)[0]
+        dy = torch.where(z.abs() < 1e-4, torch.zeros_like(dy), dy)
+    _run(x, 4, w, b, dy, name)
+
+
+@pytest.mark.parametrize("dtype", ops.DTYPES)
+def test_large_samples_of_several_waves(dtype):
+    x, w, b, dy = _case((3, 64, 512, 300), dtype, 8, seed=5)
+    _run(x, 8, w, b, dy, "silu", steps=256)  # chunks of up to 768 pixels
+
+
+@pytest.mark.parametrize("mean", [0.0, 300.0])
+def test_mean_far_from_zero(mean):
+    """The variance is summed about values of the data: a mean of 200
+    deviations costs its own digits and no others."""
+    x, w, b, dy = _case((2, 16, 64, 64), torch.float32, 4, mean=mean)
+    _run(x, 4, w, b, dy, None)
+
+
+def test_constant_input_gives_the_bias():
+    from dynamicconvolutionoperator_b200 import group_norm_act
+
+    x = torch.full((2, 8, 5, 5), 3.25, device="cuda").contiguous(memory_format=torch.channels_last)
+    b = torch.arange(8.0, device="cuda")
+    out = group_norm_act(x, 2, torch.ones(8, device="cuda"), b)
+    assert torch.equal(out, b.reshape(1, 8, 1, 1).expand_as(out))
+
+
+def test_without_weight_and_bias_and_mixed_types():
+    x, w, b, dy = _case((2, 24, 10, 9), torch.bfloat16, 4)
+    _run(x, 4, None, None, dy, "silu")
+    _run(x, 4, w, None, dy, "silu")
+    _run(x, 4, None, b.float(), dy, "silu")
+    out, grads = _run(x, 4, w.float(), b.float(), dy, "gelu")
+    assert grads[1].dtype == torch.float32 and out.dtype == torch.bfloat16
+
+
+@pytest.mark.parametrize("shape", [(0, 8, 4, 4), (2, 8, 0, 4)])
+def test_empty(shape):
+    from dynamicconvolutionoperator_b200 import group_norm_act
+
+    x = torch.empty(shape, device="cuda", requires_grad=True)
+    w = torch.ones(8, device="cuda", requires_grad=True)
+    out = group_norm_act(x, 2, w)
+    assert out.shape == x.shape
+    gx, gw = torch.autograd.grad(out, (x, w), torch.empty_like(out))
+    assert gx.shape == x.shape and not gw.any()
+
+
+def test_layouts_agree_and_output_is_channel_last():
+    from dynamicconvolutionoperator_b200 import group_norm_act
+
+    x, w, b, dy = _case((2, 24, 12, 10), torch.float32, 3)
+    want = group_norm_act(x, 3, w, b, activation="silu")
+    assert want.is_contiguous(memory_format=torch.channels_last)
+    assert torch.equal(group_norm_act(x.contiguous(), 3, w, b, activation="silu"), want)
+    wide = torch.zeros(2, 24, 12, 20, device="cuda")
+    wide[..., ::2] = x
+    assert torch.equal(group_norm_act(wide[..., ::2], 3, w, b, activation="silu"), want)
+    # an address that allows no vector loads
+    flat = torch.empty(x.numel() + 1, device="cuda")
+    off = flat[1:].view(2, 12, 10, 24)
+    off.copy_(x.permute(0, 2, 3, 1))
+    got = group_norm_act(off.permute(0, 3, 1, 2), 3, w, b, activation="silu")
+    torch.testing.assert_close(got, want, rtol=1e-5, atol=1e-5)
+
+
+def test_only_the_asked_gradients():
+    from dynamicconvolutionoperator_b200 import group_norm_act
+
+    x, w, b, dy = _case((2, 16, 8, 8), torch.float32, 4)
+    full = _run(x, 4, w, b, dy, "silu")[1]
+    for i in range(3):
+        args = [x, w, b]
+        args[i] = args[i].detach().requires_grad_()
+        got, = torch.autograd.grad(group_norm_act(args[0], 4, args[1], args[2], activation="silu"),
+                                   args[i], dy)
+        assert torch.equal(got, full[i])
+
+
+def test_gradient_matches_differences():
+    x, w, b, dy = _case((1, 4, 3, 5), torch.float32, 2, seed=9)
+    _, grads = _run(x, 2, w, b, dy, "gelu")
+    d = torch.randn(x.shape, generator=torch.Generator().manual_seed(1)).cuda()
+    h = 1e-4
+    up, down = (ops.group_norm(x.double() + s * h * d.double(), 2, w, b, 1e-5, "gelu")[0]
+                for s in (1, -1))
+    want = ((up - down) * dy.double()).sum() / (2 * h)
+    # differences: h^2 times a third derivative of order 10
+    assert abs((grads[0].double() * d).sum() - want) < 1e-5 * (1 + abs(want))
+
+
+def test_same_bits_every_time_and_on_other_streams():
+    from dynamicconvolutionoperator_b200 import group_norm_act
+
+    x, w, b, dy = _case((4, 64, 96, 96), torch.bfloat16, 8)
+    xa = x.detach().requires_grad_()
+    wa = w.detach().requires_grad_()
+
+    def once():
+        out = group_norm_act(xa, 8, wa, b, activation="silu")
+        return (out.detach(), *torch.autograd.grad(out, (xa, wa), dy))
+
+    want = once()
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    results = []
+    for _ in range(5):
+        for s in streams:  # calls of several streams in flight at once
+            with torch.cuda.stream(s):
+                results.append(once())
+    torch.cuda.synchronize()
+    for got in results:
+        assert all(torch.equal(a, e) for a, e in zip(got, want))
+
+
+def test_captured_and_replayed():
+    from dynamicconvolutionoperator_b200 import group_norm_act
+
+    x, w, b, dy = _case((2, 64, 64, 64), torch.bfloat16, 8)
+    xa, wa, ba = (t.clone().requires_grad_() for t in (x, w, b))
+
+    def once():
+        out = group_norm_act(xa, 8, wa, ba, activation="silu")
+        return [out.detach(), *torch.autograd.grad(out, (xa, wa, ba), dy)]
+
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        once()
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = once()
+    for seed in (1, 2):
+        x2 = _case((2, 64, 64, 64), torch.bfloat16, 8, seed=seed)[0]
+        with torch.no_grad():
+            xa.copy_(x2)
+        graph.replay()
+        torch.cuda.synchronize()
+        want = once()
+        assert all(torch.equal(a, e) for a, e in zip(held, want))
+
+
+def test_nan_stays_in_its_group():
+    from dynamicconvolutionoperator_b200 import group_norm_act
+
+    x, w, b, _ = _case((2, 8, 6, 6), torch.float32, 2)
+    want = group_norm_act(x, 2, w, b, activation="relu")
+    x[0, 1, 2, 3] = float("nan")
+    x[1, 6, 0, 0] = float("inf")
+    got = group_norm_act(x, 2, w, b, activation="relu")
+    assert got[0, :4].isnan().all() and got[1, 4:].isnan().all()
+    assert torch.equal(got[0, 4:], want[0, 4:]) and torch.equal(got[1, :4], want[1, :4])

@@ -1,0 +1,104 @@
+"""Argument checks of the channel-last operators (CPU: nothing is launched)."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from dynamicconvolutionoperator_b200 import _lib, dropout, group_norm_act
+from tests import _operators as ops
+
+
+def test_philox_known_answers():
+    """The published test vectors of Philox-4x32-10 (Random123 ``kat_vectors``)."""
+    assert ops.philox_words([0] * 4, [0] * 2) == [0x6627E8D5, 0xE169C58D, 0xBC57AC4C, 0x9B00DBD8]
+    assert ops.philox_words([0xFFFFFFFF] * 4, [0xFFFFFFFF] * 2) == [
+        0x408F276D, 0x41C83B0E, 0xA20BC7C6, 0x6D5451FD]
+
+
+@pytest.mark.parametrize("call", [
+    lambda x: group_norm_act(x, 2),
+    lambda x: dropout(x, 0.5, 1),
+])
+def test_cpu_tensors_fail_loudly(call):
+    with pytest.raises(RuntimeError, match="CUDA"):
+        call(torch.randn(2, 4, 3, 3))
+
+
+@pytest.mark.parametrize("kwargs,match", [
+    (dict(num_groups=3), "num_groups"),
+    (dict(num_groups=0), "num_groups"),
+    (dict(num_groups=2, activation="tanh"), "activation"),
+    (dict(num_groups=2, activation=["relu"]), "activation"),
+    (dict(num_groups=2, eps=-1.0), "eps"),
+    (dict(num_groups=2, eps=float("nan")), "eps"),
+    (dict(num_groups=2, weight=torch.ones(3)), "weight must have shape"),
+    (dict(num_groups=2, bias=torch.ones(1, 4)), "bias must have shape"),
+    (dict(num_groups=2, weight=torch.ones(4, dtype=torch.float64)), "dtype"),
+    (dict(num_groups=2, weight=torch.ones(4, dtype=torch.bfloat16)), "dtype"),
+])
+def test_group_norm_refusals(kwargs, match):
+    with pytest.raises(ValueError, match=match):
+        group_norm_act(torch.randn(2, 4, 3, 3), **kwargs)
+
+
+def test_group_norm_refuses_one_dimension_and_mixed_parameters():
+    with pytest.raises(ValueError, match="two dimensions"):
+        group_norm_act(torch.randn(4), 1)
+    with pytest.raises(ValueError, match="one dtype"):
+        group_norm_act(torch.randn(2, 4).bfloat16(), 1, torch.ones(4), torch.ones(4).bfloat16())
+
+
+@pytest.mark.parametrize("kwargs,match", [
+    (dict(p=-0.1, seed=1), "between 0 and 1"),
+    (dict(p=1.5, seed=1), "between 0 and 1"),
+    (dict(p=float("nan"), seed=1), "between 0 and 1"),
+    (dict(p=0.5, seed=1 << 64), "64 bits"),
+    (dict(p=0.5, seed=torch.tensor([1, 2])), "one int64"),
+    (dict(p=0.5, seed=torch.tensor([1], dtype=torch.int32)), "one int64"),
+    (dict(p=0.5, seed=1, offset=-1), "offset"),
+    (dict(p=0.5, seed=1, offset=1 << 64), "offset"),
+    (dict(p=0.5, seed=1, residual=torch.zeros(5)), "residual"),
+    (dict(p=0.5, seed=1, residual=torch.zeros(4, dtype=torch.float16)), "residual"),
+])
+def test_dropout_refusals(kwargs, match):
+    with pytest.raises(ValueError, match=match):
+        dropout(torch.randn(4), **kwargs)
+
+
+def test_abi_argument_errors_without_gpu():
+    lib = _lib.load()
+
+    def norm(n=1, px=4, c=8, g=2, act=0, dt=0, pdt=0, x=16, ws=256, nbytes=1 << 20):
+        return lib.ddpm_group_norm_fwd(x, None, None, 16, 16, ws, nbytes, n, px, c, g, 1e-5, act,
+                                       dt, pdt, None)
+
+    assert norm(g=3) == -1 and b"num_groups" in lib.ddpm_last_error()
+    assert norm(dt=7) == -1 and b"dtype" in lib.ddpm_last_error()
+    assert norm(act=5) == -1 and b"activation" in lib.ddpm_last_error()
+    assert norm(dt=1, pdt=2) == -1 and b"fp32" in lib.ddpm_last_error()
+    assert norm(x=None) == -1 and b"null" in lib.ddpm_last_error()
+    assert norm(x=18) == -1 and b"misaligned" in lib.ddpm_last_error()
+    assert norm(ws=128) == -1 and b"misaligned" in lib.ddpm_last_error()
+    assert norm(nbytes=16) == -4 and b"workspace" in lib.ddpm_last_error()
+    assert norm(c=1 << 17) == -2
+    assert norm(n=0) == 0 and norm(px=0) == 0
+
+    def drop(n=8, p=0.5, dt=0, x=16, seed=None):
+        return lib.ddpm_dropout(x, None, 16, n, p, 1, seed, 0, dt, None)
+
+    assert drop(p=2.0) == -1 and b"between" in lib.ddpm_last_error()
+    assert drop(dt=9) == -1 and b"dtype" in lib.ddpm_last_error()
+    assert drop(x=None) == -1 and b"null" in lib.ddpm_last_error()
+    assert drop(x=17) == -1 and b"misaligned" in lib.ddpm_last_error()
+    assert drop(seed=4) == -1 and b"misaligned" in lib.ddpm_last_error()
+    assert drop(n=-1) == -1 and drop(n=0) == 0
+
+
+@pytest.mark.parametrize("bwd", [0, 1])
+def test_group_norm_workspace_covers_every_alignment(bwd):
+    lib = _lib.load()
+    size = lib.ddpm_group_norm_workspace_bytes
+    assert size(0, 4, 8, 2, 0, bwd) == 0 and size(4, 4, 9, 2, 0, bwd) == 0
+    for c, g in ((64, 8), (60, 5), (515, 5), (4096, 32)):
+        assert size(3, 1000, c, g, 1, bwd) > 0
