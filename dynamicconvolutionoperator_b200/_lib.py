@@ -124,6 +124,17 @@ _SIGNATURES: dict[str, tuple[object, list[object]]] = {
         _c_int,
         [_c_ptr] * 9 + [_c_size] + [_c_i64] * 2 + [_c_int] * 5 + [_c_ptr],
     ),
+    "ddpm_linear_workspace_bytes": (
+        _c_size, [_c_i64, _c_int, _c_int, _c_i64] + [_c_int] * 4
+    ),
+    "ddpm_linear_fwd": (
+        _c_int,
+        [_c_ptr, _c_i64] + [_c_ptr] * 5 + [_c_size, _c_i64] + [_c_int] * 4 + [_c_ptr],
+    ),
+    "ddpm_linear_bwd": (
+        _c_int,
+        [_c_ptr, _c_i64] + [_c_ptr] * 7 + [_c_size, _c_i64] + [_c_int] * 4 + [_c_ptr],
+    ),
     "ddpm_dropout": (
         _c_int,
         [_c_ptr] * 3 + [_c_i64, ctypes.c_double, _c_u64, _c_ptr, _c_u64, _c_int, _c_ptr],

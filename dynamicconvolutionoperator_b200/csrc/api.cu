@@ -99,6 +99,14 @@ int group_norm_bwd(const void* x, const void* dy, const void* w, const void* b, 
 int dropout(const void* x, const void* residual, void* out, long long n, double p,
             unsigned long long seed, const void* seed_ptr, unsigned long long offset, int dt,
             cudaStream_t st);
+size_t linear_workspace_bytes(long long m, int n, int k, long long ldx, int act, int dt, int bwd,
+                              int aligned);
+int linear_fwd(const void* x, long long ldx, const void* w, const void* bias, const void* res,
+               void* out, void* ws, size_t ws_bytes, long long m, int n, int k, int act, int dt,
+               cudaStream_t st);
+int linear_bwd(const void* x, long long ldx, const void* w, const void* bias, const void* dy,
+               void* gx, void* gw, void* gb, void* ws, size_t ws_bytes, long long m, int n, int k,
+               int act, int dt, cudaStream_t st);
 }  // namespace ddpm
 
 extern "C" {
@@ -390,6 +398,28 @@ int ddpm_dropout(const void* x, const void* residual, void* out, long long size,
   ddpm::clear_error();
   return ddpm::dropout(x, residual, out, size, p, seed, seed_ptr, offset, dtype,
                        static_cast<cudaStream_t>(stream));
+}
+
+size_t ddpm_linear_workspace_bytes(long long m, int n, int k, long long ldx, int act, int dtype,
+                                   int bwd, int aligned) {
+  return ddpm::linear_workspace_bytes(m, n, k, ldx, act, dtype, bwd, aligned);
+}
+
+int ddpm_linear_fwd(const void* x, long long ldx, const void* weight, const void* bias,
+                    const void* residual, void* out, void* workspace, size_t workspace_bytes,
+                    long long m, int n, int k, int act, int dtype, void* stream) {
+  ddpm::clear_error();
+  return ddpm::linear_fwd(x, ldx, weight, bias, residual, out, workspace, workspace_bytes, m, n, k,
+                          act, dtype, static_cast<cudaStream_t>(stream));
+}
+
+int ddpm_linear_bwd(const void* x, long long ldx, const void* weight, const void* bias,
+                    const void* grad_out, void* grad_x, void* grad_weight, void* grad_bias,
+                    void* workspace, size_t workspace_bytes, long long m, int n, int k, int act,
+                    int dtype, void* stream) {
+  ddpm::clear_error();
+  return ddpm::linear_bwd(x, ldx, weight, bias, grad_out, grad_x, grad_weight, grad_bias, workspace,
+                          workspace_bytes, m, n, k, act, dtype, static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

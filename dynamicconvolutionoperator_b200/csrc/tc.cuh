@@ -148,6 +148,26 @@ __device__ __forceinline__ void tma_load_4d(void* dst, const void* tmap, int c0,
       : "memory");
 }
 
+// 3-D variant of tma_load_4d, and the store of a shared-memory box (a bulk
+// async-group of the calling thread; coordinates must not be negative, what
+// lies outside the tensor is not written).
+__device__ __forceinline__ void tma_load_3d(void* dst, const void* tmap, int c0, int c1, int c2,
+                                            uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(tmap)), "r"(c0), "r"(c1), "r"(c2), "r"(smem_u32(bar))
+      : "memory");
+}
+__device__ __forceinline__ void tma_store_3d(const void* tmap, const void* src, int c0, int c1,
+                                             int c2) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(
+          reinterpret_cast<uint64_t>(tmap)),
+      "r"(smem_u32(src)), "r"(c0), "r"(c1), "r"(c2)
+      : "memory");
+}
+
 // Element-wise add of a shared-memory box into a global tensor (TMA reduction,
 // 4-D tensor map), as a bulk async-group of the calling thread; coordinates
 // must not be negative.
@@ -165,6 +185,11 @@ __device__ __forceinline__ void bulk_commit() {
 // Wait until every bulk async-group of this thread has read its source.
 __device__ __forceinline__ void bulk_wait_read_all() {
   asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+}
+// Wait until all but the newest N bulk async-groups of this thread have read
+// their sources.
+template <int N> __device__ __forceinline__ void bulk_wait_read() {
+  asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory");
 }
 // Wait until every bulk async-group of this thread has completed.
 __device__ __forceinline__ void bulk_wait_all() {
@@ -229,6 +254,20 @@ __device__ __forceinline__ uint64_t smem_desc_sw128(uint32_t saddr) {
   d |= (uint64_t)(1024 >> 4) << 32;  // SBO
   d |= (uint64_t)1 << 46;            // descriptor version for sm_100
   d |= (uint64_t)2 << 61;            // layout type: SWIZZLE_128B
+  return d;
+}
+
+// Descriptor of an MN-major operand in the 128-byte swizzled form written by a
+// TMA copy with SWIZZLE_128B: one 128-byte row per K index (64 16-bit M/N
+// elements), 8-row groups 1024 bytes apart (SBO), blocks of 64 M/N elements
+// `mn_stride` bytes apart (LBO). A K step of 16 advances the start by 2048.
+__device__ __forceinline__ uint64_t smem_desc_sw128_mn(uint32_t saddr, uint32_t mn_stride) {
+  uint64_t d = 0;
+  d |= (uint64_t)((saddr >> 4) & 0x3FFFu);
+  d |= (uint64_t)((mn_stride >> 4) & 0x3FFFu) << 16;  // LBO
+  d |= (uint64_t)(1024 >> 4) << 32;                   // SBO
+  d |= (uint64_t)1 << 46;
+  d |= (uint64_t)2 << 61;
   return d;
 }
 

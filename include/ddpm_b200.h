@@ -407,6 +407,31 @@ DDPM_API int ddpm_group_norm_bwd(const void* x, const void* grad_out, const void
                                  void* stream);
 
 /*
+ * Matrix product with an epilogue: out = act(x weight^T + bias) + residual for
+ * x [m][k] (rows `ldx` >= k elements apart), weight [n][k], bias [n] or NULL,
+ * residual [m][n] or NULL, out [m][n]; one dtype, FP32 accumulation, one
+ * rounding. FP32 data is multiplied as three bf16 parts with the six products
+ * above 2^-24 (an infinity in it gives a NaN). Workspace: 256-byte aligned, at
+ * least the returned bytes; `bwd` selects the entry point, `aligned` says that
+ * every pointer of the call is on a 16-byte boundary (0 is always enough).
+ * `out` must not overlap the inputs, except that it may be `residual`.
+ */
+DDPM_API size_t ddpm_linear_workspace_bytes(long long m, int n, int k, long long ldx, int act,
+                                            int dtype, int bwd, int aligned);
+DDPM_API int ddpm_linear_fwd(const void* x, long long ldx, const void* weight, const void* bias,
+                             const void* residual, void* out, void* workspace,
+                             size_t workspace_bytes, long long m, int n, int k, int act, int dtype,
+                             void* stream);
+/* Gradients for grad_out [m][n]; grad_x [m][k], grad_weight [n][k] and
+ * grad_bias [n] may each be NULL (the residual's gradient is grad_out). With an
+ * activation its argument is computed again from x and weight. Sums in a fixed
+ * order: the same call gives the same bits. */
+DDPM_API int ddpm_linear_bwd(const void* x, long long ldx, const void* weight, const void* bias,
+                             const void* grad_out, void* grad_x, void* grad_weight,
+                             void* grad_bias, void* workspace, size_t workspace_bytes,
+                             long long m, int n, int k, int act, int dtype, void* stream);
+
+/*
  * Dropout: out[i] = x[i] / (1 - p) if the value at position offset + i is kept,
  * else 0; plus residual[i] where `residual` is not NULL. Position q is kept iff
  * word q % 4 of Philox-4x32-10 with counter (q / 4, 0) and key `seed` is at

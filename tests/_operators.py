@@ -115,3 +115,33 @@ def kept(size: int, p: float, seed: int, offset: int) -> torch.Tensor:
         words += philox(at % 2 ** 62, seed)
         at += 1
     return torch.tensor([w >= least for w in words[offset % 4:][:size]], dtype=torch.bool)
+
+
+def linear(x, w, b, name, res, dy=None):
+    """(out, scale of out, z's scale, gradients with their scales) in float64
+    for x [m, k], w [n, k]. A gradient's scales: (terms rounded in FP32, terms
+    holding dz rounded to the data's type)."""
+    xd, wd = x.double(), w.double()
+    z = xd @ wd.t()
+    zscale = xd.abs() @ wd.abs().t()
+    if b is not None:
+        z = z + b.double()
+        zscale = zscale + b.double().abs()
+    out = act(z, name)
+    # |act'| <= 1.13 for every activation here
+    scale = 1.2 * zscale + out.abs()
+    if res is not None:
+        out = out + res.double()
+        scale = scale + res.double().abs()
+    if dy is None:
+        return out, scale, zscale, None
+    g = dy.double()
+    s = slope(z, name)
+    dz = g * s
+    wobble = 0 if name in (None, "relu") else 1.2 * zscale  # |act''| <= 1.2
+    dzs = g.abs() * (s.abs() + wobble)
+    return out, scale, zscale, {
+        "x": (dz @ wd, dzs @ wd.abs(), dz.abs() @ wd.abs()),
+        "weight": (dz.t() @ xd, dzs.t() @ xd.abs(), dz.abs().t() @ xd.abs()),
+        "bias": (dz.sum(0), dzs.sum(0), torch.zeros_like(dz.sum(0))),
+    }

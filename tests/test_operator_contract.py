@@ -5,7 +5,7 @@ from __future__ import annotations
 import pytest
 import torch
 
-from dynamicconvolutionoperator_b200 import _lib, dropout, group_norm_act
+from dynamicconvolutionoperator_b200 import _lib, dropout, group_norm_act, linear_act
 from tests import _operators as ops
 
 
@@ -19,6 +19,7 @@ def test_philox_known_answers():
 @pytest.mark.parametrize("call", [
     lambda x: group_norm_act(x, 2),
     lambda x: dropout(x, 0.5, 1),
+    lambda x: linear_act(x, torch.randn(5, 3)),
 ])
 def test_cpu_tensors_fail_loudly(call):
     with pytest.raises(RuntimeError, match="CUDA"):
@@ -64,6 +65,50 @@ def test_group_norm_refuses_one_dimension_and_mixed_parameters():
 def test_dropout_refusals(kwargs, match):
     with pytest.raises(ValueError, match=match):
         dropout(torch.randn(4), **kwargs)
+
+
+@pytest.mark.parametrize("kwargs,match", [
+    (dict(weight=torch.ones(5, 4)), "weight must be"),
+    (dict(weight=torch.ones(3)), "weight must be"),
+    (dict(weight=torch.ones(5, 3, 3, 3)), "weight must be"),
+    (dict(weight=torch.ones(0, 3)), "empty"),
+    (dict(weight=torch.ones(5, 3), bias=torch.ones(3)), "bias must have shape"),
+    (dict(weight=torch.ones(5, 3), residual=torch.ones(2, 3)), "residual must have shape"),
+    (dict(weight=torch.ones(5, 3), residual=torch.ones(5)), "residual must have shape"),
+    (dict(weight=torch.ones(5, 3).half()), "one dtype"),
+    (dict(weight=torch.ones(5, 3), bias=torch.ones(5).half()), "one dtype"),
+    (dict(weight=torch.ones(5, 3), activation="swish"), "activation"),
+])
+def test_linear_refusals(kwargs, match):
+    with pytest.raises(ValueError, match=match):
+        linear_act(torch.randn(2, 3), **kwargs)
+
+
+def test_linear_abi_argument_errors_without_gpu():
+    lib = _lib.load()
+
+    def fwd(m=64, n=8, k=8, ldx=8, act=0, dt=1, x=16, ws=256, nbytes=1 << 20):
+        return lib.ddpm_linear_fwd(x, ldx, 16, None, None, 16, ws, nbytes, m, n, k, act, dt, None)
+
+    assert fwd(ldx=7) == -1 and b"stride" in lib.ddpm_last_error()
+    assert fwd(n=0) == -1 and fwd(k=0) == -1 and fwd(m=-1) == -1
+    assert fwd(act=9) == -1 and b"activation" in lib.ddpm_last_error()
+    assert fwd(dt=3) == -1 and b"dtype" in lib.ddpm_last_error()
+    assert fwd(x=None) == -1 and b"null" in lib.ddpm_last_error()
+    assert fwd(x=17) == -1 and b"misaligned" in lib.ddpm_last_error()
+    assert fwd(ws=8) == -1 and b"workspace" in lib.ddpm_last_error()
+    assert fwd(dt=0, nbytes=64) == -4 and b"workspace" in lib.ddpm_last_error()
+    assert fwd(x=18, nbytes=64) == -4  # rows that TMA cannot address are copied
+    assert fwd(m=1 << 33) == -2
+    assert fwd(m=0) == 0
+    size = lib.ddpm_linear_workspace_bytes
+    assert size(64, 8, 8, 8, 0, 1, 0, 1) == 0 and size(64, 8, 8, 8, 0, 1, 0, 0) > 0
+    assert size(64, 8, 8, 7, 0, 1, 0, 1) == 0  # refused shapes
+    for bwd in (0, 1):
+        for act in (0, 2):
+            for dt in (0, 1, 2):
+                assert size(1999, 333, 200, 200, act, dt, bwd, 0) >= size(
+                    1999, 333, 200, 200, act, dt, bwd, 1)
 
 
 def test_abi_argument_errors_without_gpu():
