@@ -179,22 +179,27 @@ def load() -> ctypes.CDLL:
 
 def call(name: str, *args) -> None:
     """Invoke an entry point; a non-zero return raises RuntimeError with its message."""
-    lib = load()
+    lib = _lib or load()
     rc = getattr(lib, name)(*args)
     if rc != 0:
         msg = lib.ddpm_last_error().decode(errors="replace")
         raise RuntimeError(f"{name} failed (code {rc}): {msg}")
 
 
+# torch's current stream without the stream object around it
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
 def call_on(device: torch.device, name: str, *args) -> None:
     """``call`` with ``device`` current and torch's current stream on it as the
     last argument."""
-    stream = torch.cuda.current_stream(device).cuda_stream
-    if torch.cuda.current_device() == device.index:
-        call(name, *args, stream)
+    index = device.index
+    if torch.cuda.current_device() == index:
+        call(name, *args, _raw_stream(index))
     else:
-        with torch.cuda.device(device):
-            call(name, *args, stream)
+        with torch.cuda.device(index):
+            call(name, *args, _raw_stream(index))
 
 
 def device_status(reset: bool = True) -> int:

@@ -8,6 +8,8 @@ is computed again by the same product.
 
 from __future__ import annotations
 
+import functools
+
 import torch
 from torch.autograd.function import once_differentiable
 
@@ -20,6 +22,8 @@ from ._norm import _ptr, activation_code
 def _rows(x: torch.Tensor) -> torch.Tensor:
     """``x`` [..., k] as [m, k] with unit column stride (a view where the
     leading dimensions fold into rows of one stride, else a copy)."""
+    if x.ndim == 2 and x.is_contiguous():
+        return x
     k = x.shape[-1]
     flat = x if x.ndim == 2 else x.reshape(-1, k)
     if flat.stride(1) == 1 or k == 1:
@@ -28,26 +32,37 @@ def _rows(x: torch.Tensor) -> torch.Tensor:
     return flat.contiguous()
 
 
+def _matrix(t: torch.Tensor, shape: tuple[int, int]) -> torch.Tensor:
+    """``t`` as a contiguous matrix."""
+    return (t if t.ndim == 2 else t.reshape(shape)).contiguous()
+
+
 def _row_stride(flat: torch.Tensor) -> int:
     return flat.stride(0) if flat.shape[0] > 1 else flat.shape[1]
 
 
-def _workspace(flat, n, act, bwd, tensors):
-    m, k = flat.shape
-    aligned = not any(t is not None and t.data_ptr() % 16 for t in tensors)
-    nbytes = int(_lib.load().ddpm_linear_workspace_bytes(
-        m, n, k, _row_stride(flat), act, _lib.dtype_code(flat.dtype), bwd, aligned))
-    return torch.empty(nbytes, dtype=torch.uint8, device=flat.device), nbytes
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(m, n, k, ld, act, code, bwd, aligned, device) -> int:
+    """The plan's size on ``device`` (it depends on the number of SMs)."""
+    with torch.cuda.device(device):
+        return int(_lib.load().ddpm_linear_workspace_bytes(m, n, k, ld, act, code, bwd, aligned))
+
+
+def _workspace(nbytes: int, device: torch.device) -> torch.Tensor | None:
+    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
 
 
 def _forward(flat, w, b, res, act):
     m, k = flat.shape
     n = w.shape[0]
-    out = torch.empty((m, n), dtype=flat.dtype, device=flat.device)
-    ws, nbytes = _workspace(flat, n, act, 0, (flat, w, b, res, out))
-    _lib.call_on(flat.device, "ddpm_linear_fwd", flat.data_ptr(), _row_stride(flat), w.data_ptr(),
-                 _ptr(b), _ptr(res), out.data_ptr(), ws.data_ptr(), nbytes, m, n, k, act,
-                 _lib.dtype_code(flat.dtype))
+    dev, code, ld = flat.device, _lib.dtype_code(flat.dtype), _row_stride(flat)
+    out = torch.empty((m, n), dtype=flat.dtype, device=dev)
+    px, pw, pb, pr, po = flat.data_ptr(), w.data_ptr(), _ptr(b), _ptr(res), out.data_ptr()
+    aligned = (px | pw | (pb or 0) | (pr or 0) | po) % 16 == 0
+    nbytes = _workspace_bytes(m, n, k, ld, act, code, 0, aligned, dev)
+    ws = _workspace(nbytes, dev)
+    _lib.call_on(dev, "ddpm_linear_fwd", px, ld, pw, pb, pr, po, _ptr(ws), nbytes, m, n, k, act,
+                 code)
     return out
 
 
@@ -56,14 +71,14 @@ class _LinearAct(torch.autograd.Function):
     def forward(ctx, x, weight, bias, residual, act):
         flat = _rows(x)
         n = weight.shape[0]
-        w = weight.reshape(n, -1).contiguous()
+        w = _matrix(weight, (n, flat.shape[1]))
         b = bias.contiguous() if bias is not None else None
-        res = residual.reshape(-1, n).contiguous() if residual is not None else None
+        res = _matrix(residual, (-1, n)) if residual is not None else None
         out = _forward(flat, w, b, res, act)
         ctx.save_for_backward(flat, w, b if act else None)
         ctx.params = (weight, bias)  # gradient buffers are looked up by identity
         ctx.act, ctx.shape = act, x.shape
-        return out.reshape(*x.shape[:-1], n)
+        return out if x.ndim == 2 else out.reshape(*x.shape[:-1], n)
 
     @staticmethod
     @once_differentiable
@@ -83,11 +98,14 @@ class _LinearAct(torch.autograd.Function):
                 if g is not None:
                     g.zero_()
         elif gx is not None or need_w or need_b:
-            g = grad_out.reshape(m, n).contiguous()
-            ws, nbytes = _workspace(flat, n, ctx.act, 1, (flat, w, b, g, gx, gw, gb))
-            _lib.call_on(dev, "ddpm_linear_bwd", flat.data_ptr(), _row_stride(flat), w.data_ptr(),
-                         _ptr(b), g.data_ptr(), _ptr(gx), _ptr(gw), _ptr(gb), ws.data_ptr(),
-                         nbytes, m, n, k, ctx.act, _lib.dtype_code(dt))
+            g = _matrix(grad_out, (m, n))
+            code, ld = _lib.dtype_code(dt), _row_stride(flat)
+            ptrs = [_ptr(t) for t in (flat, w, b, g, gx, gw, gb)]
+            aligned = not any(q and q % 16 for q in ptrs)
+            nbytes = _workspace_bytes(m, n, k, ld, ctx.act, code, 1, aligned, dev)
+            ws = _workspace(nbytes, dev)
+            _lib.call_on(dev, "ddpm_linear_bwd", ptrs[0], ld, *ptrs[1:], _ptr(ws), nbytes, m, n, k,
+                         ctx.act, code)
         if gx is not None:
             gx = gx.reshape(ctx.shape)
         return gx, gw, gb, grad_out if ctx.needs_input_grad[3] else None, None
@@ -133,10 +151,11 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None 
     _lib.dtype_code(x.dtype)
     if torch.is_grad_enabled() and (x.requires_grad or any(t.requires_grad for t in given)):
         return _LinearAct.apply(x, weight, bias, residual, act)
-    out = _forward(_rows(x), weight.reshape(n, -1).contiguous(),
+    flat = _rows(x)
+    out = _forward(flat, _matrix(weight, (n, flat.shape[1])),
                    bias.contiguous() if bias is not None else None,
-                   residual.reshape(-1, n).contiguous() if residual is not None else None, act)
-    return out.reshape(*x.shape[:-1], n)
+                   _matrix(residual, (-1, n)) if residual is not None else None, act)
+    return out if x.ndim == 2 else out.reshape(*x.shape[:-1], n)
 
 
 __all__ = ["linear_act"]

@@ -8,6 +8,7 @@
 // PackLayout): forward chunks, dX chunks and the transposed dY groups. Each
 // 16-byte row holds 8 consecutive K-dimension values; fp32 weights are stored
 // as a bf16 hi image followed by a bf16 lo (residual) image.
+#include <atomic>
 #include <mutex>
 
 #include <cudaTypedefs.h>
@@ -51,7 +52,14 @@ int check_shape_bwd(int n, int c, int h, int w, int ks, int d0, int d1, int d2, 
 }
 
 int status_ptr(int** out) {
+  // the address on each device, looked up once
+  static std::atomic<int*> cache[64];
+  int dev = 0;
+  DDPM_CUDA_TRY(cudaGetDevice(&dev));
+  if (dev >= 0 && dev < 64 && (*out = cache[dev].load(std::memory_order_relaxed)) != nullptr)
+    return DDPM_OK;
   DDPM_CUDA_TRY(cudaGetSymbolAddress(reinterpret_cast<void**>(out), g_gencat_status));
+  if (dev >= 0 && dev < 64) cache[dev].store(*out, std::memory_order_relaxed);
   return DDPM_OK;
 }
 

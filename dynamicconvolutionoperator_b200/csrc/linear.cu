@@ -12,13 +12,14 @@
 // k: weight in dx, both operands in dweight); the layout is a matter of TMA
 // boxes and descriptors, so nothing is transposed in memory.
 //
-//   tile      128 rows x BN (64, 128 or 256) columns, K in steps of 64
+//   tile      128 rows x BN (64, 128 or 256) columns, K in steps of 64; where
+//             there is work for all, a pair of blocks shares 256 rows
 //   operands  TMA, 128-byte swizzle, a ring of stages; out-of-range rows,
 //             columns and k are zero filled, which covers every ragged size
 //   issue     tcgen05.mma of 128 x BN x 16 by one thread; two TMEM
 //             accumulators, so the epilogue of a tile overlaps the next one
 //   epilogue  eight warps (lane = row, two column halves): TMEM -> registers,
-//             bias, activation, residual -> 64-byte x 32-row boxes in shared
+//             bias, activation, residual -> 128-byte x 32-row boxes in shared
 //             memory -> TMA store. The residual (or dy) comes through the same
 //             boxes by TMA, several boxes ahead.
 //
@@ -39,6 +40,7 @@
 //
 // Up to eight rows, forward: a dot-product kernel reads the weight once at the
 // memory's rate; a tensor-core tile would be 15/16 empty and its K loop serial.
+#include <atomic>
 #include <type_traits>
 
 #include "act.cuh"
@@ -60,7 +62,6 @@ constexpr int kBM = 128, kBK = 64;
 constexpr int kEpiWarps = 8;
 constexpr int kFirstEpi = 4;  // warps 0-3: TMA, MMA, TMEM allocation, none
 constexpr int kThreads = 32 * (kFirstEpi + kEpiWarps);
-constexpr int kBoxBytes = 2048;  // 32 rows x 64 bytes
 constexpr int kMaxStages = 8, kMaxBufs = 8;
 constexpr uint64_t kWaitNs = 2000000000ull;
 constexpr int kGemvRows = 8;
@@ -81,15 +82,19 @@ struct GemmParams {
   int* status;
 };
 
+// A box of the epilogue: 32 rows x 128 bytes (64 where half a tile is no wider).
+__host__ __device__ constexpr int box_row(int bn, int es) { return bn / 2 * es < 128 ? 64 : 128; }
+
 struct SmemLayout {
-  uint32_t stage, ring, boxes, total;
+  uint32_t stage, boxes, bias, total;
 };
-__host__ __device__ inline SmemLayout smem_layout(int parts, int bn, int stages, int nbuf) {
+__host__ __device__ inline SmemLayout smem_layout(int cg, int parts, int bn, int row, int stages,
+                                                  int nbuf) {
   SmemLayout L;
-  L.stage = (uint32_t)parts * (kBM + bn) * kBK * 2;
-  L.ring = 0;
+  L.stage = (uint32_t)parts * (kBM + bn / cg) * kBK * 2;
   L.boxes = L.stage * stages;
-  L.total = L.boxes + kEpiWarps * nbuf * kBoxBytes + 1024;  // + alignment of the base
+  L.bias = L.boxes + kEpiWarps * nbuf * 32 * row;
+  L.total = L.bias + kEpiWarps * (bn / 2) * 4 + 1024;  // + alignment of the base
   return L;
 }
 
@@ -98,15 +103,132 @@ __device__ __forceinline__ void give_up(volatile int* abort_flag, int* status, i
   atomicCAS(status, 0, code);
 }
 
-// Sums over the warp's rows: lane l (mod C) returns the sum of v[l] over the
-// 32 lanes. Halves the columns a lane holds at each exchange.
-template <int C> __device__ __forceinline__ float column_sums(float (&v)[C], int lane) {
-  if constexpr (C == 16) {
-#pragma unroll
-    for (int i = 0; i < 16; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], 16);
+// Warp-uniform bounded wait. The copying and the issuing warp run their loops
+// with all lanes and elect one only for the instruction itself: a loop that one
+// lane runs keeps its descriptors in vector registers, and a product then costs
+// its thread 250 clocks to issue (1.05 against 1.34 PFLOP/s at 8192^3).
+template <bool kCluster = false>
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+  auto try_wait = [&]() {
+    if constexpr (!kCluster) {
+      return tc::mbar_try_wait(bar, parity);
+    } else {  // arrivals of both blocks of a pair
+      uint32_t ok;
+      asm volatile(
+          "{\n\t.reg .pred p;\n\t"
+          "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+          "selp.u32 %0, 1, 0, p;\n\t}"
+          : "=r"(ok)
+          : "r"(tc::smem_u32(bar)), "r"(parity)
+          : "memory");
+      return ok != 0;
+    }
+  };
+  // the clock is read only once a wait has become a long one
+  bool ok = false;
+  for (int i = 0; i < 64 && !ok; ++i) ok = try_wait();
+  if (!ok) {
+    const uint64_t began = tc::globaltimer_ns();
+    while (!(ok = try_wait())) {
+      if ((abort_flag != nullptr && *abort_flag) || tc::globaltimer_ns() - began > kWaitNs) break;
+    }
   }
+  return __all_sync(0xffffffffu, ok);
+}
+
+// ------------------------------------------------------- pairs of blocks ----
+// CG = 2: two blocks of a cluster work on one tile of 256 rows. Each holds its
+// 128 rows of A and half the columns of B; the even block's thread issues the
+// products for both (cta_group::2), which halves what a block moves through
+// shared memory for the same work.
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" :::
+               "memory");
+}
+// The even block's copy of one of this block's shared addresses.
+__device__ __forceinline__ uint32_t leader_addr(const void* p) {
+  uint32_t a;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(a) : "r"(tc::smem_u32(p)));
+  return a;
+}
+template <int CG>
+__device__ __forceinline__ void load_box(void* dst, const void* map, int c0, int c1, uint64_t* bar,
+                                         uint32_t leader_bar) {
+  if constexpr (CG == 1) {
+    tc::tma_load_3d(dst, map, c0, c1, 0, bar);
+  } else {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile"
+        ".mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(tc::smem_u32(dst)),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(0), "r"(leader_bar)
+        : "memory");
+  }
+}
+template <int CG>
+__device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
+                                    uint32_t more) {
+  if constexpr (CG == 1) {
+    tc::mma_f16(d, a, b, idesc, more);
+  } else {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(more)
+        : "memory");
+  }
+}
+// Arrive, once the products issued so far are complete, on `bar` (of both blocks).
+template <int CG> __device__ __forceinline__ void commit(uint64_t* bar) {
+  if constexpr (CG == 1) {
+    tc::mma_commit(bar);
+  } else {
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64"
+        " [%0], %1;" ::"r"(tc::smem_u32(bar)),
+        "h"((uint16_t)3)
+        : "memory");
+  }
+}
+template <int CG> __device__ __forceinline__ void arrive_leader(uint64_t* bar) {
+  if constexpr (CG == 1) {
+    tc::mbar_arrive(bar);
+  } else {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(
+                     leader_addr(bar))
+                 : "memory");
+  }
+}
+template <int CG> __device__ __forceinline__ void tmem_alloc(uint32_t* dst, uint32_t cols) {
+  if constexpr (CG == 1) {
+    tc::tmem_alloc(dst, cols);
+    tc::tmem_relinquish();
+  } else {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     tc::smem_u32(dst)),
+                 "r"(cols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+}
+template <int CG> __device__ __forceinline__ void tmem_dealloc(uint32_t at, uint32_t cols) {
+  if constexpr (CG == 1)
+    tc::tmem_dealloc(at, cols);
+  else
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(at), "r"(cols)
+                 : "memory");
+}
+
+// Sums over the warp's rows of 32 columns: lane l returns the sum of v[l] over
+// the 32 lanes. Halves the columns a lane holds at each exchange.
+__device__ __forceinline__ float column_sums(float (&v)[32], int lane) {
 #pragma unroll
-  for (int off = C / 2; off > 0; off >>= 1) {
+  for (int off = 16; off > 0; off >>= 1) {
 #pragma unroll
     for (int i = 0; i < off; ++i) {
       const bool up = lane & off;
@@ -132,15 +254,20 @@ __device__ __forceinline__ void tile_at(const GemmParams& p, int t, int& tm, int
 }
 
 // T: the type of out, in and bias (kPartial: out is FP32). PARTS: 1, or 3 for
-// FP32 data split into bf16 parts.
-template <typename T, int BN, int PARTS, Epi kEpi>
+// FP32 data split into bf16 parts. CG: blocks that share a tile.
+template <typename T, int BN, int PARTS, Epi kEpi, int CG>
 __global__ void __launch_bounds__(kThreads, 1)
 linear_gemm_kernel(const __grid_constant__ GemmParams p) {
   using To = typename std::conditional<kEpi == kPartial, float, T>::type;
   constexpr bool kFast = sizeof(T) == 2;
-  constexpr int kCB = 64 / (int)sizeof(To);  // columns of a box
-  constexpr int kHalf = BN / 2;
-  constexpr int kBoxes = kHalf / kCB;        // boxes of a warp's part of a tile
+  constexpr int kHalf = BN / 2;                    // columns of a warp's part of a tile
+  constexpr int kRow = box_row(BN, sizeof(To));    // bytes of a box row
+  constexpr int kBox = 32 * kRow;
+  constexpr int kCB = kRow / (int)sizeof(To);      // columns of a box
+  constexpr int kBoxes = kHalf / kCB;
+  constexpr int kSub = kCB / 32;                   // steps of 32 columns
+  constexpr int kBNb = BN / CG;                    // columns of B this block holds
+  constexpr int kPer = 16 / (int)sizeof(To);       // values of a 16-byte chunk
   extern __shared__ uint8_t smem_raw[];
   __shared__ uint64_t full[kMaxStages], empty[kMaxStages], acc_full[2], acc_empty[2];
   __shared__ uint64_t in_full[kEpiWarps][kMaxBufs], drained;
@@ -148,8 +275,11 @@ linear_gemm_kernel(const __grid_constant__ GemmParams p) {
   __shared__ int abort_s;
   uint8_t* smem = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-  const SmemLayout L = smem_layout(PARTS, BN, p.stages, p.nbuf);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const SmemLayout L = smem_layout(CG, PARTS, BN, kRow, p.stages, p.nbuf);
+  // a shuffle, so that the compiler knows the warp's number to be uniform
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  const uint32_t rank = CG == 2 ? cluster_rank() : 0;
+  const int first_tile = blockIdx.x / CG, tile_step = gridDim.x / CG;
   volatile int* abort_flag = &abort_s;
 
   if (threadIdx.x == 0) {
@@ -159,7 +289,7 @@ linear_gemm_kernel(const __grid_constant__ GemmParams p) {
     }
     for (int i = 0; i < 2; ++i) {
       tc::mbar_init(&acc_full[i], 1);
-      tc::mbar_init(&acc_empty[i], kEpiWarps);
+      tc::mbar_init(&acc_empty[i], CG * kEpiWarps);
     }
     for (int w = 0; w < kEpiWarps; ++w)
       for (int i = 0; i < p.nbuf; ++i) tc::mbar_init(&in_full[w][i], 1);
@@ -167,55 +297,61 @@ linear_gemm_kernel(const __grid_constant__ GemmParams p) {
     abort_s = 0;
     tc::fence_mbar_init();
   }
-  if (warp == 2) {
-    tc::tmem_alloc(&tmem_base_s, 2 * BN);
-    tc::tmem_relinquish();
-  }
+  if (warp == 2) tmem_alloc<CG>(&tmem_base_s, 2 * BN);
   tc::tc_fence_before();
   __syncthreads();
+  if constexpr (CG == 2) cluster_sync();
   tc::tc_fence_after();
   const uint32_t tmem = tmem_base_s;
 
-  constexpr uint32_t kPartA = kBM * kBK * 2, kPartB = BN * kBK * 2;  // bytes of one part
+  constexpr uint32_t kPartA = kBM * kBK * 2, kPartB = kBNb * kBK * 2;  // bytes of one part
   if (warp == 0) {
-    if (lane == 0) {  // ---- operand copies ----
+    {  // ---- operand copies ----
+      const bool lead = tc::elect_one();
       uint32_t it = 0;
       bool ok = true;
-      for (int t = blockIdx.x; t < p.num_tiles && ok; t += gridDim.x) {
+      for (int t = first_tile; t < p.num_tiles && ok; t += tile_step) {
         int tm, tn, sp;
         tile_at(p, t, tm, tn, sp);
+        const int ra = (tm * CG + rank) * kBM, rb = tn * BN + rank * kBNb;
         const int kb0 = (int)((long long)p.kblocks * sp / p.splits);
         const int kb1 = (int)((long long)p.kblocks * (sp + 1) / p.splits);
         for (int kb = kb0; kb < kb1; ++kb, ++it) {
           const int s = it % p.stages;
-          if (!tc::mbar_wait(&empty[s], ((it / p.stages) & 1) ^ 1, abort_flag, kWaitNs)) {
-            give_up(abort_flag, p.status, 91);
+          if (!warp_wait(&empty[s], ((it / p.stages) & 1) ^ 1, abort_flag)) {
+            if (lead) give_up(abort_flag, p.status, 91);
             ok = false;
             break;
           }
           uint8_t* a = smem + s * L.stage;
           uint8_t* b = a + PARTS * kPartA;
-          tc::mbar_arrive_expect_tx(&full[s], L.stage);
-          // K-major: one box of [parts][rows][64 k]; MN-major: a box of
-          // [parts][64 k][64 rows] for every 64 rows
-          if (!p.a_mn) {
-            tc::tma_load_3d(a, &p.a, kb * kBK, tm * kBM, 0, &full[s]);
-          } else {
+          uint32_t bar = 0;
+          if constexpr (CG == 2) bar = leader_addr(&full[s]);
+          if (lead) {
+            // the even block's barrier counts both blocks' bytes
+            if (rank == 0) tc::mbar_arrive_expect_tx(&full[s], CG * L.stage);
+            // K-major: one box of [parts][rows][64 k]; MN-major: a box of
+            // [parts][64 k][64 rows] for every 64 rows
+            if (!p.a_mn) {
+              load_box<CG>(a, &p.a, kb * kBK, ra, &full[s], bar);
+            } else {
 #pragma unroll
-            for (int j = 0; j < kBM / 64; ++j)
-              tc::tma_load_3d(a + j * PARTS * 8192, &p.a, tm * kBM + j * 64, kb * kBK, 0, &full[s]);
-          }
-          if (!p.b_mn) {
-            tc::tma_load_3d(b, &p.b, kb * kBK, tn * BN, 0, &full[s]);
-          } else {
+              for (int j = 0; j < kBM / 64; ++j)
+                load_box<CG>(a + j * PARTS * 8192, &p.a, ra + j * 64, kb * kBK, &full[s], bar);
+            }
+            if (!p.b_mn) {
+              load_box<CG>(b, &p.b, kb * kBK, rb, &full[s], bar);
+            } else {
 #pragma unroll
-            for (int j = 0; j < BN / 64; ++j)
-              tc::tma_load_3d(b + j * PARTS * 8192, &p.b, tn * BN + j * 64, kb * kBK, 0, &full[s]);
+              for (int j = 0; j < kBNb / 64; ++j)
+                load_box<CG>(b + j * PARTS * 8192, &p.b, rb + j * 64, kb * kBK, &full[s], bar);
+            }
           }
+          __syncwarp();
         }
       }
-      // Copies still in flight have to land before the block's shared memory goes.
-      if (!ok || *abort_flag) {
+      // Copies still in flight have to land before the shared memory goes.
+      if ((!ok || *abort_flag) && rank == 0 && lead) {
         const uint32_t n = it < (uint32_t)p.stages ? it : (uint32_t)p.stages;
         for (uint32_t j = it - n; j < it; ++j)
           tc::mbar_wait(&full[j % p.stages], (j / p.stages) & 1, nullptr, kWaitNs);
@@ -223,10 +359,11 @@ linear_gemm_kernel(const __grid_constant__ GemmParams p) {
     }
     __syncwarp();
   } else if (warp == 1) {
-    if (lane == 0) {  // ---- products ----
+    if (rank == 0) {  // ---- products ----
+      const bool lead = tc::elect_one();
       uint32_t it = 0, ti = 0;  // K blocks, accumulators
       bool ok = true;
-      for (int t = blockIdx.x; t < p.num_tiles && ok; t += gridDim.x) {
+      for (int t = first_tile; t < p.num_tiles && ok; t += tile_step) {
         int tm, tn, sp;
         tile_at(p, t, tm, tn, sp);
         const int kb0 = (int)((long long)p.kblocks * sp / p.splits);
@@ -237,8 +374,8 @@ linear_gemm_kernel(const __grid_constant__ GemmParams p) {
         for (int kb = kb0; kb < kb1; ++kb, ++it) {
           const bool first = kb == kb0;
           if (first || PARTS == 3) {
-            if (!tc::mbar_wait(&acc_empty[ti & 1], ((ti >> 1) & 1) ^ 1, abort_flag, kWaitNs)) {
-              give_up(abort_flag, p.status, 92);
+            if (!warp_wait<CG == 2>(&acc_empty[ti & 1], ((ti >> 1) & 1) ^ 1, abort_flag)) {
+              if (lead) give_up(abort_flag, p.status, 92);
               ok = false;
               break;
             }
@@ -246,12 +383,11 @@ linear_gemm_kernel(const __grid_constant__ GemmParams p) {
           }
           const uint32_t d = tmem + (ti & 1) * BN;
           const int s = it % p.stages;
-          if (!tc::mbar_wait(&full[s], (it / p.stages) & 1, abort_flag, kWaitNs)) {
-            give_up(abort_flag, p.status, 93);
+          if (!warp_wait(&full[s], (it / p.stages) & 1, abort_flag)) {
+            if (lead) give_up(abort_flag, p.status, 93);
             ok = false;
             break;
           }
-          tc::tc_fence_after();
           const uint32_t sa = tc::smem_u32(smem + s * L.stage);
           const uint32_t sb = sa + PARTS * kPartA;
           const uint64_t ad = p.a_mn ? tc::smem_desc_sw128_mn(sa, PARTS * 8192)
@@ -261,80 +397,108 @@ linear_gemm_kernel(const __grid_constant__ GemmParams p) {
           // descriptor units are 16 bytes
           const uint32_t ak = (p.a_mn ? 2048 : 32) >> 4, bk = (p.b_mn ? 2048 : 32) >> 4;
           const int ksteps = kb == p.kblocks - 1 ? p.last_ksteps : kBK / 16;
-          if constexpr (PARTS == 1) {
-            for (int ks = 0; ks < ksteps; ++ks)
-              tc::mma_f16(d, ad + ks * ak, bd + ks * bk, p.idesc, (!first || ks > 0) ? 1u : 0u);
-            tc::mma_commit(&empty[s]);
-          } else {
-            const uint32_t ap = (p.a_mn ? 8192u : kPartA) >> 4, bp = (p.b_mn ? 8192u : kPartB) >> 4;
-            // the small products first, while the sum is small
-            for (int ks = 0; ks < ksteps; ++ks) {
-              const uint64_t a0 = ad + ks * ak, b0 = bd + ks * bk;
-              tc::mma_f16(d, a0 + 2 * ap, b0, p.idesc, ks > 0 ? 1u : 0u);
-              tc::mma_f16(d, a0, b0 + 2 * bp, p.idesc, 1u);
-              tc::mma_f16(d, a0 + ap, b0 + bp, p.idesc, 1u);
-              tc::mma_f16(d, a0 + ap, b0, p.idesc, 1u);
-              tc::mma_f16(d, a0, b0 + bp, p.idesc, 1u);
+          auto products = [&](auto steps) {
+            if constexpr (PARTS == 1) {
+#pragma unroll
+              for (int ks = 0; ks < steps; ++ks)
+                mma<CG>(d, ad + ks * ak, bd + ks * bk, p.idesc, (!first || ks > 0) ? 1u : 0u);
+            } else {
+              const uint32_t ap = (p.a_mn ? 8192u : kPartA) >> 4, bp = (p.b_mn ? 8192u : kPartB) >> 4;
+              // the small products first, while the sum is small
+#pragma unroll
+              for (int ks = 0; ks < steps; ++ks) {
+                const uint64_t a0 = ad + ks * ak, b0 = bd + ks * bk;
+                mma<CG>(d, a0 + 2 * ap, b0, p.idesc, ks > 0 ? 1u : 0u);
+                mma<CG>(d, a0, b0 + 2 * bp, p.idesc, 1u);
+                mma<CG>(d, a0 + ap, b0 + bp, p.idesc, 1u);
+                mma<CG>(d, a0 + ap, b0, p.idesc, 1u);
+                mma<CG>(d, a0, b0 + bp, p.idesc, 1u);
+              }
+#pragma unroll
+              for (int ks = 0; ks < steps; ++ks)
+                mma<CG>(d, ad + ks * ak, bd + ks * bk, p.idesc, 1u);
             }
-            for (int ks = 0; ks < ksteps; ++ks)
-              tc::mma_f16(d, ad + ks * ak, bd + ks * bk, p.idesc, 1u);
-            tc::mma_commit(&empty[s]);
-            tc::mma_commit(&acc_full[ti & 1]);
-            ++ti;
+          };
+          if (lead) {
+            if (ksteps == kBK / 16) products(std::integral_constant<int, kBK / 16>());
+            else products(ksteps);
+            commit<CG>(&empty[s]);
+            if constexpr (PARTS == 3) commit<CG>(&acc_full[ti & 1]);
           }
+          __syncwarp();
+          if (PARTS == 3) ++ti;
         }
         if (PARTS == 1 && ok) {
-          tc::mma_commit(&acc_full[ti & 1]);
+          if (lead) commit<CG>(&acc_full[ti & 1]);
+          __syncwarp();
           ++ti;
         }
       }
       // every product issued has completed before the tensor memory is freed
-      tc::mma_commit(&drained);
-      tc::mbar_wait(&drained, 0, nullptr, kWaitNs);
+      if (lead) commit<CG>(&drained);
+      __syncwarp();
+      warp_wait(&drained, 0, nullptr);
     }
     __syncwarp();
   } else if (warp >= kFirstEpi) {  // ---- epilogue ----
     const int ew = warp - kFirstEpi;
+    const bool lead = tc::elect_one();  // copies, stores and arrivals of the warp
     const int quad = warp & 3, half = ew >> 2;
-    uint8_t* boxes = smem + L.boxes + ew * p.nbuf * kBoxBytes;
+    uint8_t* boxes = smem + L.boxes + ew * p.nbuf * kBox;
+    float* bias_s = reinterpret_cast<float*>(smem + L.bias) + ew * kHalf;
     const To* in = static_cast<const To*>(p.in_ptr);
     const T* bias = static_cast<const T*>(p.bias);
     To* out = static_cast<To*>(p.out_ptr);
     const bool has_in = kEpi != kPartial && p.in_ptr != nullptr;
     const int ahead = has_in ? p.nbuf / 2 : 0;  // boxes loaded ahead
-    // the block's own chunk c (16 bytes) of row r: chunk c ^ (r / 2) % 4
-    const uint32_t sw = (lane >> 1) & 3;
+    // 16-byte chunk c of the box's row r lies at chunk c ^ swizzle(r), as TMA's
+    // 64- and 128-byte swizzles have it
+    auto chunk_at = [](int r, int c) {
+      return kRow == 128 ? r * 128 + ((c ^ (r & 7)) * 16) : r * 64 + ((c ^ ((r >> 1) & 3)) * 16);
+    };
+    auto value_at = [&](int r, int c) {
+      return chunk_at(r, c / kPer) + (c % kPer) * (int)sizeof(To);
+    };
     uint32_t ti = 0, q = 0;
     // the load cursor: box `lj` of tile `lt`
-    int lt = blockIdx.x, lj = 0;
+    int lt = first_tile, lj = 0;
     uint32_t lq = 0;
-    auto load_next = [&]() {  // lane 0
+    auto load_next = [&]() {  // the elected lane
       if (lt >= p.num_tiles) return;
       int tm, tn, sp;
       tile_at(p, lt, tm, tn, sp);
-      const int c = tn * BN + half * kHalf + lj * kCB, r = tm * kBM + quad * 32;
+      const int c = tn * BN + half * kHalf + lj * kCB, r = (tm * CG + rank) * kBM + quad * 32;
       const int b = lq % p.nbuf;
       if (c < p.N && r < p.M) {
-        tc::mbar_arrive_expect_tx(&in_full[ew][b], kBoxBytes);
-        tc::tma_load_3d(boxes + b * kBoxBytes, &p.in, c, r, 0, &in_full[ew][b]);
+        tc::mbar_arrive_expect_tx(&in_full[ew][b], kBox);
+        tc::tma_load_3d(boxes + b * kBox, &p.in, c, r, 0, &in_full[ew][b]);
       } else {
         tc::mbar_arrive(&in_full[ew][b]);
       }
       ++lq;
       if (++lj == kBoxes) {
         lj = 0;
-        lt += gridDim.x;
+        lt += tile_step;
       }
     };
-    if (p.tma_io && has_in && lane == 0)
+    if (p.tma_io && has_in && lead)
       for (int i = 0; i < ahead; ++i) load_next();
     bool ok = true;
-    for (int t = blockIdx.x; t < p.num_tiles && ok; t += gridDim.x) {
+    for (int t = first_tile; t < p.num_tiles && ok; t += tile_step) {
       int tm, tn, sp;
       tile_at(p, t, tm, tn, sp);
-      const int row0 = tm * kBM + quad * 32;
+      const int row0 = (tm * CG + rank) * kBM + quad * 32;
       const int row = row0 + lane;
+      const int col0 = tn * BN + half * kHalf;
       const uint32_t tcol = tmem + ((uint32_t)(quad * 32) << 16) + half * kHalf;
+      if constexpr (kEpi != kPartial) {
+        if (bias != nullptr) {
+#pragma unroll
+          for (int i = lane; i < kHalf; i += 32)
+            bias_s[i] = col0 + i < p.N ? ldg_f32<T>(bias + col0 + i) : 0.f;
+          __syncwarp();
+        }
+      }
       float sum[PARTS == 3 ? kHalf : 1];  // FP32 data: the K blocks added up
       if constexpr (PARTS == 3) {
         const int kb0 = (int)((long long)p.kblocks * sp / p.splits);
@@ -342,8 +506,7 @@ linear_gemm_kernel(const __grid_constant__ GemmParams p) {
 #pragma unroll
         for (int i = 0; i < kHalf; ++i) sum[i] = 0.f;
         for (int kb = kb0; kb < kb1; ++kb, ++ti) {
-          ok = __all_sync(0xffffffffu, tc::mbar_wait(&acc_full[ti & 1], (ti >> 1) & 1, abort_flag,
-                                                     kWaitNs));
+          ok = warp_wait(&acc_full[ti & 1], (ti >> 1) & 1, abort_flag);
           if (!ok) break;
           tc::tc_fence_after();
 #pragma unroll
@@ -357,35 +520,37 @@ linear_gemm_kernel(const __grid_constant__ GemmParams p) {
           }
           tc::tc_fence_before();
           __syncwarp();
-          if (lane == 0) tc::mbar_arrive(&acc_empty[ti & 1]);
+          if (lead) arrive_leader<CG>(&acc_empty[ti & 1]);
         }
       } else {
-        ok = __all_sync(0xffffffffu, tc::mbar_wait(&acc_full[ti & 1], (ti >> 1) & 1, abort_flag,
-                                                   kWaitNs));
+        ok = warp_wait(&acc_full[ti & 1], (ti >> 1) & 1, abort_flag);
         tc::tc_fence_after();
       }
       if (!ok) {
-        if (lane == 0) give_up(abort_flag, p.status, 94);
+        if (lead) give_up(abort_flag, p.status, 94);
         break;
       }
+      // Steps of 32 columns: while one is worked on, the next one's tensor-memory
+      // load is in flight (a step is a chain of latencies, and only two warps
+      // share a scheduler).
       const uint32_t taddr = tcol + (ti & 1) * BN;
+      float v[2][32];
+      auto fetch = [&](int step, float (&d)[32]) {
+        if constexpr (PARTS == 1) {
+          tc::tmem_ld16(taddr + step * 32, *reinterpret_cast<float(*)[16]>(d));
+          tc::tmem_ld16(taddr + step * 32 + 16, *reinterpret_cast<float(*)[16]>(d + 16));
+        }
+      };
+      fetch(0, v[0]);
 #pragma unroll (PARTS == 3 ? kBoxes : 1)
       for (int j = 0; j < kBoxes; ++j, ++q) {
-        const int c0 = tn * BN + half * kHalf + j * kCB;
+        const int c0 = col0 + j * kCB;
         const int b = q % p.nbuf;
-        uint8_t* box = boxes + b * kBoxBytes;
-        float v[kCB];
-        if constexpr (PARTS == 3) {
-#pragma unroll
-          for (int i = 0; i < kCB; ++i) v[i] = sum[j * kCB + i];
-        } else {
-#pragma unroll
-          for (int i = 0; i < kCB; i += 16)
-            tc::tmem_ld16(taddr + j * kCB + i, *reinterpret_cast<float(*)[16]>(v + i));
-        }
+        uint8_t* box = boxes + b * kBox;
+        const bool live = c0 < p.N && row0 < p.M;  // the box holds anything
         // make room, and fetch a later box of the residual
         if (p.tma_io) {
-          if (lane == 0) {
+          if (lead) {
             const int pending = has_in ? p.nbuf - ahead - 1 : p.nbuf - 1;
             if (pending >= 7) tc::bulk_wait_read<7>();
             else if (pending >= 3) tc::bulk_wait_read<3>();
@@ -395,96 +560,109 @@ linear_gemm_kernel(const __grid_constant__ GemmParams p) {
           }
           __syncwarp();
         }
-        if constexpr (PARTS == 1) tc::tmem_ld_wait();
-        const bool live = c0 < p.N && row0 < p.M;  // the box holds anything
-        if constexpr (kEpi != kPartial) {
-          if (bias != nullptr && live) {
-#pragma unroll
-            for (int i = 0; i < kCB; ++i) {
-              const int c = c0 + i < p.N ? c0 + i : p.N - 1;
-              v[i] += ldg_f32<T>(bias + c);
-            }
-          }
-          if constexpr (kEpi == kOut) act_values<kFast, kCB>(p.act, v);
-          else act_slopes<kFast, kCB>(p.act, v);
-        }
         if (has_in) {
           if (p.tma_io) {
-            ok = __all_sync(0xffffffffu, tc::mbar_wait(&in_full[ew][b], (q / p.nbuf) & 1,
-                                                       abort_flag, kWaitNs));
+            ok = warp_wait(&in_full[ew][b], (q / p.nbuf) & 1, abort_flag);
             if (!ok) {
-              if (lane == 0) give_up(abort_flag, p.status, 95);
+              if (lead) give_up(abort_flag, p.status, 95);
               break;
             }
           } else if (live) {
             // rows one after the other, a lane per column
-            if (lane < kCB && c0 + lane < p.N) {
+#pragma unroll
+            for (int cc = 0; cc < kCB; cc += 32) {
+              const int c = cc + lane;
+              if (c0 + c < p.N) {
 #pragma unroll 8
-              for (int r = 0; r < 32; ++r) {
-                if (row0 + r < p.M) {
-                  const uint32_t at = r * 64 + (((lane * sizeof(To) / 16) ^ ((r >> 1) & 3)) * 16) +
-                                      lane * sizeof(To) % 16;
-                  *reinterpret_cast<To*>(box + at) = in[(long long)(row0 + r) * p.ld_in + c0 + lane];
-                }
+                for (int r = 0; r < 32; ++r)
+                  if (row0 + r < p.M)
+                    *reinterpret_cast<To*>(box + value_at(r, c)) =
+                        in[(long long)(row0 + r) * p.ld_in + c0 + c];
               }
             }
             __syncwarp();
           }
         }
-        if (live) {
-          union Chunk { uint4 u; To e[16 / sizeof(To)]; };
-          constexpr int kPer = 16 / (int)sizeof(To);
-          if constexpr (kEpi == kDz) {
-            float s[kCB];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              Chunk ch;
-              ch.u = *reinterpret_cast<const uint4*>(box + lane * 64 + ((k ^ sw) * 16));
+        for (int sub = 0; sub < kSub; ++sub) {
+          float (&w)[32] = v[kSub == 2 ? sub : 0];
+          if constexpr (PARTS == 3) {
 #pragma unroll
-              for (int i = 0; i < kPer; ++i) {
-                const float dz = to_f32<To>(ch.e[i]) * v[k * kPer + i];
-                ch.e[i] = from_f32<To>(dz);
-                s[k * kPer + i] = row < p.M ? dz : 0.f;
-              }
-              *reinterpret_cast<uint4*>(box + lane * 64 + ((k ^ sw) * 16)) = ch.u;
-            }
-            if (p.colsum != nullptr) {
-              const float total = column_sums<kCB>(s, lane);
-              if (lane < kCB && c0 + lane < p.N)
-                p.colsum[(long long)(tm * 4 + quad) * p.N + c0 + lane] = total;
-            }
+            for (int i = 0; i < 32; ++i) w[i] = sum[j * kCB + sub * 32 + i];
           } else {
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              Chunk ch;
-              uint4* at = reinterpret_cast<uint4*>(box + lane * 64 + ((k ^ sw) * 16));
-              if (has_in) ch.u = *at;
-#pragma unroll
-              for (int i = 0; i < kPer; ++i) {
-                float y = v[k * kPer + i];
-                if (has_in) y += to_f32<To>(ch.e[i]);
-                ch.e[i] = from_f32<To>(y);
-              }
-              *at = ch.u;
+            tc::tmem_ld_wait();
+            if constexpr (kSub == 2) {
+              if (sub == 0) fetch(j * 2 + 1, v[1]);
+              else if (j + 1 < kBoxes) fetch(j * 2 + 2, v[0]);
+            }
+            if (sub == kSub - 1 && j == kBoxes - 1) {  // the accumulator is free
+              tc::tc_fence_before();
+              __syncwarp();
+              if (lead) arrive_leader<CG>(&acc_empty[ti & 1]);
             }
           }
+          if (live) {
+            if constexpr (kEpi != kPartial) {
+              if (bias != nullptr) {
+                const float4* bs = reinterpret_cast<const float4*>(bias_s + j * kCB + sub * 32);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                  const float4 u = bs[i];
+                  w[4 * i] += u.x;
+                  w[4 * i + 1] += u.y;
+                  w[4 * i + 2] += u.z;
+                  w[4 * i + 3] += u.w;
+                }
+              }
+              if constexpr (kEpi == kOut) act_values<kFast, 32>(p.act, w);
+              else act_slopes<kFast, 32>(p.act, w);
+            }
+#pragma unroll
+            for (int k = 0; k < 32 / kPer; ++k) {
+              uint4* at = reinterpret_cast<uint4*>(box + chunk_at(lane, sub * (32 / kPer) + k));
+              if (has_in) {
+                float f[kPer];
+                unpack16<To>(*at, f);
+#pragma unroll
+                for (int i = 0; i < kPer; ++i) {
+                  if constexpr (kEpi == kDz) w[k * kPer + i] *= f[i];
+                  else w[k * kPer + i] += f[i];
+                }
+              }
+              *at = pack16<To>(w + k * kPer);
+            }
+            if constexpr (kEpi == kDz) {
+              if (p.colsum != nullptr) {
+                if (row >= p.M) {
+#pragma unroll
+                  for (int i = 0; i < 32; ++i) w[i] = 0.f;
+                }
+                const float total = column_sums(w, lane);
+                if (c0 + sub * 32 + lane < p.N)
+                  p.colsum[(long long)(row0 / 32) * p.N + c0 + sub * 32 + lane] = total;
+              }
+            }
+          }
+          if constexpr (PARTS == 1 && kSub == 1) {
+            if (j + 1 < kBoxes) fetch(j + 1, v[0]);
+          }
+        }
+        if (live) {
           if (p.tma_io) {
             tc::fence_proxy_async_smem();
             __syncwarp();
-            if (lane == 0) {
-              tc::tma_store_3d(&p.out, box, c0, row0, sp);
-            }
+            if (lead) tc::tma_store_3d(&p.out, box, c0, row0, sp);
           } else {
             __syncwarp();
-            if (lane < kCB && c0 + lane < p.N) {
+#pragma unroll
+            for (int cc = 0; cc < kCB; cc += 32) {
+              const int c = cc + lane;
+              if (c0 + c < p.N) {
 #pragma unroll 8
-              for (int r = 0; r < 32; ++r) {
-                if (row0 + r < p.M) {
-                  const uint32_t at = r * 64 + (((lane * sizeof(To) / 16) ^ ((r >> 1) & 3)) * 16) +
-                                      lane * sizeof(To) % 16;
-                  out[(long long)(row0 + r) * p.ld_out + c0 + lane] =
-                      *reinterpret_cast<const To*>(box + at);
-                }
+                for (int r = 0; r < 32; ++r)
+                  if (row0 + r < p.M)
+                    out[(long long)(row0 + r) * p.ld_out + c0 + c] =
+                        *reinterpret_cast<const To*>(box + value_at(r, c));
               }
             }
             __syncwarp();
@@ -492,17 +670,12 @@ linear_gemm_kernel(const __grid_constant__ GemmParams p) {
         }
         // a group for every box, written or not, so that counting groups
         // counts boxes
-        if (p.tma_io && lane == 0) tc::bulk_commit();
+        if (p.tma_io && lead) tc::bulk_commit();
       }
       if (!ok) break;
-      if constexpr (PARTS == 1) {
-        tc::tc_fence_before();
-        __syncwarp();
-        if (lane == 0) tc::mbar_arrive(&acc_empty[ti & 1]);
-        ++ti;
-      }
+      if constexpr (PARTS == 1) ++ti;
     }
-    if (p.tma_io && lane == 0) {
+    if (p.tma_io && lead) {
       if (!ok || *abort_flag) {  // loads ahead of the failure land first
         for (uint32_t i = q; i < lq; ++i)
           tc::mbar_wait(&in_full[ew][i % p.nbuf], (i / p.nbuf) & 1, nullptr, kWaitNs);
@@ -513,9 +686,10 @@ linear_gemm_kernel(const __grid_constant__ GemmParams p) {
   }
   tc::tc_fence_before();
   __syncthreads();
+  if constexpr (CG == 2) cluster_sync();  // the pair's products and arrivals are over
   if (warp == 2) {
     tc::tc_fence_after();
-    tc::tmem_dealloc(tmem, 2 * BN);
+    tmem_dealloc<CG>(tmem, 2 * BN);
   }
 }
 
@@ -706,53 +880,97 @@ int stage(const void* src, long long ld, long long rows, int cols, void* dst, cu
   return DDPM_OK;
 }
 
-// Column tile: the widest of 256, 128, 64 that wastes less than a quarter of
-// its columns more than the next narrower one and leaves a tile for every SM.
-int pick_bn(long long m, int n, int most) {
-  const long long tm = (m + kBM - 1) / kBM;
-  for (int bn = most; bn > 64; bn /= 2) {
-    const long long tn = (n + bn - 1) / bn;
-    const long long narrow = (n + bn / 2 - 1) / (bn / 2);
-    if (tm * tn >= gencat::num_sms() && 2 * tn - narrow <= narrow / 4) return bn;
-  }
-  return 64;
+// Tile of a product: columns and blocks that share it.
+struct Tile {
+  int bn, cg;
+};
+
+// The tile with the least estimated time: rounds of tiles over the SMs, each
+// the clocks of its K blocks (the larger of what the tensor cores and the
+// shared memory need: a block's operands are written once and read once per
+// product) plus a constant for filling and draining.
+Tile pick_tile(long long m, int n, long long k, int parts, int splits) {
+  const int sms = gencat::num_sms();
+  const long long kb = ((k + kBK - 1) / kBK + splits - 1) / splits;
+  const int products = parts == 3 ? 6 : 1;
+  Tile best{64, 1};
+  double least = 0;
+  for (int cg = 1; cg <= 2; ++cg)
+    for (int bn = parts == 3 ? 128 : 256; bn >= (cg == 2 ? (parts == 3 ? 128 : 256) : 64); bn /= 2) {
+      const long long tiles =
+          ((m + kBM * cg - 1) / (kBM * cg)) * ((n + bn - 1) / bn) * splits;
+      const long long units = sms / cg;
+      const long long rounds = (tiles + units - 1) / units;
+      const double mma = products * 2.0 * bn;
+      const double move = (parts * (kBM + bn / cg) + products * (kBM + bn / cg)) * (double)kBK * 2 / 128;
+      const double t = rounds * (kb * (mma > move ? mma : move) + 1000.0 + 4.0 * bn);
+      if (least == 0 || t < least) {
+        least = t;
+        best = Tile{bn, cg};
+      }
+    }
+  return best;
 }
 
-template <typename T, int BN, int PARTS, Epi kEpi>
+template <typename T, int BN, int PARTS, Epi kEpi, int CG>
 int launch_gemm_as(GemmParams& p, cudaStream_t st) {
-  auto fn = linear_gemm_kernel<T, BN, PARTS, kEpi>;
+  auto fn = linear_gemm_kernel<T, BN, PARTS, kEpi, CG>;
+  constexpr int kRow = box_row(BN, kEpi == kPartial ? 4 : (int)sizeof(T));
   const int tiles_k = (p.kblocks + p.splits - 1) / p.splits;
   const int limit = gencat::max_smem_optin() - 2048;  // static shared memory
   // As many stages as the K loop can use, at least two; what is left goes to
   // the epilogue's boxes, eight a warp at most, two at least.
   p.nbuf = 2;
   int stages = kMaxStages;
-  auto total = [&](int s, int b) { return (int)smem_layout(PARTS, BN, s, b).total; };
+  auto total = [&](int s, int b) { return (int)smem_layout(CG, PARTS, BN, kRow, s, b).total; };
   // a persistent block streams several tiles through the ring: twice a tile's
   // steps is as far ahead as it needs to look
   const int useful = tiles_k * 2 < 2 ? 2 : tiles_k * 2;
   if (stages > useful) stages = useful;
   while (stages > 1 && total(stages, p.nbuf) > limit) --stages;
-  while (p.nbuf < kMaxBufs && total(stages, p.nbuf * 2) <= limit) p.nbuf *= 2;
+  while (p.nbuf < kMaxBufs && total(stages, p.nbuf + 1) <= limit) ++p.nbuf;
   p.stages = stages;
   const int smem = total(stages, p.nbuf);
-  DDPM_CUDA_TRY(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-  const int sms = gencat::num_sms();
-  const int grid = p.num_tiles < sms ? p.num_tiles : sms;
-  fn<<<grid, kThreads, smem, st>>>(p);
+  static std::atomic<unsigned long long> ready{0};  // devices whose limit is raised
+  int dev = 0;
+  DDPM_CUDA_TRY(cudaGetDevice(&dev));
+  if (dev >= 64 || !(ready.load(std::memory_order_relaxed) >> dev & 1)) {
+    DDPM_CUDA_TRY(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, limit));
+    if (dev < 64) ready.fetch_or(1ull << dev, std::memory_order_relaxed);
+  }
+  const int units = gencat::num_sms() / CG;
+  const int grid = (p.num_tiles < units ? p.num_tiles : units) * CG;
+  if constexpr (CG == 1) {
+    fn<<<grid, kThreads, smem, st>>>(p);
+  } else {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = CG;
+    at.val.clusterDim.y = at.val.clusterDim.z = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    DDPM_CUDA_TRY(cudaLaunchKernelEx(&cfg, fn, p));
+  }
   DDPM_CHECK_LAUNCH("linear_gemm_kernel");
   return DDPM_OK;
 }
 
 template <typename T, Epi kEpi>
-int launch_gemm(GemmParams& p, int bn, cudaStream_t st) {
+int launch_gemm(GemmParams& p, Tile t, cudaStream_t st) {
   if constexpr (sizeof(T) == 4) {
-    return bn == 128 ? launch_gemm_as<T, 128, 3, kEpi>(p, st)
-                     : launch_gemm_as<T, 64, 3, kEpi>(p, st);
+    return t.cg == 2     ? launch_gemm_as<T, 128, 3, kEpi, 2>(p, st)
+           : t.bn == 128 ? launch_gemm_as<T, 128, 3, kEpi, 1>(p, st)
+                         : launch_gemm_as<T, 64, 3, kEpi, 1>(p, st);
   } else {
-    return bn == 256   ? launch_gemm_as<T, 256, 1, kEpi>(p, st)
-           : bn == 128 ? launch_gemm_as<T, 128, 1, kEpi>(p, st)
-                       : launch_gemm_as<T, 64, 1, kEpi>(p, st);
+    return t.cg == 2     ? launch_gemm_as<T, 256, 1, kEpi, 2>(p, st)
+           : t.bn == 256 ? launch_gemm_as<T, 256, 1, kEpi, 1>(p, st)
+           : t.bn == 128 ? launch_gemm_as<T, 128, 1, kEpi, 1>(p, st)
+                         : launch_gemm_as<T, 64, 1, kEpi, 1>(p, st);
   }
 }
 
@@ -767,15 +985,16 @@ int operand_map(CUtensorMap* map, const Operand& o, bool mn_major, int tile_rows
 }
 
 int io_map(CUtensorMap* map, const void* ptr, int es, bool bf16, long long rows, int cols,
-           long long ld, int splits) {
+           long long ld, int splits, int row_bytes) {
   const uint64_t dims[3] = {(uint64_t)cols, (uint64_t)rows, (uint64_t)splits};
   const uint64_t strides[2] = {(uint64_t)ld * es, (uint64_t)rows * ld * es};
-  const uint32_t box[3] = {(uint32_t)(64 / es), 32, 1};
+  const uint32_t box[3] = {(uint32_t)(row_bytes / es), 32, 1};
   return encode_tmap(map,
                      es == 4  ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
                      : bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
                             : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
-                     3, ptr, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_64B);
+                     3, ptr, dims, strides, box,
+                     row_bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
 }
 
 // D[M][N] = sum over K of A and B as described above. `k` counts A's columns
@@ -793,7 +1012,8 @@ struct Gemm {
   long long ld_out;
   int act;
   float* colsum;
-  int splits, bn;
+  int splits;
+  Tile tile;
 };
 
 bool tma_ready(const void* ptr, long long ld, int es) {
@@ -806,8 +1026,9 @@ int run_gemm(const Gemm& g, cudaStream_t st) {
   constexpr bool kBf16 = std::is_same<Op, __nv_bfloat16>::value;
   const int es = kEpi == kPartial ? 4 : (int)sizeof(T);
   GemmParams p{};
-  p.tiles_m = (int)((g.M + kBM - 1) / kBM);
-  p.tiles_n = (g.N + g.bn - 1) / g.bn;
+  const int tile_m = kBM * g.tile.cg, bn = g.tile.bn;
+  p.tiles_m = (int)((g.M + tile_m - 1) / tile_m);
+  p.tiles_n = (g.N + bn - 1) / bn;
   p.splits = g.splits;
   p.num_tiles = p.tiles_m * p.tiles_n * g.splits;
   p.kblocks = (int)((g.K + kBK - 1) / kBK);
@@ -823,30 +1044,32 @@ int run_gemm(const Gemm& g, cudaStream_t st) {
   p.ld_in = g.ld_in;
   p.ld_out = g.ld_out;
   p.colsum = g.colsum;
-  p.idesc = tc::idesc_f16(kBM, g.bn, kBf16, g.a_mn, g.b_mn);
+  p.idesc = tc::idesc_f16(tile_m, bn, kBf16, g.a_mn, g.b_mn);
   p.tma_io = tma_ready(g.out, g.ld_out, es) && (g.in == nullptr || tma_ready(g.in, g.ld_in, es));
   int rc = gencat::status_ptr(&p.status);
   if (rc) return rc;
   rc = operand_map(&p.a, g.a, g.a_mn, kBM, kBf16);
   if (rc) return rc;
-  rc = operand_map(&p.b, g.b, g.b_mn, g.bn, kBf16);
+  rc = operand_map(&p.b, g.b, g.b_mn, bn / g.tile.cg, kBf16);
   if (rc) return rc;
+  const int row = box_row(bn, es);
   if (p.tma_io) {
-    rc = io_map(&p.out, g.out, es, kBf16, g.M, g.N, g.ld_out, g.splits);
+    rc = io_map(&p.out, g.out, es, kBf16, g.M, g.N, g.ld_out, g.splits, row);
     if (rc) return rc;
     if (g.in != nullptr) {
-      rc = io_map(&p.in, g.in, es, kBf16, g.M, g.N, g.ld_in, 1);
+      rc = io_map(&p.in, g.in, es, kBf16, g.M, g.N, g.ld_in, 1, row);
       if (rc) return rc;
     }
   }
-  return launch_gemm<T, kEpi>(p, g.bn, st);
+  return launch_gemm<T, kEpi>(p, g.tile, st);
 }
 
 // What a call has to lay out in its workspace.
 struct LinearPlan {
   bool rows_path;            // the dot-product kernel
   bool stage_x, stage_w, stage_dz;
-  int parts, bn_z, bn_x, bn_w, splits_w;
+  int parts, splits_w;
+  Tile tile_z, tile_x, tile_w;
   long long colsum_rows, colsum_chunk;
   size_t x_off, w_off, dz_off, dzp_off, colsum_off, part_off, total;
 };
@@ -863,7 +1086,6 @@ LinearPlan plan_linear(const LinearShape& s, bool bwd) {
   LinearPlan q{};
   const int es = dtype_size(s.dt);
   const bool f32 = s.dt == DDPM_F32;
-  const int widest = f32 ? 128 : 256;
   q.parts = f32 ? 3 : 1;
   q.rows_path = !bwd && s.m <= kGemvRows;
   size_t at = 0;
@@ -878,7 +1100,7 @@ LinearPlan plan_linear(const LinearShape& s, bool bwd) {
     q.x_off = q.stage_x ? take(plane_bytes(s.m, s.k, q.parts)) : 0;
     q.w_off = q.stage_w ? take(plane_bytes(s.n, s.k, q.parts)) : 0;
   }
-  q.bn_z = pick_bn(s.m, s.n, widest);
+  q.tile_z = pick_tile(s.m, s.n, s.k, q.parts, 1);
   if (bwd) {
     const bool recompute = s.act != DDPM_ACT_NONE;
     // dz as the data's type (recomputed), then as operand planes where that is
@@ -886,7 +1108,7 @@ LinearPlan plan_linear(const LinearShape& s, bool bwd) {
     if (recompute) q.dz_off = take((size_t)s.m * round8(s.n) * es);
     q.stage_dz = f32 || (!recompute && (!s.aligned || s.n % 8));
     q.dzp_off = q.stage_dz ? take(plane_bytes(s.m, s.n, q.parts)) : 0;
-    q.bn_x = pick_bn(s.m, s.k, widest);
+    q.tile_x = pick_tile(s.m, s.k, s.n, q.parts, 1);
     if (recompute) {
       q.colsum_rows = (s.m + 31) / 32;  // a row of sums for every 32 rows
     } else {
@@ -899,13 +1121,21 @@ LinearPlan plan_linear(const LinearShape& s, bool bwd) {
       q.colsum_rows = (s.m + q.colsum_chunk - 1) / q.colsum_chunk;
     }
     q.colsum_off = take((size_t)q.colsum_rows * s.n * 4);
-    // dweight: split the rows over the SMs, at least four K blocks a split
+    // dweight: the rows are split over the SMs that have no tile, at least four
+    // K blocks a split
     const long long kb = (s.m + kBK - 1) / kBK;
-    q.bn_w = s.k > 128 && widest == 256 ? 256 : s.k > 64 ? 128 : 64;
-    const long long tiles = (long long)((s.n + kBM - 1) / kBM) * ((s.k + q.bn_w - 1) / q.bn_w);
-    long long splits = gencat::num_sms() / tiles;
-    if (splits > kb / 4) splits = kb / 4;
-    q.splits_w = (int)(splits < 1 ? 1 : splits);
+    q.tile_w = pick_tile(s.n, s.k, s.m, q.parts, 1);
+    q.splits_w = 1;
+    {
+      const int bn = f32 || s.k <= 128 ? (s.k > 64 ? 128 : 64) : 256;
+      const long long tiles = (long long)((s.n + kBM - 1) / kBM) * ((s.k + bn - 1) / bn);
+      long long splits = gencat::num_sms() / tiles;
+      if (splits > kb / 4) splits = kb / 4;
+      if (splits > 1) {
+        q.splits_w = (int)splits;
+        q.tile_w = Tile{bn, 1};
+      }
+    }
     if (q.splits_w > 1) q.part_off = take((size_t)q.splits_w * s.n * ((s.k + 3) / 4 * 4) * 4);
   }
   q.total = at;
@@ -975,7 +1205,7 @@ int forward(const LinearShape& s, const LinearPlan& q, const void* x, const void
   g.ld_out = s.n;
   g.act = s.act;
   g.splits = 1;
-  g.bn = q.bn_z;
+  g.tile = q.tile_z;
   return run_gemm<T, kOut>(g, st);
 }
 
@@ -1011,7 +1241,7 @@ int backward(const LinearShape& s, const LinearPlan& q, const void* x, const voi
     g.act = s.act;
     g.colsum = gb ? colsum : nullptr;
     g.splits = 1;
-    g.bn = q.bn_z;
+    g.tile = q.tile_z;
     if ((rc = run_gemm<T, kDz>(g, st))) return rc;
     dz = g.out;
     ld_dz = g.ld_out;
@@ -1043,7 +1273,7 @@ int backward(const LinearShape& s, const LinearPlan& q, const void* x, const voi
     g.out = gx;
     g.ld_out = s.k;
     g.splits = 1;
-    g.bn = q.bn_x;
+    g.tile = q.tile_x;
     if ((rc = run_gemm<T, kOut>(g, st))) return rc;
   }
   if (gw) {
@@ -1055,7 +1285,7 @@ int backward(const LinearShape& s, const LinearPlan& q, const void* x, const voi
     g.N = s.k;
     g.K = s.m;
     g.splits = q.splits_w;
-    g.bn = q.bn_w;
+    g.tile = q.tile_w;
     if (q.splits_w > 1) {
       const int pitch = (s.k + 3) / 4 * 4;
       g.out = ws + q.part_off;
