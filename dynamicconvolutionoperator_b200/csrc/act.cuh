@@ -49,15 +49,53 @@ template <typename T> __device__ __forceinline__ uint4 pack16(const float* v) {
                       pack2<T>(v[6], v[7]));
 }
 
+// Two FP32 values in a register pair: one instruction does both.
+struct F2 {
+  unsigned long long v;
+};
+__device__ __forceinline__ F2 f2(float a, float b) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ F2 f2(float a) { return f2(a, a); }
+__device__ __forceinline__ float2 split(F2 a) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a.v));
+  return r;
+}
+__device__ __forceinline__ F2 operator+(F2 a, F2 b) {
+  F2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 operator*(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+
 __host__ inline bool act_known(int act) { return act >= DDPM_ACT_NONE && act <= DDPM_ACT_GELU_TANH; }
 
 // 1 / (1 + 2^t) by the hardware's exponential and reciprocal (2^-22 each); an
 // overflow of 2^t gives 0.
-__device__ __forceinline__ float logistic2(float t) {
-  float e, r;
+__device__ __forceinline__ float exp2_fast(float t) {
+  float e;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
-  return r;
+  return e;
+}
+__device__ __forceinline__ F2 logistic2(F2 t) {
+  const float2 u = split(t);
+  const float2 d = split(f2(exp2_fast(u.x), exp2_fast(u.y)) + f2(1.f));
+  float rx, ry;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(rx) : "f"(d.x));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(ry) : "f"(d.y));
+  return f2(rx, ry);
 }
 
 constexpr float kLog2e = 1.4426950408889634f;
@@ -67,64 +105,88 @@ constexpr float kLog2e = 1.4426950408889634f;
 // least maximum of Phi's relative error below zero, 1.6e-5; |z Phi(z)| is off
 // by at most 2.8e-6. A 16-bit value's half step is 2.4e-4 or more of it. The
 // coefficients hold the factor -log2(e).
-__device__ __forceinline__ float normal_cdf(float z) {
-  const float u = fminf(z * z, 25.f);
-  float q = fmaf(u, 7.628720572e-11f, -8.903303872e-09f);
-  q = fmaf(u, q, 4.363843402e-07f);
-  q = fmaf(u, q, -1.140831500e-05f);
-  q = fmaf(u, q, 1.531346206e-04f);
-  q = fmaf(u, q, 1.431668934e-04f);
-  q = fmaf(u, q, -1.049632579e-01f);
-  q = fmaf(u, q, -2.302116394e+00f);
+__device__ __forceinline__ F2 normal_cdf(F2 z) {
+  const float2 sq = split(z * z);
+  const F2 u = f2(fminf(sq.x, 25.f), fminf(sq.y, 25.f));
+  F2 q = fma2(u, f2(7.628720572e-11f), f2(-8.903303872e-09f));
+  q = fma2(u, q, f2(4.363843402e-07f));
+  q = fma2(u, q, f2(-1.140831500e-05f));
+  q = fma2(u, q, f2(1.531346206e-04f));
+  q = fma2(u, q, f2(1.431668934e-04f));
+  q = fma2(u, q, f2(-1.049632579e-01f));
+  q = fma2(u, q, f2(-2.302116394e+00f));
   return logistic2(z * q);
 }
 
-// Factors of the forms that are z / (1 + e^-s(z)).
-template <bool kFast, int A> __device__ __forceinline__ float act_gate(float z) {
-  if constexpr (A == DDPM_ACT_SILU) {
-    if constexpr (kFast) return logistic2(-kLog2e * z);
-    else return 1.f / (1.f + expf(-z));
-  } else if constexpr (A == DDPM_ACT_GELU) {
-    if constexpr (kFast) return normal_cdf(z);
-    // erfc keeps the relative precision of the tail below zero
-    else return 0.5f * erfcf(-0.70710678118654752f * z);
-  } else {  // (1 + tanh u) / 2 = 1 / (1 + e^-2u)
-    const float u2 = z * fmaf(0.07135481627f, z * z, 1.59576912161f);
-    if constexpr (kFast) return logistic2(-kLog2e * u2);
-    else return 1.f / (1.f + expf(-u2));
+// Factors of the forms that are z / (1 + e^-s(z)): Phi and its like.
+template <int A> __device__ __forceinline__ float act_gate(float z) {  // FP32 data
+  if constexpr (A == DDPM_ACT_SILU) return 1.f / (1.f + expf(-z));
+  // erfc keeps the relative precision of the tail below zero
+  else if constexpr (A == DDPM_ACT_GELU) return 0.5f * erfcf(-0.70710678118654752f * z);
+  // (1 + tanh u) / 2 = 1 / (1 + e^-2u)
+  else return 1.f / (1.f + expf(-z * fmaf(0.07135481627f, z * z, 1.59576912161f)));
+}
+template <int A> __device__ __forceinline__ F2 act_gate(F2 z) {  // 16-bit data
+  if constexpr (A == DDPM_ACT_SILU) return logistic2(z * f2(-kLog2e));
+  else if constexpr (A == DDPM_ACT_GELU) return normal_cdf(z);
+  else return logistic2(z * fma2(z * z, f2(-kLog2e * 0.07135481627f), f2(-kLog2e * 1.59576912161f)));
+}
+
+template <bool kFast, int A> __device__ __forceinline__ F2 act_value(F2 z) {
+  if constexpr (A == DDPM_ACT_NONE) {
+    return z;
+  } else {
+    const float2 u = split(z);
+    if constexpr (A == DDPM_ACT_RELU)
+      return f2(u.x < 0.f ? 0.f : u.x, u.y < 0.f ? 0.f : u.y);  // keeps a NaN
+    else if constexpr (kFast)
+      return z * act_gate<A>(z);
+    else
+      return z * f2(act_gate<A>(u.x), act_gate<A>(u.y));
   }
 }
 
-template <bool kFast, int A> __device__ __forceinline__ float act_value(float z) {
-  if constexpr (A == DDPM_ACT_NONE) return z;
-  else if constexpr (A == DDPM_ACT_RELU) return z < 0.f ? 0.f : z;  // keeps a NaN
-  else return z * act_gate<kFast, A>(z);
-}
-
-template <bool kFast, int A> __device__ __forceinline__ float act_slope(float z) {
+template <bool kFast, int A> __device__ __forceinline__ F2 act_slope(F2 z) {
   if constexpr (A == DDPM_ACT_NONE) {
-    return 1.f;
-  } else if constexpr (A == DDPM_ACT_RELU) {
-    return z > 0.f ? 1.f : 0.f;
+    return f2(1.f);
   } else {
-    const float g = act_gate<kFast, A>(z);
-    if constexpr (A == DDPM_ACT_SILU) {
-      return g * fmaf(z, 1.f - g, 1.f);
-    } else if constexpr (A == DDPM_ACT_GELU) {
-      const float x = -0.5f * z * z;
-      return fmaf(z * 0.39894228040143268f, kFast ? __expf(x) : expf(x), g);
+    const float2 u = split(z);
+    if constexpr (A == DDPM_ACT_RELU) {
+      return f2(u.x > 0.f ? 1.f : 0.f, u.y > 0.f ? 1.f : 0.f);
     } else {
-      const float du2 = fmaf(0.21406444881f, z * z, 1.59576912161f);
-      return fmaf(z * g, (1.f - g) * du2, g);
+      F2 g;
+      if constexpr (kFast) g = act_gate<A>(z);
+      else g = f2(act_gate<A>(u.x), act_gate<A>(u.y));
+      const F2 rest = fma2(g, f2(-1.f), f2(1.f));
+      if constexpr (A == DDPM_ACT_SILU) {
+        return g * fma2(z, rest, f2(1.f));
+      } else if constexpr (A == DDPM_ACT_GELU) {
+        F2 e;
+        if constexpr (kFast) {
+          const float2 x = split(z * z * f2(-0.5f * kLog2e));
+          e = f2(exp2_fast(x.x), exp2_fast(x.y));
+        } else {
+          e = f2(expf(-0.5f * u.x * u.x), expf(-0.5f * u.y * u.y));
+        }
+        return fma2(z * f2(0.39894228040143268f), e, g);
+      } else {
+        const F2 du = fma2(z * z, f2(0.21406444881f), f2(1.59576912161f));
+        return fma2(z * g, rest * du, g);
+      }
     }
   }
 }
 
-// v[i] = act(v[i]) and s[i] = act'(v[i]) for n values, the choice made once.
+// v[i] = act(v[i]), and v[i] = act'(v[i]), for n (even) values, the choice made
+// once.
 template <bool kFast, int n> __device__ __forceinline__ void act_values(int act, float (&v)[n]) {
 #define DDPM_ACT_CASE(A)                                        \
   case A:                                                       \
-    _Pragma("unroll") for (int i = 0; i < n; ++i) v[i] = act_value<kFast, A>(v[i]); \
+    _Pragma("unroll") for (int i = 0; i < n; i += 2) {                               \
+      const float2 r = split(act_value<kFast, A>(f2(v[i], v[i + 1])));                       \
+      v[i] = r.x;                                                                            \
+      v[i + 1] = r.y;                                                                        \
+    }                                                                                        \
     break;
   switch (act) {
     DDPM_ACT_CASE(DDPM_ACT_RELU)
@@ -138,7 +200,11 @@ template <bool kFast, int n> __device__ __forceinline__ void act_values(int act,
 template <bool kFast, int n> __device__ __forceinline__ void act_slopes(int act, float (&v)[n]) {
 #define DDPM_ACT_CASE(A)                                        \
   case A:                                                       \
-    _Pragma("unroll") for (int i = 0; i < n; ++i) v[i] = act_slope<kFast, A>(v[i]); \
+    _Pragma("unroll") for (int i = 0; i < n; i += 2) {                               \
+      const float2 r = split(act_slope<kFast, A>(f2(v[i], v[i + 1])));                       \
+      v[i] = r.x;                                                                            \
+      v[i + 1] = r.y;                                                                        \
+    }                                                                                        \
     break;
   switch (act) {
     DDPM_ACT_CASE(DDPM_ACT_RELU)

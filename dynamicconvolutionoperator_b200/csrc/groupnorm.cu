@@ -26,6 +26,9 @@
 // Variance: every thread sums x - s and (x - s)^2 for its own channel about
 // its first value s, then (count, mean, squared deviations) triples are merged
 // exactly, so a mean far from zero costs no precision.
+#include <atomic>
+#include <type_traits>
+
 #include "act.cuh"
 #include "common.cuh"
 #include "tc.cuh"
@@ -100,6 +103,29 @@ __device__ __forceinline__ Chunk chunk_of(const NormParams& p, long long t) {
   return k;
 }
 
+// The chunks of a block in order, t = block + i * grid, without a division a
+// step (one tile of columns).
+struct Walk {
+  int n, s, dn, ds;
+  __device__ __forceinline__ Walk(const NormParams& p)
+      : n((int)(blockIdx.x / (unsigned)p.S)), s((int)(blockIdx.x % (unsigned)p.S)),
+        dn((int)(gridDim.x / (unsigned)p.S)), ds((int)(gridDim.x % (unsigned)p.S)) {}
+  __device__ __forceinline__ Chunk next(const NormParams& p) {
+    Chunk k;
+    k.n = n;
+    const long long first = (long long)s * p.R;
+    k.at = (long long)n * p.P + first;
+    k.rows = (int)(p.P - first < p.R ? p.P - first : p.R);
+    n += dn;
+    s += ds;
+    if (s >= p.S) {
+      s -= p.S;
+      ++n;
+    }
+    return k;
+  }
+};
+
 __device__ __forceinline__ unsigned add_acq_rel(unsigned* p) {
   unsigned old;
   asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(old) : "l"(p) : "memory");
@@ -140,54 +166,74 @@ __device__ __forceinline__ float2 merge_unit(const NormParams& p, const float2* 
   return make_float2(mean, warp_sum(m2));
 }
 
-// Forward statistics of sample n from its chunks' partials (one block).
-__device__ void fold_stats(const NormParams& p, int n, int warp, int lane) {
-  const int upg = p.U / p.G;
-  const int items = p.S * upg;
-  const float total = (float)((double)p.P * p.cg);
-  const int last = (int)(p.P - (long long)(p.S - 1) * p.R);
-  for (int g = warp; g < p.G; g += kWarps) {
-    const float2* base = p.part + (long long)n * p.S * p.U + (long long)g * upg;
-    const float m0 = __ldcg(&base[0].x);
-    float s = 0.f;
-    for (int i = lane; i < items; i += 32) {
-      const int k = i / upg;
-      const float cnt = (float)(k == p.S - 1 ? last : p.R) * (float)p.uw;
-      s += cnt * (__ldcg(&base[(long long)k * p.U + (i - k * upg)].x) - m0);
-    }
-    const float mean = m0 + warp_sum(s) / total;
-    float m2 = 0.f;
-    for (int i = lane; i < items; i += 32) {
-      const int k = i / upg;
-      const float cnt = (float)(k == p.S - 1 ? last : p.R) * (float)p.uw;
-      const float2 v = __ldcg(&base[(long long)k * p.U + (i - k * upg)]);
-      const float d = v.x - mean;
-      m2 += v.y + cnt * d * d;
-    }
-    m2 = warp_sum(m2);
-    if (lane == 0)
-      p.stats[(long long)n * p.G + g] = make_float2(mean, 1.f / sqrtf(m2 / total + p.eps));
-  }
+__device__ __forceinline__ void count_release(unsigned* p) {
+  asm volatile("red.release.gpu.global.add.u32 [%0], 1;" ::"l"(p) : "memory");
 }
 
-// Backward group sums of sample n.
-__device__ void fold_sums(const NormParams& p, int n, int warp, int lane) {
+// Partials of a group as a warp folds them: kKept values a lane stay in
+// registers for the second pass, longer lists are read twice. The loads of a
+// pass are in flight together: the sample's whole grid waits for this fold.
+constexpr int kKept = 12;
+
+// Mean and rstd of group g of sample n from its chunks' partials (one warp).
+__device__ __forceinline__ float2 fold_stats(const NormParams& p, int n, int g, int lane) {
   const int upg = p.U / p.G;
   const int items = p.S * upg;
   const float total = (float)((double)p.P * p.cg);
-  for (int g = warp; g < p.G; g += kWarps) {
-    const float2* base = p.part + (long long)n * p.S * p.U + (long long)g * upg;
-    float a = 0.f, b = 0.f;
-    for (int i = lane; i < items; i += 32) {
-      const int k = i / upg;
-      const float2 v = __ldcg(&base[(long long)k * p.U + (i - k * upg)]);
-      a += v.x;
-      b += v.y;
+  const float* base =
+      reinterpret_cast<const float*>(p.part + (long long)n * p.S * p.U + (long long)g * upg);
+  const float per = (float)p.R * (float)p.uw;  // values behind a partial, and behind the last chunk's
+  const float last = (float)(p.P - (long long)(p.S - 1) * p.R) * (float)p.uw;
+  auto load = [&](int i) {
+    const int k = upg == 1 ? i : i / upg;
+    return __ldcg(reinterpret_cast<const float2*>(base) + (long long)k * p.U + (i - k * upg));
+  };
+  auto count = [&](int i) { return i >= items - upg ? last : per; };
+  float2 v[kKept];
+#pragma unroll
+  for (int j = 0; j < kKept; ++j)
+    if (lane + 32 * j < items) v[j] = load(lane + 32 * j);
+  const float m0 = __ldcg(base);  // sums about the first mean
+  float s = 0.f, m2 = 0.f;
+#pragma unroll
+  for (int j = 0; j < kKept; ++j)
+    if (lane + 32 * j < items) s += count(lane + 32 * j) * (v[j].x - m0);
+#pragma unroll 4
+  for (int i = lane + 32 * kKept; i < items; i += 32) s += count(i) * (load(i).x - m0);
+  const float mean = m0 + warp_sum(s) / total;
+#pragma unroll
+  for (int j = 0; j < kKept; ++j)
+    if (lane + 32 * j < items) {
+      const float d = v[j].x - mean;
+      m2 += v[j].y + count(lane + 32 * j) * d * d;
     }
-    a = warp_sum(a);
-    b = warp_sum(b);
-    if (lane == 0) p.grp[(long long)n * p.G + g] = make_float2(a / total, b / total);
+#pragma unroll 4
+  for (int i = lane + 32 * kKept; i < items; i += 32) {
+    const float2 u = load(i);
+    const float d = u.x - mean;
+    m2 += u.y + count(i) * d * d;
   }
+  m2 = warp_sum(m2);
+  return make_float2(mean, 1.f / sqrtf(m2 / total + p.eps));
+}
+
+// A and B of group g of sample n (one warp).
+__device__ __forceinline__ float2 fold_sums(const NormParams& p, int n, int g, int lane) {
+  const int upg = p.U / p.G;
+  const int items = p.S * upg;
+  const float total = (float)((double)p.P * p.cg);
+  const float2* base = p.part + (long long)n * p.S * p.U + (long long)g * upg;
+  float a = 0.f, b = 0.f;
+#pragma unroll 8
+  for (int i = lane; i < items; i += 32) {
+    const int k = upg == 1 ? i : i / upg;
+    const float2 v = __ldcg(&base[(long long)k * p.U + (i - k * upg)]);
+    a += v.x;
+    b += v.y;
+  }
+  a = warp_sum(a);
+  b = warp_sum(b);
+  return make_float2(a / total, b / total);
 }
 
 template <typename T, int V, bool kBwd>
@@ -284,13 +330,14 @@ __global__ void __launch_bounds__(kThreads, kBwd ? 2 : 3) norm_kernel(const Norm
 #pragma unroll
             for (int j = 0; j < kUnroll; ++j)
               if (r + j < mine) {
-                float xh[V], sl[V];
+                float xh[V], sl[V + V % 2];
+                if constexpr (V == 1) sl[1] = 0.f;
 #pragma unroll
                 for (int e = 0; e < V; ++e) {
                   xh[e] = (to_f32<T>(v[j].e[e]) - mean[e]) * rstd[e];
                   sl[e] = xh[e] * col.w[e] + col.b[e];
                 }
-                act_slopes<kFast, V>(p.act, sl);
+                act_slopes<kFast, V + V % 2>(p.act, sl);
 #pragma unroll
                 for (int e = 0; e < V; ++e) {
                   const float dz = to_f32<T>(g[j].e[e]) * sl[e];
@@ -336,8 +383,10 @@ __global__ void __launch_bounds__(kThreads, kBwd ? 2 : 3) norm_kernel(const Norm
       }
       __syncthreads();
       if (sh_last) {  // the sample's last chunk: fold its partials
-        if constexpr (kBwd) fold_sums(p, k.n, warp, lane);
-        else fold_stats(p, k.n, warp, lane);
+        for (int g = warp; g < p.G; g += kWarps) {
+          const float2 r = kBwd ? fold_sums(p, k.n, g, lane) : fold_stats(p, k.n, g, lane);
+          if (lane == 0) (kBwd ? p.grp : p.stats)[(long long)k.n * p.G + g] = r;
+        }
         __threadfence();
         __syncthreads();
         if (tid == 0) store_release(&flags[k.n], 1u);
@@ -388,7 +437,8 @@ __global__ void __launch_bounds__(kThreads, kBwd ? 2 : 3) norm_kernel(const Norm
 #pragma unroll
           for (int j = 0; j < kUnroll; ++j)
             if (r + j < mine) {
-              float xh[V], z[V];
+              float xh[V], z[V + V % 2];
+              if constexpr (V == 1) z[1] = 0.f;
 #pragma unroll
               for (int e = 0; e < V; ++e) {
                 xh[e] = (to_f32<T>(v[j].e[e]) - mean[e]) * rstd[e];
@@ -396,11 +446,11 @@ __global__ void __launch_bounds__(kThreads, kBwd ? 2 : 3) norm_kernel(const Norm
               }
               Vt o;
               if constexpr (!kBwd) {
-                act_values<kFast, V>(p.act, z);
+                act_values<kFast, V + V % 2>(p.act, z);
 #pragma unroll
                 for (int e = 0; e < V; ++e) o.e[e] = from_f32<T>(z[e]);
               } else {
-                act_slopes<kFast, V>(p.act, z);
+                act_slopes<kFast, V + V % 2>(p.act, z);
 #pragma unroll
                 for (int e = 0; e < V; ++e) {
                   const float dz = to_f32<T>(d[j].e[e]) * z[e];
@@ -457,8 +507,487 @@ __global__ void __launch_bounds__(256) norm_param_kernel(const float2* __restric
   }
 }
 
+// ---------------------------------------------------------- ring kernel ----
+// The same two phases for large, regular data (channels of a group in fours,
+// 16-byte rows): one block an SM, whose warps have roles.
+//   copy warp      bulk copies of chunks into a ring of shared-memory slots
+//   20 work warps  phase 1 from a slot: sums of 4 channels a thread; phase 2
+//                  from the same slot (or from a second copy where a sample
+//                  needs more steps than the ring has slots): the result
+//   4 merge warps  merge a chunk's sums, write them and count the chunk
+//   4 fold warps   wait until a sample's chunks are all counted, fold its
+//                  partials for phase 2
+// so the copies, the sums' way through global memory and the work overlap, and
+// no role waits for another's round trip: the counting is a reduction without
+// an answer, and every block folds the samples that it writes, all in the same
+// order. A slot holds a chunk of x (backward: of x and dy).
+constexpr int kWorkWarps = 20, kMergeWarps = 4, kFoldWarps = 4;
+constexpr int kWork = 32 * kWorkWarps;
+constexpr int kRingThreads = kWork + 32 * (kMergeWarps + kFoldWarps + 1);
+constexpr int kMaxSlots = 8, kRingGroups = 64;
+constexpr int kRingSmem = 196608;     // bytes of the ring
+constexpr int kSlack = 3;             // steps
+constexpr double kRingBytes = 4e6;    // least size of x
+
+struct RingParams {
+  NormParams n;
+  int slots, slot_bytes, resident;
+};
+
+struct RingShared {
+  uint64_t full[kMaxSlots], empty[kMaxSlots], part[2], part_free[2], ready[2], ready_free[2];
+  float2 sums[2][kWork];
+  float2 stat1[kMaxSlots][kRingGroups];  // backward, phase 1: mean, rstd
+  float4 stat2[2][kRingGroups];          // phase 2: mean, rstd, A, B
+  int abort, last;
+};
+
+// The row loop of a phase, specialised for the activation.
+template <typename F> __device__ __forceinline__ void with_act(int act, F&& f) {
+  switch (act) {
+    case DDPM_ACT_RELU: f(std::integral_constant<int, DDPM_ACT_RELU>()); break;
+    case DDPM_ACT_SILU: f(std::integral_constant<int, DDPM_ACT_SILU>()); break;
+    case DDPM_ACT_GELU: f(std::integral_constant<int, DDPM_ACT_GELU>()); break;
+    case DDPM_ACT_GELU_TANH: f(std::integral_constant<int, DDPM_ACT_GELU_TANH>()); break;
+    default: f(std::integral_constant<int, DDPM_ACT_NONE>());
+  }
+}
+
+// A quad of channels as two pairs.
+template <typename T> __device__ __forceinline__ void load4(const uint8_t* p, F2 (&v)[2]) {
+  if constexpr (sizeof(T) == 4) {
+    const float4 u = *reinterpret_cast<const float4*>(p);
+    v[0] = f2(u.x, u.y);
+    v[1] = f2(u.z, u.w);
+  } else {
+    const uint2 u = *reinterpret_cast<const uint2*>(p);
+    const float2 a = unpack2<T>(u.x), b = unpack2<T>(u.y);
+    v[0] = f2(a.x, a.y);
+    v[1] = f2(b.x, b.y);
+  }
+}
+template <typename T> __device__ __forceinline__ void store4(T* p, const F2 (&v)[2]) {
+  const float2 a = split(v[0]), b = split(v[1]);
+  if constexpr (sizeof(T) == 4)
+    __stcs(reinterpret_cast<float4*>(p), make_float4(a.x, a.y, b.x, b.y));
+  else
+    __stcs(reinterpret_cast<uint2*>(p), make_uint2(pack2<T>(a.x, a.y), pack2<T>(b.x, b.y)));
+}
+
+// Warp-uniform bounded wait (the clock is read only in a long one).
+__device__ __forceinline__ bool ring_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+  bool ok = false;
+  for (int i = 0; i < 64 && !ok; ++i) ok = tc::mbar_try_wait(bar, parity);
+  if (!ok) {
+    const uint64_t began = tc::globaltimer_ns();
+    while (!(ok = tc::mbar_try_wait(bar, parity)))
+      if (*abort_flag || tc::globaltimer_ns() - began > kWaitLimitNs) break;
+  }
+  return __all_sync(0xffffffffu, ok);
+}
+
+// Barrier of kCount threads that tells all of them whether any passed `bad`.
+template <int kId, int kCount> __device__ __forceinline__ bool any_of(bool bad) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 q, %1, 0;\n\t"
+      "bar.red.or.pred p, %2, %3, q;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(r)
+      : "r"((uint32_t)bad), "n"(kId), "n"(kCount)
+      : "memory");
+  return r != 0;
+}
+
+template <typename T, bool kBwd>
+__global__ void __launch_bounds__(kRingThreads, 1) norm_ring_kernel(const RingParams rp) {
+  constexpr bool kFast = sizeof(T) == 2;
+  constexpr int kQuad = 4 * (int)sizeof(T);  // bytes of a thread's four channels
+  const NormParams& p = rp.n;
+  extern __shared__ __align__(128) uint8_t ring[];
+  __shared__ RingShared sh;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  volatile int* abort_flag = &sh.abort;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < rp.slots; ++i) {
+      tc::mbar_init(&sh.full[i], 1);
+      tc::mbar_init(&sh.empty[i], kWorkWarps);
+    }
+    for (int i = 0; i < 2; ++i) {
+      tc::mbar_init(&sh.part[i], kWorkWarps);
+      tc::mbar_init(&sh.part_free[i], kMergeWarps);
+      tc::mbar_init(&sh.ready[i], kFoldWarps);
+      tc::mbar_init(&sh.ready_free[i], kWorkWarps);
+    }
+    sh.abort = 0;
+    tc::fence_mbar_init();
+  }
+  __syncthreads();
+
+  const bool write = p.out != nullptr;  // the backward may want the sums only
+  // steps this block has work in: its chunks are t = i * grid + block
+  const int mine = ((int)p.chunks - 1 - (int)blockIdx.x) / (int)gridDim.x + 1;  // grid <= chunks
+  const int steps = mine + (write ? p.lag : 0);
+  auto fail = [&](int code) {
+    if (lane == 0) {
+      sh.abort = 1;
+      atomicCAS(p.status, 0, code);
+    }
+  };
+
+  if (warp == kWorkWarps + kMergeWarps + kFoldWarps) {  // ---- copies ----
+    const bool lead = tc::elect_one();
+    uint32_t q = 0;
+    bool ok = true;
+    int s = 0;             // the next slot, and the parity of its next copy
+    uint32_t turn = 0;
+    Walk first(p), second(p);
+    auto fetch = [&](Walk& walk) {
+      if (!ring_wait(&sh.empty[s], turn ^ 1, abort_flag)) {
+        fail(96);
+        ok = false;
+        return;
+      }
+      const Chunk k = walk.next(p);
+      const uint32_t bytes = (uint32_t)k.rows * p.C * sizeof(T);
+      if (lead) {
+        uint8_t* slot = ring + (size_t)s * rp.slot_bytes;
+        const long long at = k.at * p.C * (long long)sizeof(T);
+        tc::mbar_expect_tx(&sh.full[s], kBwd ? 2 * bytes : bytes);
+        tc::bulk_g2s(slot, static_cast<const uint8_t*>(p.x) + at, bytes, &sh.full[s]);
+        if constexpr (kBwd)
+          tc::bulk_g2s(slot + rp.slot_bytes / 2, static_cast<const uint8_t*>(p.dy) + at, bytes,
+                       &sh.full[s]);
+      }
+      if constexpr (kBwd) {
+        for (int g = lane; g < p.G; g += 32) sh.stat1[s][g] = __ldg(&p.stats[(long long)k.n * p.G + g]);
+      }
+      __syncwarp();
+      if (lead) tc::mbar_arrive(&sh.full[s]);
+      ++q;
+      if (++s == rp.slots) {
+        s = 0;
+        turn ^= 1;
+      }
+    };
+    for (int i = 0; i < steps && ok; ++i) {
+      if (i < mine) fetch(first);
+      if (ok && !rp.resident && write && i >= p.lag) fetch(second);
+    }
+    if (!ok || *abort_flag) {  // what is in flight lands first
+      const uint32_t n = q < (uint32_t)rp.slots ? q : (uint32_t)rp.slots;
+      int never = 0;
+      for (uint32_t j = q - n; j < q; ++j) ring_wait(&sh.full[j % rp.slots], (j / rp.slots) & 1, &never);
+    }
+  } else if (warp >= kWorkWarps + kMergeWarps) {  // ---- samples ----
+    const int fw = warp - kWorkWarps - kMergeWarps;
+    const unsigned all = (unsigned)p.S * kMergeWarps;
+    Walk walk(p);
+    int known = -1;  // the sample whose values are in the other buffer already
+    for (int i = 0; write && i < mine; ++i) {
+      const int b = i & 1;
+      if (!ring_wait(&sh.ready_free[b], ((i >> 1) & 1) ^ 1, abort_flag)) {
+        fail(97);
+        break;
+      }
+      const bool mine_first = walk.s == 0;  // this block writes the sample's statistics
+      const Chunk k = walk.next(p);
+      if (k.n != known) {
+        bool ok = true;
+        if (load_acquire(&p.count[k.n]) != all) {
+          const uint64_t began = tc::globaltimer_ns();
+          while (load_acquire(&p.count[k.n]) != all) {
+            __nanosleep(64);
+            if (*abort_flag || tc::globaltimer_ns() - began > kWaitLimitNs) {
+              ok = false;
+              break;
+            }
+          }
+        }
+        if (!__all_sync(0xffffffffu, ok)) {
+          fail(98);
+          break;
+        }
+      }
+      for (int g = fw; g < p.G; g += kFoldWarps) {
+        float4 v;
+        if (k.n == known) {
+          v = sh.stat2[b ^ 1][g];
+        } else if constexpr (kBwd) {
+          const float2 st = __ldg(&p.stats[(long long)k.n * p.G + g]);
+          const float2 ab = fold_sums(p, k.n, g, lane);
+          v = make_float4(st.x, st.y, ab.x, ab.y);
+        } else {
+          const float2 st = fold_stats(p, k.n, g, lane);
+          v = make_float4(st.x, st.y, 0.f, 0.f);
+        }
+        if (lane == 0) {
+          sh.stat2[b][g] = v;
+          if (!kBwd && mine_first) p.stats[(long long)k.n * p.G + g] = make_float2(v.x, v.y);
+        }
+      }
+      known = k.n;
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(&sh.ready[b]);
+    }
+  } else if (warp >= kWorkWarps) {  // ---- chunks ----
+    const int fw = warp - kWorkWarps;
+    const int per = p.cg / 4;  // columns of a group
+    Walk walk(p);
+    const bool pow2 = (per & (per - 1)) == 0;
+    const int shift = __popc(per - 1);
+    auto split = [&](int j, int& y, int& x) {  // entry of a group -> row, column
+      y = pow2 ? j >> shift : j / per;
+      x = j - y * per;
+    };
+    for (int i = 0; i < mine; ++i) {
+      const int b = i & 1;
+      if (!ring_wait(&sh.part[b], (i >> 1) & 1, abort_flag)) {
+        fail(99);
+        break;
+      }
+      const Chunk k = walk.next(p);
+      const int full = (unsigned)k.rows / (unsigned)p.TY, rest = k.rows - full * p.TY;
+      for (int g = fw; g < p.G; g += kMergeWarps) {
+        const float2* base = sh.sums[b] + g * per;
+        const int items = p.TY * per;
+        float2 r;
+        if constexpr (!kBwd) {
+          const float m0 = base[0].x;  // sums about the first mean
+          float s = 0.f, m2 = 0.f;
+          for (int j = lane; j < items; j += 32) {
+            int ty, cx;
+            split(j, ty, cx);
+            const float cnt = 4.f * (float)(full + (ty < rest));
+            const float2 v = base[ty * p.TX + cx];
+            if (cnt > 0.f) s += cnt * (v.x - m0);
+          }
+          const float mean = m0 + warp_sum(s) / ((float)k.rows * (float)p.cg);
+          for (int j = lane; j < items; j += 32) {
+            int ty, cx;
+            split(j, ty, cx);
+            const float cnt = 4.f * (float)(full + (ty < rest));
+            const float2 v = base[ty * p.TX + cx];
+            const float d = v.x - mean;
+            if (cnt > 0.f) m2 += v.y + cnt * d * d;
+          }
+          r = make_float2(mean, warp_sum(m2));
+        } else {
+          float a = 0.f, c = 0.f;
+          for (int j = lane; j < items; j += 32) {
+            int ty, cx;
+            split(j, ty, cx);
+            const float2 v = base[ty * p.TX + cx];
+            a += v.x;
+            c += v.y;
+          }
+          r = make_float2(warp_sum(a), warp_sum(c));
+        }
+        if (lane == 0) p.part[((long long)i * gridDim.x + blockIdx.x) * p.G + g] = r;
+      }
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(&sh.part_free[b]);
+      if (lane == 0) count_release(&p.count[k.n]);  // behind this lane's own partials
+    }
+  } else {  // ---- work ----
+    const int tid = threadIdx.x;
+    const int tx = tid % p.TX, ty = tid / p.TX;
+    const bool live = ty < p.TY;
+    const int c0 = tx * 4, g = live ? c0 / p.cg : 0;
+    const int stride = p.TX * p.TY;  // quads between a thread's rows
+    F2 w[2], bb[2], r1[2], r2[2];  // r1, r2: this block's sums of dz, dz * xhat
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      auto param = [&](const void* q, int c, float none) {
+        return live && q ? load_param<T>(q, c, p.param_f32) : none;
+      };
+      w[e] = f2(param(p.weight, c0 + 2 * e, 1.f), param(p.weight, c0 + 2 * e + 1, 1.f));
+      bb[e] = f2(param(p.bias, c0 + 2 * e, 0.f), param(p.bias, c0 + 2 * e + 1, 0.f));
+      r1[e] = r2[e] = f2(0.f);
+    }
+    // the next slot to take (phase 1, and phase 2 where it has copies of its
+    // own) and the slot of phase 2 where it is phase 1's
+    int s1 = 0, s2 = 0;
+    uint32_t turn = 0;
+    Walk first(p), second(p);
+    auto take = [&]() {
+      if (++s1 == rp.slots) {
+        s1 = 0;
+        turn ^= 1;
+      }
+    };
+    bool ok = true;
+    for (int i = 0; i < steps && ok; ++i) {
+      if (i < mine) {  // phase 1
+        const int s = s1, b = i & 1;
+        ok = ring_wait(&sh.full[s], turn, abort_flag) &&
+             ring_wait(&sh.part_free[b], ((i >> 1) & 1) ^ 1, abort_flag);
+        if (!ok) {
+          fail(100);
+          break;
+        }
+        const Chunk k = first.next(p);
+        const uint8_t* slot = ring + (size_t)s * rp.slot_bytes;
+        const int quads = k.rows * p.TX;
+        if (live) {
+          if constexpr (!kBwd) {
+            float s0 = 0.f;
+            if (tid < quads) {
+              F2 v[2];
+              load4<T>(slot + (size_t)tid * kQuad, v);
+              s0 = split(v[0]).x;
+            }
+            const F2 less = f2(-s0);
+            F2 a1[2] = {f2(0.f), f2(0.f)}, a2[2] = {f2(0.f), f2(0.f)};
+            int count = 0;
+#pragma unroll 4
+            for (int j = tid; j < quads; j += stride) {
+              F2 v[2];
+              load4<T>(slot + (size_t)j * kQuad, v);
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                const F2 d = v[e] + less;
+                a1[e] = a1[e] + d;
+                a2[e] = fma2(d, d, a2[e]);
+              }
+              count += 4;
+            }
+            const float2 t1 = split(a1[0] + a1[1]), t2 = split(a2[0] + a2[1]);
+            const float sum = t1.x + t1.y;
+            const float m = sum / (float)(count ? count : 1);
+            sh.sums[b][tid] = make_float2(s0 + m, fmaxf(t2.x + t2.y - sum * m, 0.f));
+          } else {
+            const float2 st = sh.stat1[s][g];
+            const F2 less = f2(-st.x), rstd = f2(st.y);
+            F2 c1[2] = {f2(0.f), f2(0.f)}, c2[2] = {f2(0.f), f2(0.f)};
+            with_act(p.act, [&](auto A) {
+#pragma unroll 2
+              for (int j = tid; j < quads; j += stride) {
+                F2 x[2], d[2];
+                load4<T>(slot + (size_t)j * kQuad, x);
+                load4<T>(slot + rp.slot_bytes / 2 + (size_t)j * kQuad, d);
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                  const F2 xh = (x[e] + less) * rstd;
+                  const F2 dz = d[e] * act_slope<kFast, A.value>(fma2(xh, w[e], bb[e]));
+                  c1[e] = c1[e] + dz;
+                  c2[e] = fma2(dz, xh, c2[e]);
+                }
+              }
+            });
+            const float2 ta = split(fma2(w[0], c1[0], w[1] * c1[1]));
+            const float2 tb = split(fma2(w[0], c2[0], w[1] * c2[1]));
+            sh.sums[b][tid] = make_float2(ta.x + ta.y, tb.x + tb.y);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              r1[e] = r1[e] + c1[e];
+              r2[e] = r2[e] + c2[e];
+            }
+          }
+        }
+        __syncwarp();
+        if (lane == 0) {
+          tc::mbar_arrive(&sh.part[b]);
+          if (!rp.resident || !write) tc::mbar_arrive(&sh.empty[s]);
+        }
+        take();
+      }
+      if (write && i >= p.lag) {  // phase 2
+        const int i2 = i - p.lag;
+        const int b = i2 & 1;
+        int s;
+        if (rp.resident) {
+          s = s2;
+          if (++s2 == rp.slots) s2 = 0;
+        } else {
+          s = s1;
+          ok = ring_wait(&sh.full[s], turn, abort_flag);
+          take();
+        }
+        ok = ok && ring_wait(&sh.ready[b], (i2 >> 1) & 1, abort_flag);
+        if (!ok) {
+          fail(101);
+          break;
+        }
+        const Chunk k = second.next(p);
+        const uint8_t* slot = ring + (size_t)s * rp.slot_bytes;
+        const int quads = k.rows * p.TX;
+        if (live) {
+          const float4 st = sh.stat2[b][g];
+          T* out = static_cast<T*>(p.out) + k.at * p.C;
+          const F2 less = f2(-st.x), rstd = f2(st.y);
+          const F2 wr[2] = {w[0] * rstd, w[1] * rstd};
+          if constexpr (!kBwd) {
+            with_act(p.act, [&](auto A) {
+#pragma unroll 2
+              for (int j = tid; j < quads; j += stride) {
+                F2 v[2];
+                load4<T>(slot + (size_t)j * kQuad, v);
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+                  v[e] = act_value<kFast, A.value>(fma2(v[e] + less, wr[e], bb[e]));
+                store4<T>(out + (size_t)j * 4, v);
+              }
+            });
+          } else {
+            const F2 na = f2(-st.y * st.z), nb = f2(-st.y * st.w);
+            with_act(p.act, [&](auto A) {
+#pragma unroll 2
+              for (int j = tid; j < quads; j += stride) {
+                F2 x[2], d[2];
+                load4<T>(slot + (size_t)j * kQuad, x);
+                load4<T>(slot + rp.slot_bytes / 2 + (size_t)j * kQuad, d);
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                  const F2 xh = (x[e] + less) * rstd;
+                  const F2 dz = d[e] * act_slope<kFast, A.value>(fma2(xh, w[e], bb[e]));
+                  x[e] = fma2(dz, wr[e], fma2(xh, nb, na));
+                }
+                store4<T>(out + (size_t)j * 4, x);
+              }
+            });
+          }
+        }
+        __syncwarp();
+        if (lane == 0) {
+          tc::mbar_arrive(&sh.ready_free[b]);
+          tc::mbar_arrive(&sh.empty[s]);
+        }
+      }
+    }
+    if constexpr (kBwd) {
+      // the block's sums of a channel, its rows folded in order (the ring is
+      // free: every copy has been waited for)
+      if (p.wsum != nullptr && !any_of<2, kWork>(!ok)) {
+        float2* run = reinterpret_cast<float2*>(ring);
+        if (live) {
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float2 u = split(r1[e]), v = split(r2[e]);
+            run[ty * p.C + c0 + 2 * e] = make_float2(u.x, v.x);
+            run[ty * p.C + c0 + 2 * e + 1] = make_float2(u.y, v.y);
+          }
+        }
+        asm volatile("bar.sync 2, %0;" ::"n"(kWork) : "memory");
+        for (int c = tid; c < p.C; c += kWork) {
+          float2 a = make_float2(0.f, 0.f);
+          for (int y = 0; y < p.TY; ++y) {
+            const float2 v = run[y * p.C + c];
+            a.x += v.x;
+            a.y += v.y;
+          }
+          p.wsum[(long long)blockIdx.x * p.C + c] = a;
+        }
+      }
+    }
+  }
+}
+
 // ------------------------------------------------------------------ plan ----
 struct Plan {
+  bool ring;
+  int slots, slot_bytes, resident;
   int V, CT, TX, TY, U, uw, R, S, grid, lag;
   long long chunks;
   size_t part_off, grp_off, wsum_off, count_off, total;
@@ -470,11 +999,66 @@ int gcd_pow2(long long v, int most) {  // largest power of two <= most that divi
   return r;
 }
 
+// Workspace layout of a plan.
+void place(Plan* q, long long n, int G, int C, bool bwd) {
+  auto up = [](size_t v) { return (v + 255) / 256 * 256; };
+  q->count_off = 0;
+  q->part_off = up((size_t)n * 8);
+  q->grp_off = q->part_off + up((size_t)n * q->S * q->U * 8);
+  q->wsum_off = q->grp_off + (bwd ? up((size_t)n * G * 8) : 0);
+  q->total = q->wsum_off + (bwd ? up((size_t)(q->grid / q->CT) * C * 8) : 0);
+}
+
+// The ring kernel's plan, where it applies: rows of whole 16-byte words, groups
+// of whole quads, and enough data to fill its pipeline.
+bool plan_ring(Plan* q, long long n, long long P, int C, int G, int es, bool bwd, int align) {
+  if (align * es < 16 || C * es % 16 || C / G % 4 || C / 4 > kWork || G > kRingGroups) return false;
+  const int grid = gencat::num_sms();
+  const double bytes = (double)n * P * C * es;
+  if (bytes < kRingBytes) return false;
+  const long long row = (long long)C * es;
+  // A chunk is a slot's worth of pixels, fewer where that evens out the blocks.
+  const int slots = 4;
+  const int slot = kRingSmem / slots / 256 * 256;
+  long long r = slot / (bwd ? 2 : 1) / row;
+  if (r < 1) return false;
+  const long long even = (n * P + grid - 1) / grid;
+  const long long steps = (even + r - 1) / r;
+  r = (even + steps - 1) / steps;
+  if (r > P) r = P;
+  const long long s = (P + r - 1) / r;
+  if (n * s >= (1LL << 28)) return false;
+  q->ring = true;
+  q->slots = slots;
+  q->slot_bytes = slot;
+  q->V = 4;
+  q->CT = 1;
+  q->TX = C / 4;
+  q->TY = kWork / q->TX;
+  q->U = G;
+  q->uw = C / G;
+  q->R = (int)r;
+  q->S = (int)s;
+  q->chunks = n * s;
+  q->grid = (int)(q->chunks < grid ? q->chunks : grid);
+  q->lag = (int)((s - 1 + q->grid - 1) / q->grid);
+  // more steps than the sums need: the folds' latency is then nobody's wait
+  if (s > 1) q->lag += kSlack;
+  q->resident = q->lag <= slots - 2;
+  return true;
+}
+
 // `align`: the largest power of two (in elements, at most 16 bytes' worth)
 // that divides every tensor's address.
 int make_plan(Plan* q, long long n, long long P, int C, int G, int dt, bool bwd, int align) {
   const int es = dtype_size(dt);
-  q->V = gcd_pow2(C, align);
+  *q = Plan{};
+  if (plan_ring(q, n, P, C, G, es, bwd, align)) {
+    place(q, n, G, C, bwd);
+    return DDPM_OK;
+  }
+  // four channels a thread: eight spill (80 registers, three blocks an SM)
+  q->V = gcd_pow2(C, align < 4 ? align : 4);
   const int cols = C / q->V;
   q->CT = (cols + kThreads - 1) / kThreads;
   q->TX = (cols + q->CT - 1) / q->CT;
@@ -503,12 +1087,7 @@ int make_plan(Plan* q, long long n, long long P, int C, int G, int dt, bool bwd,
   q->S = (int)s;
   q->grid = (int)(q->chunks < most ? q->chunks : most);
   q->lag = (int)((s * q->CT - 1 + q->grid - 1) / q->grid);
-  auto up = [](size_t v) { return (v + 255) / 256 * 256; };
-  q->count_off = 0;
-  q->part_off = up((size_t)n * 8);
-  q->grp_off = q->part_off + up((size_t)n * s * q->U * 8);
-  q->wsum_off = q->grp_off + (bwd ? up((size_t)n * G * 8) : 0);
-  q->total = q->wsum_off + (bwd ? up((size_t)(q->grid / q->CT) * C * 8) : 0);
+  place(q, n, G, C, bwd);
   return DDPM_OK;
 }
 
@@ -542,10 +1121,30 @@ int launch_norm(const NormParams& p, const Plan& q, cudaStream_t st) {
 }
 
 template <typename T, bool kBwd>
-int dispatch_norm(const NormParams& p, const Plan& q, cudaStream_t st) {
-  if constexpr (sizeof(T) == 2) {
-    if (q.V == 8) return launch_norm<T, 8, kBwd>(p, q, st);
+int launch_ring(const NormParams& p, const Plan& q, cudaStream_t st) {
+  auto fn = norm_ring_kernel<T, kBwd>;
+  static std::atomic<unsigned long long> ready{0};  // devices whose limit is raised
+  int dev = 0;
+  DDPM_CUDA_TRY(cudaGetDevice(&dev));
+  if (dev >= 64 || !(ready.load(std::memory_order_relaxed) >> dev & 1)) {
+    DDPM_CUDA_TRY(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingSmem));
+    if (dev < 64) ready.fetch_or(1ull << dev, std::memory_order_relaxed);
   }
+  RingParams arg{p, q.slots, q.slot_bytes, q.resident};
+  void* args[] = {&arg};
+  if (q.S > 1) {
+    DDPM_CUDA_TRY(cudaLaunchCooperativeKernel(reinterpret_cast<const void*>(fn), dim3(q.grid),
+                                              dim3(kRingThreads), args, (size_t)kRingSmem, st));
+  } else {
+    fn<<<q.grid, kRingThreads, kRingSmem, st>>>(arg);
+  }
+  DDPM_CHECK_LAUNCH(kBwd ? "group_norm_bwd_kernel" : "group_norm_fwd_kernel");
+  return DDPM_OK;
+}
+
+template <typename T, bool kBwd>
+int dispatch_norm(const NormParams& p, const Plan& q, cudaStream_t st) {
+  if (q.ring) return launch_ring<T, kBwd>(p, q, st);
   switch (q.V) {
     case 4: return launch_norm<T, 4, kBwd>(p, q, st);
     case 2: return launch_norm<T, 2, kBwd>(p, q, st);

@@ -832,13 +832,13 @@ __global__ void __launch_bounds__(256) linear_rows_kernel(const T* __restrict__ 
   for (int r = 0; r < MR; ++r)
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) acc[r] += __shfl_xor_sync(0xffffffffu, acc[r], o);
-  float z[1] = {0.f};
+  float z[2] = {0.f, 0.f};
 #pragma unroll
   for (int r = 0; r < MR; ++r)
     if (lane == r) z[0] = acc[r];
   if (lane < m) {
     if (bias != nullptr) z[0] += to_f32<T>(bias[col]);
-    act_values<sizeof(T) == 2, 1>(act, z);
+    act_values<sizeof(T) == 2, 2>(act, z);
     const long long at = (long long)lane * n + col;
     if (res != nullptr) z[0] += to_f32<T>(res[at]);
     out[at] = from_f32<T>(z[0]);

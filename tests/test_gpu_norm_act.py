@@ -87,9 +87,28 @@ def test_activations(name, dtype):
 
 
 @pytest.mark.parametrize("dtype", ops.DTYPES)
-def test_large_samples_of_several_waves(dtype):
-    x, w, b, dy = _case((3, 64, 512, 300), dtype, 8, seed=5)
-    _run(x, 8, w, b, dy, "silu", steps=256)  # chunks of up to 768 pixels
+@pytest.mark.parametrize("shape,groups", [
+    ((3, 64, 512, 300), 8),    # a sample of more chunks than a block can hold
+    ((2, 64, 256, 257), 8),    # samples held between the phases
+    ((7, 256, 60, 61), 64),    # many groups, four channels each
+    ((40, 24, 100, 71), 1),    # 48-byte rows (96 in float32), one group
+    ((5, 2048, 20, 33), 32),   # few rows a block
+    ((1000, 32, 9, 15), 4),    # more samples than blocks
+    ((1, 16, 1024, 1024), 4),
+])
+def test_large(shape, groups, dtype):
+    x, w, b, dy = _case(shape, dtype, groups, seed=5)
+    _run(x, groups, w, b, dy, "silu", steps=256)
+
+
+@pytest.mark.parametrize("name", ops.ACTS)
+@pytest.mark.parametrize("dtype", ops.DTYPES)
+def test_large_activations(name, dtype):
+    x, w, b, dy = _case((4, 64, 100, 120), dtype, 8, seed=6, mean=3.0)
+    if name == "relu":
+        z = ops.group_norm(x, 8, w, b, 1e-5, None)[0]
+        dy = torch.where(z.abs() < 1e-4, torch.zeros_like(dy), dy)
+    _run(x, 8, w, b, dy, name)
 
 
 @pytest.mark.parametrize("mean", [0.0, 300.0])
@@ -148,10 +167,11 @@ def test_layouts_agree_and_output_is_channel_last():
     torch.testing.assert_close(got, want, rtol=1e-5, atol=1e-5)
 
 
-def test_only_the_asked_gradients():
+@pytest.mark.parametrize("side", [8, 300])
+def test_only_the_asked_gradients(side):
     from dynamicconvolutionoperator_b200 import group_norm_act
 
-    x, w, b, dy = _case((2, 16, 8, 8), torch.float32, 4)
+    x, w, b, dy = _case((2, 16, side, side), torch.float32, 4)
     full = _run(x, 4, w, b, dy, "silu")[1]
     for i in range(3):
         args = [x, w, b]
