@@ -9,21 +9,20 @@ equal arguments give equal results, on every device and in every order.
 from __future__ import annotations
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 from ._kernels import _require_cuda
+from ._op import first_order, ptr
 
 _U64 = (1 << 64) - 1
 
 
 def _launch(x, residual, p, seed, offset):
-    out = torch.empty_like(x, memory_format=torch.contiguous_format)
-    tensor = isinstance(seed, torch.Tensor)
-    _lib.call_on(x.device, "ddpm_dropout", x.data_ptr(),
-                 residual.data_ptr() if residual is not None else None, out.data_ptr(), x.numel(),
-                 p, 0 if tensor else seed, seed.data_ptr() if tensor else None, offset,
-                 _lib.dtype_code(x.dtype))
+    """``x`` (and ``residual``) contiguous; ``seed`` a number or a tensor."""
+    out = torch.empty_like(x)
+    number, held = (0, seed.data_ptr()) if isinstance(seed, torch.Tensor) else (seed, None)
+    _lib.call_on(x.device, "ddpm_dropout", x.data_ptr(), ptr(residual), out.data_ptr(), x.numel(),
+                 p, number, held, offset, _lib.dtype_code(x.dtype))
     return out
 
 
@@ -32,18 +31,22 @@ class _Dropout(torch.autograd.Function):
     def forward(ctx, x, residual, p, seed, offset):
         # a seed on the device is saved, so that writing to it before the
         # backward (which has to draw the same mask) raises
-        ctx.save_for_backward(seed if isinstance(seed, torch.Tensor) else None)
-        ctx.args = (p, None if isinstance(seed, torch.Tensor) else seed, offset)
+        if isinstance(seed, torch.Tensor):
+            ctx.save_for_backward(seed)
+            ctx.args = (p, None, offset)
+        else:
+            ctx.args = (p, seed, offset)
         return _launch(x, residual, p, seed, offset)
 
     @staticmethod
-    @once_differentiable
+    @first_order
     def backward(ctx, grad_out):
         p, seed, offset = ctx.args
-        held, = ctx.saved_tensors
         gx = None
         if ctx.needs_input_grad[0]:
-            gx = _launch(grad_out.contiguous(), None, p, seed if held is None else held, offset)
+            if seed is None:
+                seed, = ctx.saved_tensors
+            gx = _launch(grad_out.contiguous(), None, p, seed, offset)
         return gx, grad_out if ctx.needs_input_grad[1] else None, None, None, None
 
 
@@ -88,7 +91,7 @@ def dropout(x: torch.Tensor, p: float, seed: int | torch.Tensor, offset: int = 0
         if residual.shape != x.shape or residual.dtype != x.dtype:
             raise ValueError(f"residual must have x's shape and dtype, got {tuple(residual.shape)} "
                              f"of {residual.dtype} for {tuple(x.shape)} of {x.dtype}")
-    _require_cuda(x, *(t for t in (seed, residual) if isinstance(t, torch.Tensor)))
+    _require_cuda(x, *[t for t in (seed, residual) if isinstance(t, torch.Tensor)])
     _lib.dtype_code(x.dtype)
     x = x.contiguous()
     residual = residual.contiguous() if residual is not None else None

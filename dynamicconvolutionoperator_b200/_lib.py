@@ -114,7 +114,7 @@ _SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "ddpm_fuseconv_bwd_weight": (
         _c_int, [_c_ptr] * 5 + [_c_size] + [_c_int] * 6 + [_c_ptr]
     ),
-    "ddpm_group_norm_workspace_bytes": (_c_size, [_c_i64] * 2 + [_c_int] * 4),
+    "ddpm_group_norm_workspace_bytes": (_c_size, [_c_i64] * 2 + [_c_int] * 5),
     "ddpm_group_norm_fwd": (
         _c_int,
         [_c_ptr] * 6 + [_c_size] + [_c_i64] * 2 + [_c_int] * 2 + [_c_float] + [_c_int] * 3
@@ -148,6 +148,7 @@ _SIGNATURES: dict[str, tuple[object, list[object]]] = {
 
 _lock = threading.Lock()
 _lib: ctypes.CDLL | None = None
+_calls: dict[str, object] = {}  # entry points by name
 
 
 def exported_symbols() -> list[str]:
@@ -179,10 +180,12 @@ def load() -> ctypes.CDLL:
 
 def call(name: str, *args) -> None:
     """Invoke an entry point; a non-zero return raises RuntimeError with its message."""
-    lib = _lib or load()
-    rc = getattr(lib, name)(*args)
+    fn = _calls.get(name)
+    if fn is None:
+        fn = _calls[name] = getattr(load(), name)
+    rc = fn(*args)
     if rc != 0:
-        msg = lib.ddpm_last_error().decode(errors="replace")
+        msg = load().ddpm_last_error().decode(errors="replace")
         raise RuntimeError(f"{name} failed (code {rc}): {msg}")
 
 

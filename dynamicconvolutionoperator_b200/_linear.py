@@ -11,12 +11,11 @@ from __future__ import annotations
 import functools
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 from ._gradbuf import grad_buffer
 from ._kernels import _require_cuda
-from ._norm import _ptr, activation_code
+from ._op import activation_code, aligned, first_order, ptr, workspace
 
 
 def _rows(x: torch.Tensor) -> torch.Tensor:
@@ -42,14 +41,10 @@ def _row_stride(flat: torch.Tensor) -> int:
 
 
 @functools.lru_cache(maxsize=1024)
-def _workspace_bytes(m, n, k, ld, act, code, bwd, aligned, device) -> int:
-    """The plan's size on ``device`` (it depends on the number of SMs)."""
-    with torch.cuda.device(device):
-        return int(_lib.load().ddpm_linear_workspace_bytes(m, n, k, ld, act, code, bwd, aligned))
-
-
-def _workspace(nbytes: int, device: torch.device) -> torch.Tensor | None:
-    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+def _workspace_bytes(m, n, k, ld, act, code, bwd, is_aligned, index) -> int:
+    """The plan's size on device ``index`` (it depends on the number of SMs)."""
+    with torch.cuda.device(index):
+        return int(_lib.load().ddpm_linear_workspace_bytes(m, n, k, ld, act, code, bwd, is_aligned))
 
 
 def _forward(flat, w, b, res, act):
@@ -57,11 +52,10 @@ def _forward(flat, w, b, res, act):
     n = w.shape[0]
     dev, code, ld = flat.device, _lib.dtype_code(flat.dtype), _row_stride(flat)
     out = torch.empty((m, n), dtype=flat.dtype, device=dev)
-    px, pw, pb, pr, po = flat.data_ptr(), w.data_ptr(), _ptr(b), _ptr(res), out.data_ptr()
-    aligned = (px | pw | (pb or 0) | (pr or 0) | po) % 16 == 0
-    nbytes = _workspace_bytes(m, n, k, ld, act, code, 0, aligned, dev)
-    ws = _workspace(nbytes, dev)
-    _lib.call_on(dev, "ddpm_linear_fwd", px, ld, pw, pb, pr, po, _ptr(ws), nbytes, m, n, k, act,
+    px, pw, pb, pr, po = flat.data_ptr(), w.data_ptr(), ptr(b), ptr(res), out.data_ptr()
+    nbytes = _workspace_bytes(m, n, k, ld, act, code, 0, aligned(px, pw, pb, pr, po), dev.index)
+    ws = workspace(nbytes, dev)
+    _lib.call_on(dev, "ddpm_linear_fwd", px, ld, pw, pb, pr, po, ptr(ws), nbytes, m, n, k, act,
                  code)
     return out
 
@@ -81,34 +75,34 @@ class _LinearAct(torch.autograd.Function):
         return out if x.ndim == 2 else out.reshape(*x.shape[:-1], n)
 
     @staticmethod
-    @once_differentiable
+    @first_order
     def backward(ctx, grad_out):
         flat, w, b = ctx.saved_tensors
         weight, bias = ctx.params
+        need_x, need_w, need_b, need_res = ctx.needs_input_grad[:4]
         m, k = flat.shape
         n = w.shape[0]
         dev, dt = flat.device, flat.dtype
-        need_w = ctx.needs_input_grad[1]
-        need_b = bias is not None and ctx.needs_input_grad[2]
-        gx = torch.empty((m, k), dtype=dt, device=dev) if ctx.needs_input_grad[0] else None
+        gx = torch.empty((m, k), dtype=dt, device=dev) if need_x else None
         gw = grad_buffer(weight, weight.shape, dt, dev) if need_w else None
         gb = grad_buffer(bias, bias.shape, dt, dev) if need_b else None
         if m == 0:
             for g in (gw, gb):
                 if g is not None:
                     g.zero_()
-        elif gx is not None or need_w or need_b:
+        elif need_x or need_w or need_b:
             g = _matrix(grad_out, (m, n))
             code, ld = _lib.dtype_code(dt), _row_stride(flat)
-            ptrs = [_ptr(t) for t in (flat, w, b, g, gx, gw, gb)]
-            aligned = not any(q and q % 16 for q in ptrs)
-            nbytes = _workspace_bytes(m, n, k, ld, ctx.act, code, 1, aligned, dev)
-            ws = _workspace(nbytes, dev)
-            _lib.call_on(dev, "ddpm_linear_bwd", ptrs[0], ld, *ptrs[1:], _ptr(ws), nbytes, m, n, k,
-                         ctx.act, code)
-        if gx is not None:
+            px, pw, pb, pg = flat.data_ptr(), w.data_ptr(), ptr(b), g.data_ptr()
+            ox, ow, ob = ptr(gx), ptr(gw), ptr(gb)
+            nbytes = _workspace_bytes(m, n, k, ld, ctx.act, code, 1,
+                                      aligned(px, pw, pb, pg, ox, ow, ob), dev.index)
+            ws = workspace(nbytes, dev)
+            _lib.call_on(dev, "ddpm_linear_bwd", px, ld, pw, pb, pg, ox, ow, ob, ptr(ws), nbytes,
+                         m, n, k, ctx.act, code)
+        if need_x and len(ctx.shape) != 2:
             gx = gx.reshape(ctx.shape)
-        return gx, gw, gb, grad_out if ctx.needs_input_grad[3] else None, None
+        return gx, gw, gb, grad_out if need_res else None, None
 
 
 def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None,
@@ -149,7 +143,7 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None 
             raise ValueError(f"all tensors must have one dtype, got {x.dtype} and {t.dtype}")
     _require_cuda(x, *given)
     _lib.dtype_code(x.dtype)
-    if torch.is_grad_enabled() and (x.requires_grad or any(t.requires_grad for t in given)):
+    if torch.is_grad_enabled() and (x.requires_grad or any([t.requires_grad for t in given])):
         return _LinearAct.apply(x, weight, bias, residual, act)
     flat = _rows(x)
     out = _forward(flat, _matrix(weight, (n, flat.shape[1])),

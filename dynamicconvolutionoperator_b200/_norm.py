@@ -9,22 +9,15 @@ is stored.
 
 from __future__ import annotations
 
+import functools
+import math
+
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 from ._gradbuf import grad_buffer
 from ._kernels import _require_cuda
-
-ACTIVATIONS = {None: 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}
-
-
-def activation_code(activation: str | None) -> int:
-    try:
-        return ACTIVATIONS[activation]
-    except (KeyError, TypeError):
-        raise ValueError(f"activation must be one of {sorted(k for k in ACTIVATIONS if k)} or "
-                         f"None, got {activation!r}") from None
+from ._op import activation_code, aligned, first_order, ptr, workspace
 
 
 def _channel_last(t: torch.Tensor) -> torch.Tensor:
@@ -36,29 +29,28 @@ def _channel_first(t: torch.Tensor) -> torch.Tensor:
     return t.movedim(-1, 1) if t.ndim > 2 else t
 
 
-def _ptr(t: torch.Tensor | None):
-    return t.data_ptr() if t is not None else None
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(n, pixels, c, groups, code, bwd, is_aligned, index) -> int:
+    """The plan's size on device ``index`` (it depends on the number of SMs)."""
+    with torch.cuda.device(index):
+        return int(_lib.load().ddpm_group_norm_workspace_bytes(n, pixels, c, groups, code, bwd,
+                                                               is_aligned))
 
 
-def _sizes(xl: torch.Tensor) -> tuple[int, int, int]:
-    n, c = xl.shape[0], xl.shape[-1]
-    pixels = 1
-    for d in xl.shape[1:-1]:
-        pixels *= d
-    return n, pixels, c
-
-
-def _forward(xl, weight, bias, groups, eps, act):
-    n, pixels, c = _sizes(xl)
+def _forward(xl, w, b, groups, eps, act):
+    shape = xl.shape
+    n, c = shape[0], shape[-1]
+    pixels = math.prod(shape[1:-1])
+    dev, code = xl.device, _lib.dtype_code(xl.dtype)
     out = torch.empty_like(xl)
-    stats = torch.empty((n, groups, 2), dtype=torch.float32, device=xl.device)
-    code = _lib.dtype_code(xl.dtype)
-    nbytes = int(_lib.load().ddpm_group_norm_workspace_bytes(n, pixels, c, groups, code, 0))
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=xl.device)
-    params = weight if weight is not None else bias
-    _lib.call_on(xl.device, "ddpm_group_norm_fwd", xl.data_ptr(), _ptr(weight), _ptr(bias),
-                 out.data_ptr(), stats.data_ptr(), ws.data_ptr(), nbytes, n, pixels, c, groups,
-                 eps, act, code, code if params is None else _lib.dtype_code(params.dtype))
+    stats = torch.empty((n, groups, 2), dtype=torch.float32, device=dev)
+    px, po = xl.data_ptr(), out.data_ptr()
+    nbytes = _workspace_bytes(n, pixels, c, groups, code, 0, aligned(px, po), dev.index)
+    ws = workspace(nbytes, dev)
+    params = w if w is not None else b
+    _lib.call_on(dev, "ddpm_group_norm_fwd", px, ptr(w), ptr(b), po, stats.data_ptr(), ptr(ws),
+                 nbytes, n, pixels, c, groups, eps, act, code,
+                 code if params is None else _lib.dtype_code(params.dtype))
     return out, stats
 
 
@@ -69,37 +61,39 @@ class _GroupNormAct(torch.autograd.Function):
         w = weight.contiguous() if weight is not None else None
         b = bias.contiguous() if bias is not None else None
         out, stats = _forward(xl, w, b, groups, eps, act)
-        ctx.save_for_backward(xl, w, b, stats)
+        ctx.save_for_backward(xl, w, b)
+        ctx.stats = stats
         ctx.params = (weight, bias)  # gradient buffers are looked up by identity
-        ctx.groups, ctx.act = groups, act
+        ctx.args = (groups, act)
         return _channel_first(out)
 
     @staticmethod
-    @once_differentiable
+    @first_order
     def backward(ctx, grad_out):
-        xl, w, b, stats = ctx.saved_tensors
+        xl, w, b = ctx.saved_tensors
         weight, bias = ctx.params
-        n, pixels, c = _sizes(xl)
-        need_x = ctx.needs_input_grad[0]
-        need_w = weight is not None and ctx.needs_input_grad[1]
-        need_b = bias is not None and ctx.needs_input_grad[2]
+        groups, act = ctx.args
+        need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        dev = xl.device
         gx = torch.empty_like(xl) if need_x else None
-        gw = grad_buffer(weight, weight.shape, weight.dtype, xl.device) if need_w else None
-        gb = grad_buffer(bias, bias.shape, bias.dtype, xl.device) if need_b else None
+        gw = grad_buffer(weight, weight.shape, weight.dtype, dev) if need_w else None
+        gb = grad_buffer(bias, bias.shape, bias.dtype, dev) if need_b else None
         if xl.numel() == 0:
             for g in (gw, gb):
                 if g is not None:
                     g.zero_()
         else:
             g = _channel_last(grad_out)
+            shape = xl.shape
+            n, c = shape[0], shape[-1]
+            pixels = math.prod(shape[1:-1])
             code = _lib.dtype_code(xl.dtype)
-            nbytes = int(_lib.load().ddpm_group_norm_workspace_bytes(n, pixels, c, ctx.groups,
-                                                                     code, 1))
-            ws = torch.empty(nbytes, dtype=torch.uint8, device=xl.device)
+            px, pg, po = xl.data_ptr(), g.data_ptr(), ptr(gx)
+            nbytes = _workspace_bytes(n, pixels, c, groups, code, 1, aligned(px, pg, po), dev.index)
+            ws = workspace(nbytes, dev)
             params = w if w is not None else b
-            _lib.call_on(xl.device, "ddpm_group_norm_bwd", xl.data_ptr(), g.data_ptr(), _ptr(w),
-                         _ptr(b), stats.data_ptr(), _ptr(gx), _ptr(gw), _ptr(gb), ws.data_ptr(),
-                         nbytes, n, pixels, c, ctx.groups, ctx.act, code,
+            _lib.call_on(dev, "ddpm_group_norm_bwd", px, pg, ptr(w), ptr(b), ctx.stats.data_ptr(),
+                         po, ptr(gw), ptr(gb), ptr(ws), nbytes, n, pixels, c, groups, act, code,
                          code if params is None else _lib.dtype_code(params.dtype))
         return _channel_first(gx) if need_x else None, gw, gb, None, None, None
 
@@ -141,12 +135,13 @@ def group_norm_act(x: torch.Tensor, num_groups: int, weight: torch.Tensor | None
         raise ValueError(f"weight and bias must have one dtype, got {weight.dtype} and {bias.dtype}")
     _require_cuda(x, *(t for t in (weight, bias) if t is not None))
     _lib.dtype_code(x.dtype)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad
-                                       for t in (x, weight, bias)):
+    if torch.is_grad_enabled() and (x.requires_grad
+                                    or (weight is not None and weight.requires_grad)
+                                    or (bias is not None and bias.requires_grad)):
         return _GroupNormAct.apply(x, weight, bias, num_groups, float(eps), act)
     out, _ = _forward(_channel_last(x), weight.contiguous() if weight is not None else None,
                       bias.contiguous() if bias is not None else None, num_groups, float(eps), act)
     return _channel_first(out)
 
 
-__all__ = ["ACTIVATIONS", "activation_code", "group_norm_act"]
+__all__ = ["group_norm_act"]

@@ -89,7 +89,8 @@ int read_status(int reset, int* code);
 size_t fuseconv_wgrad_workspace_bytes(int n, int cin, int cout, int h, int w);
 int fuseconv_wgrad(const void* cat, const void* gout, void* gw, void* gb, void* ws, size_t ws_bytes,
                    int n, int cin, int cout, int h, int w, int dt, cudaStream_t st);
-size_t group_norm_workspace_bytes(long long n, long long P, int C, int G, int dt, int bwd);
+size_t group_norm_workspace_bytes(long long n, long long P, int C, int G, int dt, int bwd,
+                                  int aligned);
 int group_norm_fwd(const void* x, const void* w, const void* b, void* out, void* stats, void* ws,
                    size_t ws_bytes, long long n, long long P, int C, int G, float eps, int act,
                    int dt, int pdt, cudaStream_t st);
@@ -367,8 +368,8 @@ int ddpm_fuseconv_bwd_weight(const void* x, const void* grad_out, void* grad_wei
 }
 
 size_t ddpm_group_norm_workspace_bytes(long long n, long long pixels, int channels, int groups,
-                                       int dtype, int bwd) {
-  return ddpm::group_norm_workspace_bytes(n, pixels, channels, groups, dtype, bwd);
+                                       int dtype, int bwd, int aligned) {
+  return ddpm::group_norm_workspace_bytes(n, pixels, channels, groups, dtype, bwd, aligned);
 }
 
 int ddpm_group_norm_fwd(const void* x, const void* weight, const void* bias, void* out, void* stats,

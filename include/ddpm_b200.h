@@ -388,11 +388,13 @@ DDPM_API int ddpm_gencat_bwd_yw_static(const void* x, const void* y, const void*
  * channels / groups channels over all pixels (biased variance, FP32).
  * weight and bias [channels] may be NULL (ones, zeros); `param_dtype` is
  * `dtype` or DDPM_F32. `stats` [n][groups][2] FP32 receives (mean, rstd) and is
- * what the backward reads. Workspace: `bwd` 0 / 1 selects the entry point;
- * 256-byte aligned, 0 bytes for an empty x. n or pixels of 0: nothing runs.
+ * what the backward reads. Workspace: `bwd` 0 / 1 selects the entry point,
+ * `aligned` says that x, out, grad_out and grad_x are on 16-byte boundaries (0
+ * is always enough); 256-byte aligned, may be NULL where 0 bytes are asked for.
+ * n or pixels of 0: nothing runs.
  */
 DDPM_API size_t ddpm_group_norm_workspace_bytes(long long n, long long pixels, int channels,
-                                                int groups, int dtype, int bwd);
+                                                int groups, int dtype, int bwd, int aligned);
 DDPM_API int ddpm_group_norm_fwd(const void* x, const void* weight, const void* bias, void* out,
                                  void* stats, void* workspace, size_t workspace_bytes,
                                  long long n, long long pixels, int channels, int groups,

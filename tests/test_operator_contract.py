@@ -125,7 +125,8 @@ def test_abi_argument_errors_without_gpu():
     assert norm(x=None) == -1 and b"null" in lib.ddpm_last_error()
     assert norm(x=18) == -1 and b"misaligned" in lib.ddpm_last_error()
     assert norm(ws=128) == -1 and b"misaligned" in lib.ddpm_last_error()
-    assert norm(nbytes=16) == -4 and b"workspace" in lib.ddpm_last_error()
+    assert norm(px=1 << 20, nbytes=16) == -4 and b"workspace" in lib.ddpm_last_error()
+    assert norm(px=1 << 20, ws=None) == -4
     assert norm(c=1 << 17) == -2
     assert norm(n=0) == 0 and norm(px=0) == 0
 
@@ -144,6 +145,8 @@ def test_abi_argument_errors_without_gpu():
 def test_group_norm_workspace_covers_every_alignment(bwd):
     lib = _lib.load()
     size = lib.ddpm_group_norm_workspace_bytes
-    assert size(0, 4, 8, 2, 0, bwd) == 0 and size(4, 4, 9, 2, 0, bwd) == 0
+    assert size(0, 4, 8, 2, 0, bwd, 0) == 0 and size(4, 4, 9, 2, 0, bwd, 0) == 0
     for c, g in ((64, 8), (60, 5), (515, 5), (4096, 32)):
-        assert size(3, 1000, c, g, 1, bwd) > 0
+        for n, px in ((3, 1000), (5, 100_000)):
+            assert size(n, px, c, g, 1, bwd, 0) >= size(n, px, c, g, 1, bwd, 1)
+        assert size(5, 100_000, c, g, 1, bwd, 1) > 0
