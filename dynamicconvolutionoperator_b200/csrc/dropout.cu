@@ -16,6 +16,7 @@
 // integer multiplies close behind for 16-bit data: 20 32x32->64-bit products
 // per four values. Hence one Philox block serves four neighbouring values and
 // a thread handles 16 bytes (one or two blocks) per step.
+#include "act.cuh"
 #include "common.cuh"
 
 namespace ddpm {
@@ -31,7 +32,6 @@ struct DropParams {
   const unsigned long long* seed_ptr;  // nullable: read on the device instead of `seed`
   unsigned long long offset;
   uint32_t threshold;    // keep iff word >= threshold
-  int drop_all;          // p == 1
   float scale;
 };
 
@@ -50,56 +50,62 @@ __device__ __forceinline__ void philox(uint64_t block, uint32_t k0, uint32_t k1,
   w[0] = c0; w[1] = c1; w[2] = c2; w[3] = c3;
 }
 
-template <typename T>
+template <bool kAll>
 __device__ __forceinline__ float drop_one(const DropParams& p, uint32_t word, float x) {
-  return word >= p.threshold && !p.drop_all ? x * p.scale : 0.f;
+  return !kAll && word >= p.threshold ? x * p.scale : 0.f;
 }
 
 // Aligned form: offset % 4 == 0 and every pointer on a 16-byte boundary. A
 // thread handles kVec = 16 / sizeof(T) values (one or two generator blocks).
-template <typename T, bool kRes>
+// kAll: p is 1.
+template <typename T, bool kRes, bool kAll>
 __global__ void __launch_bounds__(256) dropout_vec_kernel(const DropParams p) {
   constexpr int kVec = 16 / (int)sizeof(T);
   const uint64_t seed = p.seed_ptr ? *p.seed_ptr : p.seed;
   const uint32_t k0 = (uint32_t)seed, k1 = (uint32_t)(seed >> 32);
-  const T* x = static_cast<const T*>(p.x);
-  const T* res = static_cast<const T*>(p.res);
-  T* out = static_cast<T*>(p.out);
+  const uint4* x = static_cast<const uint4*>(p.x);
+  const uint4* res = static_cast<const uint4*>(p.res);
+  uint4* out = static_cast<uint4*>(p.out);
   const long long nvec = p.n / kVec;
   const long long step = (long long)gridDim.x * blockDim.x;
   const uint64_t b0 = p.offset >> 2;
-  union Pack { uint4 u; T e[kVec]; };
+  const F2 scale = f2(p.scale);
   for (long long i = blockIdx.x * (long long)blockDim.x + threadIdx.x; i < nvec; i += step) {
-    Pack v, r, o;
-    v.u = __ldcs(reinterpret_cast<const uint4*>(x) + i);
-    if constexpr (kRes) r.u = __ldcs(reinterpret_cast<const uint4*>(res) + i);
+    float v[kVec], r[kVec];
+    unpack16<T>(__ldcs(x + i), v);
+    if constexpr (kRes) unpack16<T>(__ldcs(res + i), r);
+    uint32_t w[kVec / 4][4];
+    if constexpr (!kAll) {
 #pragma unroll
-    for (int q = 0; q < kVec / 4; ++q) {
-      uint32_t w[4];
-      philox(b0 + (uint64_t)i * (kVec / 4) + q, k0, k1, w);
+      for (int q = 0; q < kVec / 4; ++q) philox(b0 + (uint64_t)i * (kVec / 4) + q, k0, k1, w[q]);
+    }
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        float y = drop_one<T>(p, w[e], to_f32<T>(v.e[q * 4 + e]));
-        if constexpr (kRes) y += to_f32<T>(r.e[q * 4 + e]);
-        o.e[q * 4 + e] = from_f32<T>(y);
+    for (int e = 0; e < kVec; e += 2) {
+      const float2 y = split(f2(v[e], v[e + 1]) * scale);
+      v[e] = !kAll && w[e / 4][e % 4] >= p.threshold ? y.x : 0.f;
+      v[e + 1] = !kAll && w[e / 4][e % 4 + 1] >= p.threshold ? y.y : 0.f;
+      if constexpr (kRes) {
+        const float2 z = split(f2(v[e], v[e + 1]) + f2(r[e], r[e + 1]));
+        v[e] = z.x;
+        v[e + 1] = z.y;
       }
     }
-    __stcs(reinterpret_cast<uint4*>(out) + i, o.u);
+    __stcs(out + i, pack16<T>(v));
   }
   // the last n % kVec values: the first threads of block 0 take one each
   const long long i = nvec * kVec + threadIdx.x;
   if (blockIdx.x == 0 && i < p.n) {
     uint32_t w[4];
     philox(b0 + (uint64_t)(i >> 2), k0, k1, w);
-    float y = drop_one<T>(p, w[i & 3], to_f32<T>(x[i]));
-    if constexpr (kRes) y += to_f32<T>(res[i]);
-    out[i] = from_f32<T>(y);
+    float y = drop_one<kAll>(p, w[i & 3], to_f32<T>(static_cast<const T*>(p.x)[i]));
+    if constexpr (kRes) y += to_f32<T>(static_cast<const T*>(p.res)[i]);
+    static_cast<T*>(p.out)[i] = from_f32<T>(y);
   }
 }
 
 // Any offset and alignment: a thread handles the (at most four) values of one
 // generator block.
-template <typename T, bool kRes>
+template <typename T, bool kRes, bool kAll>
 __global__ void __launch_bounds__(256) dropout_any_kernel(const DropParams p) {
   const uint64_t seed = p.seed_ptr ? *p.seed_ptr : p.seed;
   const uint32_t k0 = (uint32_t)seed, k1 = (uint32_t)(seed >> 32);
@@ -122,28 +128,31 @@ __global__ void __launch_bounds__(256) dropout_any_kernel(const DropParams p) {
     philox((p.offset >> 2) + (uint64_t)b, k0, k1, w);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      float y = drop_one<T>(p, w[e], v[e]);
+      float y = drop_one<kAll>(p, w[e], v[e]);
       if constexpr (kRes) y += r[e];
       if (i0 + e >= 0 && i0 + e < p.n) out[i0 + e] = from_f32<T>(y);
     }
   }
 }
 
-template <typename T>
-int launch_dropout(const DropParams& p, bool vec, cudaStream_t st) {
+template <typename T, bool kRes, bool kAll>
+int launch_dropout_as(const DropParams& p, bool vec, cudaStream_t st) {
   const long long items = vec ? (p.n + 16 / sizeof(T) - 1) / (16 / sizeof(T)) : (p.n + 6) / 4;
   const long long most = 148LL * 8 * 4;
   const long long want = (items + 255) / 256;
   const int grid = (int)(want < most ? want : most);
-  if (vec) {
-    if (p.res) dropout_vec_kernel<T, true><<<grid, 256, 0, st>>>(p);
-    else dropout_vec_kernel<T, false><<<grid, 256, 0, st>>>(p);
-  } else {
-    if (p.res) dropout_any_kernel<T, true><<<grid, 256, 0, st>>>(p);
-    else dropout_any_kernel<T, false><<<grid, 256, 0, st>>>(p);
-  }
+  if (vec) dropout_vec_kernel<T, kRes, kAll><<<grid, 256, 0, st>>>(p);
+  else dropout_any_kernel<T, kRes, kAll><<<grid, 256, 0, st>>>(p);
   DDPM_CHECK_LAUNCH("dropout_kernel");
   return DDPM_OK;
+}
+
+template <typename T> int launch_dropout(const DropParams& p, bool all, bool vec, cudaStream_t st) {
+  if (all)
+    return p.res ? launch_dropout_as<T, true, true>(p, vec, st)
+                 : launch_dropout_as<T, false, true>(p, vec, st);
+  return p.res ? launch_dropout_as<T, true, false>(p, vec, st)
+               : launch_dropout_as<T, false, false>(p, vec, st);
 }
 
 }  // namespace
@@ -168,14 +177,14 @@ int dropout(const void* x, const void* residual, void* out, long long n, double 
   q.seed_ptr = static_cast<const unsigned long long*>(seed_ptr);
   q.offset = offset;
   const double t = p * 4294967296.0 + 0.5;  // floor(t) = round(p * 2^32)
-  q.drop_all = t >= 4294967296.0;
-  q.threshold = q.drop_all ? 0xFFFFFFFFu : (uint32_t)t;
+  const bool all = t >= 4294967296.0;
+  q.threshold = all ? 0xFFFFFFFFu : (uint32_t)t;
   q.scale = p < 1.0 ? (float)(1.0 / (1.0 - p)) : 0.f;
   const bool vec = at % 16 == 0 && offset % 4 == 0;
   switch (dt) {
-    case DDPM_F32: return launch_dropout<float>(q, vec, st);
-    case DDPM_BF16: return launch_dropout<__nv_bfloat16>(q, vec, st);
-    default: return launch_dropout<__half>(q, vec, st);
+    case DDPM_F32: return launch_dropout<float>(q, all, vec, st);
+    case DDPM_BF16: return launch_dropout<__nv_bfloat16>(q, all, vec, st);
+    default: return launch_dropout<__half>(q, all, vec, st);
   }
 }
 
