@@ -256,6 +256,15 @@ int encode_tmap(CUtensorMap* map, CUtensorMapDataType type, int rank, const void
   });
   if (encode == nullptr)
     return set_error(DDPM_ERR_CUDA, "cuTensorMapEncodeTiled is not available");
+  // A driver call needs a current context, which a thread that has made no
+  // runtime call yet (autograd's, for one) does not have.
+  int dev = 0;
+  thread_local int bound = -1;
+  DDPM_CUDA_TRY(cudaGetDevice(&dev));
+  if (bound != dev) {
+    DDPM_CUDA_TRY(cudaSetDevice(dev));
+    bound = dev;
+  }
   cuuint64_t d[5], s[4];
   cuuint32_t b[5], e[5];
   for (int i = 0; i < rank; ++i) {

@@ -1065,7 +1065,7 @@ bool plan_ring(Plan* q, long long n, long long P, int C, int G, int es, bool bwd
   if (bytes < kRingBytes) return false;
   const long long row = (long long)C * es;
   // A chunk is a slot's worth of pixels, fewer where that evens out the blocks.
-  const int slots = 4;
+  const int slots = 3;
   const int slot = kRingSmem / slots / 256 * 256;
   long long r = slot / (bwd ? 2 : 1) / row;
   if (r < 1) return false;

@@ -12,8 +12,8 @@
 // k: weight in dx, both operands in dweight); the layout is a matter of TMA
 // boxes and descriptors, so nothing is transposed in memory.
 //
-//   tile      128 rows x BN (64, 128 or 256) columns, K in steps of 64; where
-//             there is work for all, a pair of blocks shares 256 rows
+//   tile      128 rows x BN (64, 128 or 256) columns, K in steps of 64 (FP32:
+//             32); where there is work for all, a pair of blocks shares 256 rows
 //   operands  TMA, 128-byte swizzle, a ring of stages; out-of-range rows,
 //             columns and k are zero filled, which covers every ragged size
 //   issue     tcgen05.mma of 128 x BN x 16 by one thread; two TMEM
@@ -29,11 +29,15 @@
 // rounding in dz. dz is rounded to the data's type, as an operand of the
 // tensor cores has to be; the bias gradient sums it before that rounding.
 //
-// FP32 data: every operand is split once into three bf16 parts that hold its
-// 24 bits, x = x0 + x1 + x2, and a K step issues the six products whose size is
-// above 2^-24 of x0 y0. Exponents stay in range (bf16 has FP32's). Each K block
-// has an accumulator of its own, and the epilogue's registers add the blocks: a
-// chain of 384 tensor-core additions (k = 1024) left a 2-norm error of 4.9e-6.
+// FP32 data: the tensor cores multiply bf16, so every value is split into three
+// bf16 parts that hold its 24 bits, x = x0 + x1 + x2, and a K step issues the six
+// products whose size is above 2^-24 of x0 y0 (exponents stay in range: bf16 has
+// FP32's). The epilogue's warps split the operands on their way: FP32 tiles come
+// by TMA, their parts go to a second ring as core matrices (16 bytes = 8 values
+// along the contiguous axis). A split in a pass of its own moved 2.5 times the
+// bytes (65536 x 256 -> 64, training: 199 us). Each K block has an accumulator
+// of its own, and the epilogue's registers add the blocks: a chain of 384
+// tensor-core additions (k = 1024) left a 2-norm error of 4.9e-6.
 //
 // dweight sums over all rows: its K axis is split over the SMs left without a
 // tile, FP32 partials are added in a fixed order.
@@ -58,7 +62,8 @@ int max_smem_optin();
 
 namespace {
 
-constexpr int kBM = 128, kBK = 64;
+constexpr int kBM = 128;
+__host__ __device__ constexpr int block_k(int parts) { return parts == 3 ? 32 : 64; }
 constexpr int kEpiWarps = 8;
 constexpr int kFirstEpi = 4;  // warps 0-3: TMA, MMA, TMEM allocation, none
 constexpr int kThreads = 32 * (kFirstEpi + kEpiWarps);
@@ -86,15 +91,17 @@ struct GemmParams {
 __host__ __device__ constexpr int box_row(int bn, int es) { return bn / 2 * es < 128 ? 64 : 128; }
 
 struct SmemLayout {
-  uint32_t stage, boxes, bias, total;
+  uint32_t stage, planes, boxes, bias, total;
 };
 __host__ __device__ inline SmemLayout smem_layout(int cg, int parts, int bn, int row, int stages,
                                                   int nbuf) {
   SmemLayout L;
-  L.stage = (uint32_t)parts * (kBM + bn / cg) * kBK * 2;
-  L.boxes = L.stage * stages;
+  // a stage: 64 k of 16-bit values or 32 of FP32; FP32: two sets of parts
+  L.stage = (uint32_t)(kBM + bn / cg) * 128;
+  L.planes = L.stage * stages;
+  L.boxes = L.planes + (parts == 3 ? 2 * 3 * (kBM + bn) * 64 : 0);
   L.bias = L.boxes + kEpiWarps * nbuf * 32 * row;
-  L.total = L.bias + kEpiWarps * (bn / 2) * 4 + 1024;  // + alignment of the base
+  L.total = L.bias + (parts == 3 ? 0 : kEpiWarps * (bn / 2) * 4) + 1024;  // + alignment
   return L;
 }
 
@@ -254,7 +261,7 @@ __device__ __forceinline__ void tile_at(const GemmParams& p, int t, int& tm, int
 }
 
 // T: the type of out, in and bias (kPartial: out is FP32). PARTS: 1, or 3 for
-// FP32 data split into bf16 parts. CG: blocks that share a tile.
+// FP32 data, split into bf16 parts. CG: blocks that share a tile.
 template <typename T, int BN, int PARTS, Epi kEpi, int CG>
 __global__ void __launch_bounds__(kThreads, 1)
 linear_gemm_kernel(const __grid_constant__ GemmParams p) {
@@ -266,10 +273,13 @@ linear_gemm_kernel(const __grid_constant__ GemmParams p) {
   constexpr int kCB = kRow / (int)sizeof(To);      // columns of a box
   constexpr int kBoxes = kHalf / kCB;
   constexpr int kSub = kCB / 32;                   // steps of 32 columns
+  constexpr int kBK = block_k(PARTS);
+  constexpr int kRows64 = PARTS == 3 ? 32 : 64;    // MN-major: contiguous values of a box
   constexpr int kBNb = BN / CG;                    // columns of B this block holds
   constexpr int kPer = 16 / (int)sizeof(To);       // values of a 16-byte chunk
   extern __shared__ uint8_t smem_raw[];
   __shared__ uint64_t full[kMaxStages], empty[kMaxStages], acc_full[2], acc_empty[2];
+  __shared__ uint64_t parts_full[2], parts_empty[2];
   __shared__ uint64_t in_full[kEpiWarps][kMaxBufs], drained;
   __shared__ uint32_t tmem_base_s;
   __shared__ int abort_s;
@@ -285,11 +295,13 @@ linear_gemm_kernel(const __grid_constant__ GemmParams p) {
   if (threadIdx.x == 0) {
     for (int i = 0; i < p.stages; ++i) {
       tc::mbar_init(&full[i], 1);
-      tc::mbar_init(&empty[i], 1);
+      tc::mbar_init(&empty[i], PARTS == 3 ? kEpiWarps : 1);
     }
     for (int i = 0; i < 2; ++i) {
       tc::mbar_init(&acc_full[i], 1);
       tc::mbar_init(&acc_empty[i], CG * kEpiWarps);
+      tc::mbar_init(&parts_full[i], kEpiWarps);
+      tc::mbar_init(&parts_empty[i], 1);
     }
     for (int w = 0; w < kEpiWarps; ++w)
       for (int i = 0; i < p.nbuf; ++i) tc::mbar_init(&in_full[w][i], 1);
@@ -304,7 +316,8 @@ linear_gemm_kernel(const __grid_constant__ GemmParams p) {
   tc::tc_fence_after();
   const uint32_t tmem = tmem_base_s;
 
-  constexpr uint32_t kPartA = kBM * kBK * 2, kPartB = kBNb * kBK * 2;  // bytes of one part
+  // bytes of A in a stage; of one part of A and of B
+  constexpr uint32_t kStageA = kBM * 128, kPartA = kBM * kBK * 2, kPartB = kBNb * kBK * 2;
   if (warp == 0) {
     {  // ---- operand copies ----
       const bool lead = tc::elect_one();
@@ -324,27 +337,27 @@ linear_gemm_kernel(const __grid_constant__ GemmParams p) {
             break;
           }
           uint8_t* a = smem + s * L.stage;
-          uint8_t* b = a + PARTS * kPartA;
+          uint8_t* b = a + kStageA;
           uint32_t bar = 0;
           if constexpr (CG == 2) bar = leader_addr(&full[s]);
           if (lead) {
             // the even block's barrier counts both blocks' bytes
             if (rank == 0) tc::mbar_arrive_expect_tx(&full[s], CG * L.stage);
-            // K-major: one box of [parts][rows][64 k]; MN-major: a box of
-            // [parts][64 k][64 rows] for every 64 rows
+            // K-major: one box of [rows][128 bytes of k]; MN-major: a box of
+            // [k][128 bytes of rows] for every 64 (FP32: 32) rows
             if (!p.a_mn) {
               load_box<CG>(a, &p.a, kb * kBK, ra, &full[s], bar);
             } else {
 #pragma unroll
-              for (int j = 0; j < kBM / 64; ++j)
-                load_box<CG>(a + j * PARTS * 8192, &p.a, ra + j * 64, kb * kBK, &full[s], bar);
+              for (int j = 0; j < kBM / kRows64; ++j)
+                load_box<CG>(a + j * kBK * 128, &p.a, ra + j * kRows64, kb * kBK, &full[s], bar);
             }
             if (!p.b_mn) {
               load_box<CG>(b, &p.b, kb * kBK, rb, &full[s], bar);
             } else {
 #pragma unroll
-              for (int j = 0; j < kBNb / 64; ++j)
-                load_box<CG>(b + j * PARTS * 8192, &p.b, rb + j * 64, kb * kBK, &full[s], bar);
+              for (int j = 0; j < kBNb / kRows64; ++j)
+                load_box<CG>(b + j * kBK * 128, &p.b, rb + j * kRows64, kb * kBK, &full[s], bar);
             }
           }
           __syncwarp();
@@ -382,20 +395,31 @@ linear_gemm_kernel(const __grid_constant__ GemmParams p) {
             tc::tc_fence_after();
           }
           const uint32_t d = tmem + (ti & 1) * BN;
-          const int s = it % p.stages;
-          if (!warp_wait(&full[s], (it / p.stages) & 1, abort_flag)) {
+          // the operands' slot: the stage itself, or (FP32 data) its parts
+          const int s = PARTS == 3 ? it & 1 : it % p.stages;
+          const uint32_t phase = PARTS == 3 ? (it >> 1) & 1 : (it / p.stages) & 1;
+          if (!warp_wait(PARTS == 3 ? &parts_full[s] : &full[s], phase, abort_flag)) {
             if (lead) give_up(abort_flag, p.status, 93);
             ok = false;
             break;
           }
-          const uint32_t sa = tc::smem_u32(smem + s * L.stage);
-          const uint32_t sb = sa + PARTS * kPartA;
-          const uint64_t ad = p.a_mn ? tc::smem_desc_sw128_mn(sa, PARTS * 8192)
-                                     : tc::smem_desc_sw128(sa);
-          const uint64_t bd = p.b_mn ? tc::smem_desc_sw128_mn(sb, PARTS * 8192)
-                                     : tc::smem_desc_sw128(sb);
-          // descriptor units are 16 bytes
-          const uint32_t ak = (p.a_mn ? 2048 : 32) >> 4, bk = (p.b_mn ? 2048 : 32) >> 4;
+          uint64_t ad, bd;
+          uint32_t ak, bk;  // a K step of 16, in descriptor units of 16 bytes
+          if constexpr (PARTS == 1) {
+            const uint32_t sa = tc::smem_u32(smem + s * L.stage);
+            const uint32_t sb = sa + kStageA;
+            ad = p.a_mn ? tc::smem_desc_sw128_mn(sa, 8192) : tc::smem_desc_sw128(sa);
+            bd = p.b_mn ? tc::smem_desc_sw128_mn(sb, 8192) : tc::smem_desc_sw128(sb);
+            ak = (p.a_mn ? 2048 : 32) >> 4;
+            bk = (p.b_mn ? 2048 : 32) >> 4;
+          } else {  // core matrices, [8 values][outer index]
+            const uint32_t sa = tc::smem_u32(smem + L.planes + s * 3 * (kPartA + kPartB));
+            const uint32_t sb = sa + 3 * kPartA;
+            ad = p.a_mn ? tc::smem_desc(sa, 128, kBK * 16) : tc::smem_desc(sa, kBM * 16, 128);
+            bd = p.b_mn ? tc::smem_desc(sb, 128, kBK * 16) : tc::smem_desc(sb, BN * 16, 128);
+            ak = (p.a_mn ? 256 : 2 * kBM * 16) >> 4;
+            bk = (p.b_mn ? 256 : 2 * BN * 16) >> 4;
+          }
           const int ksteps = kb == p.kblocks - 1 ? p.last_ksteps : kBK / 16;
           auto products = [&](auto steps) {
             if constexpr (PARTS == 1) {
@@ -403,7 +427,7 @@ linear_gemm_kernel(const __grid_constant__ GemmParams p) {
               for (int ks = 0; ks < steps; ++ks)
                 mma<CG>(d, ad + ks * ak, bd + ks * bk, p.idesc, (!first || ks > 0) ? 1u : 0u);
             } else {
-              const uint32_t ap = (p.a_mn ? 8192u : kPartA) >> 4, bp = (p.b_mn ? 8192u : kPartB) >> 4;
+              constexpr uint32_t ap = kPartA >> 4, bp = kPartB >> 4;
               // the small products first, while the sum is small
 #pragma unroll
               for (int ks = 0; ks < steps; ++ks) {
@@ -422,7 +446,7 @@ linear_gemm_kernel(const __grid_constant__ GemmParams p) {
           if (lead) {
             if (ksteps == kBK / 16) products(std::integral_constant<int, kBK / 16>());
             else products(ksteps);
-            commit<CG>(&empty[s]);
+            commit<CG>(PARTS == 3 ? &parts_empty[s] : &empty[s]);
             if constexpr (PARTS == 3) commit<CG>(&acc_full[ti & 1]);
           }
           __syncwarp();
@@ -484,6 +508,75 @@ linear_gemm_kernel(const __grid_constant__ GemmParams p) {
     if (p.tma_io && has_in && lead)
       for (int i = 0; i < ahead; ++i) load_next();
     bool ok = true;
+    // FP32 data: the K blocks of this block's tiles in order, each split by all
+    // eight warps; a 16-byte row of a part holds 8 values along the contiguous
+    // axis, rows lie along the other one
+    uint32_t done = 0, blocks = 0;  // split so far, and in all
+    if constexpr (PARTS == 3) {
+      for (int t = first_tile; t < p.num_tiles; t += tile_step) {
+        const int sp = t / (p.tiles_m * p.tiles_n);
+        blocks += (uint32_t)((long long)p.kblocks * (sp + 1) / p.splits) -
+                  (uint32_t)((long long)p.kblocks * sp / p.splits);
+      }
+    }
+    int stage = 0;
+    uint32_t turn = 0;
+    auto split_operand = [&](const uint8_t* raw, uint8_t* dst, bool mn, auto width) {
+      constexpr int kW = decltype(width)::value;  // rows (columns) of the operand
+      constexpr uint32_t kPart = kW * kBK * 2;
+#pragma unroll
+      for (int i = 0; i < kW * kBK / 8; i += 32 * kEpiWarps) {
+        const int item = i + ew * 32 + lane;
+        // K-major: [k / 8][row]; MN-major: [row / 8][k]
+        const int o = mn ? item % kBK : item % kW, g = mn ? item / kBK : item / kW;
+        const uint8_t* line = raw + (mn ? (g / 4) * kBK * 128 + o * 128 : o * 128);
+        const int c = mn ? (g % 4) * 2 : g * 2;
+        float v[8];
+        *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(line + ((c ^ (o & 7)) * 16));
+        *reinterpret_cast<float4*>(v + 4) =
+            *reinterpret_cast<const float4*>(line + (((c + 1) ^ (o & 7)) * 16));
+        uint32_t part[3][4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          // the first part is cut off, not rounded: it cannot overflow
+          const uint32_t a = __float_as_uint(v[2 * e]), b = __float_as_uint(v[2 * e + 1]);
+          part[0][e] = __byte_perm(a, b, 0x7632);
+          const float ra = v[2 * e] - __uint_as_float(a & 0xffff0000u);
+          const float rb = v[2 * e + 1] - __uint_as_float(b & 0xffff0000u);
+          part[1][e] = pack2<__nv_bfloat16>(ra, rb);
+          const float2 h = unpack2<__nv_bfloat16>(part[1][e]);
+          part[2][e] = pack2<__nv_bfloat16>(ra - h.x, rb - h.y);
+        }
+#pragma unroll
+        for (int q3 = 0; q3 < 3; ++q3)
+          *reinterpret_cast<uint4*>(dst + q3 * kPart + item * 16) =
+              make_uint4(part[q3][0], part[q3][1], part[q3][2], part[q3][3]);
+      }
+    };
+    auto split_next = [&]() -> bool {
+      if (done == blocks) return true;
+      const int b = done & 1;
+      if (!warp_wait(&full[stage], turn, abort_flag) ||
+          !warp_wait(&parts_empty[b], ((done >> 1) & 1) ^ 1, abort_flag))
+        return false;
+      const uint8_t* raw = smem + stage * L.stage;
+      uint8_t* dst = smem + L.planes + b * 3 * (kPartA + kPartB);
+      split_operand(raw, dst, p.a_mn, std::integral_constant<int, kBM>());
+      split_operand(raw + kStageA, dst + 3 * kPartA, p.b_mn, std::integral_constant<int, kBNb>());
+      tc::fence_proxy_async_smem();
+      __syncwarp();
+      if (lead) {
+        tc::mbar_arrive(&empty[stage]);
+        tc::mbar_arrive(&parts_full[b]);
+      }
+      ++done;
+      if (++stage == p.stages) {
+        stage = 0;
+        turn ^= 1;
+      }
+      return true;
+    };
+    if constexpr (PARTS == 3) ok = split_next();
     for (int t = first_tile; t < p.num_tiles && ok; t += tile_step) {
       int tm, tn, sp;
       tile_at(p, t, tm, tn, sp);
@@ -491,7 +584,7 @@ linear_gemm_kernel(const __grid_constant__ GemmParams p) {
       const int row = row0 + lane;
       const int col0 = tn * BN + half * kHalf;
       const uint32_t tcol = tmem + ((uint32_t)(quad * 32) << 16) + half * kHalf;
-      if constexpr (kEpi != kPartial) {
+      if constexpr (kEpi != kPartial && PARTS == 1) {
         if (bias != nullptr) {
 #pragma unroll
           for (int i = lane; i < kHalf; i += 32)
@@ -505,8 +598,11 @@ linear_gemm_kernel(const __grid_constant__ GemmParams p) {
         const int kb1 = (int)((long long)p.kblocks * (sp + 1) / p.splits);
 #pragma unroll
         for (int i = 0; i < kHalf; ++i) sum[i] = 0.f;
+        // the parts of the next block (the next tile's at the end) are made
+        // while this one is multiplied
         for (int kb = kb0; kb < kb1; ++kb, ++ti) {
-          ok = warp_wait(&acc_full[ti & 1], (ti >> 1) & 1, abort_flag);
+          ok = split_next();
+          ok = ok && warp_wait(&acc_full[ti & 1], (ti >> 1) & 1, abort_flag);
           if (!ok) break;
           tc::tc_fence_after();
 #pragma unroll
@@ -604,14 +700,22 @@ linear_gemm_kernel(const __grid_constant__ GemmParams p) {
           if (live) {
             if constexpr (kEpi != kPartial) {
               if (bias != nullptr) {
-                const float4* bs = reinterpret_cast<const float4*>(bias_s + j * kCB + sub * 32);
+                if constexpr (PARTS == 1) {
+                  const float4* bs = reinterpret_cast<const float4*>(bias_s + j * kCB + sub * 32);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                  const float4 u = bs[i];
-                  w[4 * i] += u.x;
-                  w[4 * i + 1] += u.y;
-                  w[4 * i + 2] += u.z;
-                  w[4 * i + 3] += u.w;
+                  for (int i = 0; i < 8; ++i) {
+                    const float4 u = bs[i];
+                    w[4 * i] += u.x;
+                    w[4 * i + 1] += u.y;
+                    w[4 * i + 2] += u.z;
+                    w[4 * i + 3] += u.w;
+                  }
+                } else {  // no room for it beside the parts
+#pragma unroll
+                  for (int i = 0; i < 32; ++i) {
+                    const int c = c0 + sub * 32 + i;
+                    w[i] += ldg_f32<T>(bias + (c < p.N ? c : p.N - 1));
+                  }
                 }
               }
               if constexpr (kEpi == kOut) act_values<kFast, 32>(p.act, w);
@@ -694,49 +798,28 @@ linear_gemm_kernel(const __grid_constant__ GemmParams p) {
 }
 
 // --------------------------------------------------------- small kernels ----
-// Rows of `src` as operand planes [parts][rows][pitch] (pitch a multiple of 8,
-// zero padded): FP32 as three bf16 parts, 16-bit data as it is. The first part
-// is cut off, not rounded, so that it never overflows; an infinity or NaN keeps
-// its place in the first part.
+// Rows of `src` copied to a pitch (a multiple of 8 values) that TMA can address.
 template <typename T>
 __global__ void __launch_bounds__(256) linear_stage_kernel(const T* __restrict__ src, long long ld,
                                                            long long rows, int cols, int pitch,
                                                            uint4* __restrict__ dst) {
-  const int per = pitch / 8;
+  constexpr int kPer = 16 / (int)sizeof(T);
+  const int per = pitch / kPer;
   const long long total = rows * per;
   const bool vec = ld * sizeof(T) % 16 == 0 && (uintptr_t)src % 16 == 0;
   for (long long i = blockIdx.x * (long long)blockDim.x + threadIdx.x; i < total;
        i += (long long)gridDim.x * blockDim.x) {
     const long long r = i / per;
-    const int c = (int)(i - r * per) * 8;
-    union { uint4 u[sizeof(T) / 2]; T e[8]; } v;
+    const int c = (int)(i - r * per) * kPer;
+    union { uint4 u; T e[kPer]; } v;
     const T* s = src + r * ld + c;
-    if (vec && c + 8 <= cols) {
-#pragma unroll
-      for (int k = 0; k < (int)sizeof(T) / 2; ++k) v.u[k] = __ldg(reinterpret_cast<const uint4*>(s) + k);
+    if (vec && c + kPer <= cols) {
+      v.u = __ldg(reinterpret_cast<const uint4*>(s));
     } else {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) v.e[k] = c + k < cols ? s[k] : from_f32<T>(0.f);
+      for (int k = 0; k < kPer; ++k) v.e[k] = c + k < cols ? s[k] : from_f32<T>(0.f);
     }
-    if constexpr (sizeof(T) == 2) {
-      dst[i] = v.u[0];
-    } else {
-      union { uint4 u; __nv_bfloat16 e[8]; } o[3];
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const float f = v.e[k];
-        const __nv_bfloat16 h0 = __float2bfloat16_rz(f);
-        const float r1 = f - __bfloat162float(h0);
-        const bool fin = isfinite(f);
-        const __nv_bfloat16 h1 = __float2bfloat16_rn(fin ? r1 : 0.f);
-        const float r2 = fin ? r1 - __bfloat162float(h1) : 0.f;
-        o[0].e[k] = h0;
-        o[1].e[k] = h1;
-        o[2].e[k] = __float2bfloat16_rn(r2);
-      }
-#pragma unroll
-      for (int k = 0; k < 3; ++k) dst[k * total + i] = o[k].u;
-    }
+    dst[i] = v.u;
   }
 }
 
@@ -849,14 +932,12 @@ __global__ void __launch_bounds__(256) linear_rows_kernel(const T* __restrict__ 
 size_t up256(size_t v) { return (v + 255) / 256 * 256; }
 int round8(int v) { return (v + 7) / 8 * 8; }
 
-// A tensor-core operand in memory: rows x cols of 16-bit values, `parts`
-// planes of rows * pitch.
+// An operand in memory: rows x cols values, `pitch` values from row to row.
 struct Operand {
   const void* ptr;
   long long rows;
   int cols;
   long long pitch;
-  int parts;
 };
 
 template <typename T> struct OpOf { using type = T; };
@@ -867,14 +948,14 @@ int small_grid(long long items) {
   return (int)(want < 1 ? 1 : want < most ? want : most);
 }
 
-size_t plane_bytes(long long rows, int cols, int parts) {
-  return up256((size_t)parts * rows * round8(cols) * 2);
+size_t staged_bytes(long long rows, int cols, int es) {
+  return up256((size_t)rows * round8(cols) * es);
 }
 
 template <typename T>
 int stage(const void* src, long long ld, long long rows, int cols, void* dst, cudaStream_t st) {
   const int pitch = round8(cols);
-  linear_stage_kernel<T><<<small_grid(rows * (pitch / 8)), 256, 0, st>>>(
+  linear_stage_kernel<T><<<small_grid(rows * (pitch * (int)sizeof(T) / 16)), 256, 0, st>>>(
       static_cast<const T*>(src), ld, rows, cols, pitch, static_cast<uint4*>(dst));
   DDPM_CHECK_LAUNCH("linear_stage_kernel");
   return DDPM_OK;
@@ -890,20 +971,20 @@ struct Tile {
 // shared memory need: a block's operands are written once and read once per
 // product) plus a constant for filling and draining.
 Tile pick_tile(long long m, int n, long long k, int parts, int splits) {
-  const int sms = gencat::num_sms();
-  const long long kb = ((k + kBK - 1) / kBK + splits - 1) / splits;
-  const int products = parts == 3 ? 6 : 1;
+  const int sms = gencat::num_sms(), bk = block_k(parts);
+  const long long kb = ((k + bk - 1) / bk + splits - 1) / splits;
   Tile best{64, 1};
   double least = 0;
-  for (int cg = 1; cg <= 2; ++cg)
-    for (int bn = parts == 3 ? 128 : 256; bn >= (cg == 2 ? (parts == 3 ? 128 : 256) : 64); bn /= 2) {
+  for (int cg = 1; cg <= (parts == 3 ? 1 : 2); ++cg)
+    for (int bn = parts == 3 ? 128 : 256; bn >= (cg == 2 ? 256 : 64); bn /= 2) {
       const long long tiles =
           ((m + kBM * cg - 1) / (kBM * cg)) * ((n + bn - 1) / bn) * splits;
       const long long units = sms / cg;
       const long long rounds = (tiles + units - 1) / units;
-      const double mma = products * 2.0 * bn;
-      const double move = (parts * (kBM + bn / cg) + products * (kBM + bn / cg)) * (double)kBK * 2 / 128;
-      const double t = rounds * (kb * (mma > move ? mma : move) + 1000.0 + 4.0 * bn);
+      // FP32: splitting the operands is the longest part of a block
+      const double mma = 2.0 * bn, move = 2.0 * (kBM + bn / cg);
+      const double block = parts == 3 ? 150.0 + 3.2 * (kBM + bn) : mma > move ? mma : move;
+      const double t = rounds * (kb * block + 1000.0 + 4.0 * bn);
       if (least == 0 || t < least) {
         least = t;
         best = Tile{bn, cg};
@@ -963,9 +1044,8 @@ int launch_gemm_as(GemmParams& p, cudaStream_t st) {
 template <typename T, Epi kEpi>
 int launch_gemm(GemmParams& p, Tile t, cudaStream_t st) {
   if constexpr (sizeof(T) == 4) {
-    return t.cg == 2     ? launch_gemm_as<T, 128, 3, kEpi, 2>(p, st)
-           : t.bn == 128 ? launch_gemm_as<T, 128, 3, kEpi, 1>(p, st)
-                         : launch_gemm_as<T, 64, 3, kEpi, 1>(p, st);
+    return t.bn == 128 ? launch_gemm_as<T, 128, 3, kEpi, 1>(p, st)
+                       : launch_gemm_as<T, 64, 3, kEpi, 1>(p, st);
   } else {
     return t.cg == 2     ? launch_gemm_as<T, 256, 1, kEpi, 2>(p, st)
            : t.bn == 256 ? launch_gemm_as<T, 256, 1, kEpi, 1>(p, st)
@@ -974,13 +1054,16 @@ int launch_gemm(GemmParams& p, Tile t, cudaStream_t st) {
   }
 }
 
-int operand_map(CUtensorMap* map, const Operand& o, bool mn_major, int tile_rows, bool bf16) {
-  // K-major: [parts][rows][k], box 64 k x tile rows; MN-major: the operand's
-  // rows are the contraction's k, box 64 columns x 64 k
-  const uint64_t dims[3] = {(uint64_t)o.cols, (uint64_t)o.rows, (uint64_t)o.parts};
-  const uint64_t strides[2] = {(uint64_t)o.pitch * 2, (uint64_t)o.rows * o.pitch * 2};
-  const uint32_t box[3] = {64, (uint32_t)(mn_major ? kBK : tile_rows), (uint32_t)o.parts};
-  return encode_tmap(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+int operand_map(CUtensorMap* map, const Operand& o, bool mn_major, int tile_rows, int es, bool bf16) {
+  // 128 bytes along the contiguous axis; K-major: x the tile's rows, MN-major
+  // (the operand's rows are the contraction's k): x a block of k
+  const uint64_t dims[3] = {(uint64_t)o.cols, (uint64_t)o.rows, 1};
+  const uint64_t strides[2] = {(uint64_t)o.pitch * es, (uint64_t)o.rows * o.pitch * es};
+  const uint32_t box[3] = {(uint32_t)(128 / es), (uint32_t)(mn_major ? 128 / es : tile_rows), 1};
+  return encode_tmap(map,
+                     es == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                     : bf16  ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                             : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
                      3, o.ptr, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
@@ -1031,6 +1114,7 @@ int run_gemm(const Gemm& g, cudaStream_t st) {
   p.tiles_n = (g.N + bn - 1) / bn;
   p.splits = g.splits;
   p.num_tiles = p.tiles_m * p.tiles_n * g.splits;
+  constexpr int kBK = block_k(sizeof(T) == 4 ? 3 : 1);
   p.kblocks = (int)((g.K + kBK - 1) / kBK);
   p.last_ksteps = (int)((g.K - (long long)(p.kblocks - 1) * kBK + 15) / 16);
   p.M = (int)g.M;
@@ -1048,9 +1132,9 @@ int run_gemm(const Gemm& g, cudaStream_t st) {
   p.tma_io = tma_ready(g.out, g.ld_out, es) && (g.in == nullptr || tma_ready(g.in, g.ld_in, es));
   int rc = gencat::status_ptr(&p.status);
   if (rc) return rc;
-  rc = operand_map(&p.a, g.a, g.a_mn, kBM, kBf16);
+  rc = operand_map(&p.a, g.a, g.a_mn, kBM, (int)sizeof(T), kBf16);
   if (rc) return rc;
-  rc = operand_map(&p.b, g.b, g.b_mn, bn / g.tile.cg, kBf16);
+  rc = operand_map(&p.b, g.b, g.b_mn, bn / g.tile.cg, (int)sizeof(T), kBf16);
   if (rc) return rc;
   const int row = box_row(bn, es);
   if (p.tma_io) {
@@ -1095,19 +1179,19 @@ LinearPlan plan_linear(const LinearShape& s, bool bwd) {
     return o;
   };
   if (!q.rows_path) {
-    q.stage_x = f32 || !s.aligned || s.ldx % 8;
-    q.stage_w = f32 || !s.aligned || s.k % 8;
-    q.x_off = q.stage_x ? take(plane_bytes(s.m, s.k, q.parts)) : 0;
-    q.w_off = q.stage_w ? take(plane_bytes(s.n, s.k, q.parts)) : 0;
+    const int whole = 16 / es;  // values of a 16-byte word
+    q.stage_x = !s.aligned || s.ldx % whole;
+    q.stage_w = !s.aligned || s.k % whole;
+    q.x_off = q.stage_x ? take(staged_bytes(s.m, s.k, es)) : 0;
+    q.w_off = q.stage_w ? take(staged_bytes(s.n, s.k, es)) : 0;
   }
   q.tile_z = pick_tile(s.m, s.n, s.k, q.parts, 1);
   if (bwd) {
     const bool recompute = s.act != DDPM_ACT_NONE;
-    // dz as the data's type (recomputed), then as operand planes where that is
-    // not one already
+    // dz: recomputed, or dy, copied where TMA cannot address it
     if (recompute) q.dz_off = take((size_t)s.m * round8(s.n) * es);
-    q.stage_dz = f32 || (!recompute && (!s.aligned || s.n % 8));
-    q.dzp_off = q.stage_dz ? take(plane_bytes(s.m, s.n, q.parts)) : 0;
+    q.stage_dz = !recompute && (!s.aligned || s.n % (16 / es));
+    q.dzp_off = q.stage_dz ? take(staged_bytes(s.m, s.n, es)) : 0;
     q.tile_x = pick_tile(s.m, s.k, s.n, q.parts, 1);
     if (recompute) {
       q.colsum_rows = (s.m + 31) / 32;  // a row of sums for every 32 rows
@@ -1123,7 +1207,8 @@ LinearPlan plan_linear(const LinearShape& s, bool bwd) {
     q.colsum_off = take((size_t)q.colsum_rows * s.n * 4);
     // dweight: the rows are split over the SMs that have no tile, at least four
     // K blocks a split
-    const long long kb = (s.m + kBK - 1) / kBK;
+    const int bk = block_k(q.parts);
+    const long long kb = (s.m + bk - 1) / bk;
     q.tile_w = pick_tile(s.n, s.k, s.m, q.parts, 1);
     q.splits_w = 1;
     {
@@ -1178,10 +1263,6 @@ int check_linear(long long m, int n, int k, long long ldx, int act, int dt) {
   return DDPM_OK;
 }
 
-Operand make_operand(const void* ptr, long long rows, int cols, long long pitch, int parts) {
-  return Operand{ptr, rows, cols, pitch, parts};
-}
-
 template <typename T>
 int forward(const LinearShape& s, const LinearPlan& q, const void* x, const void* w,
             const void* bias, const void* res, void* out, uint8_t* ws, cudaStream_t st) {
@@ -1191,10 +1272,10 @@ int forward(const LinearShape& s, const LinearPlan& q, const void* x, const void
   if (q.stage_x && (rc = stage<T>(x, s.ldx, s.m, s.k, ws + q.x_off, st))) return rc;
   if (q.stage_w && (rc = stage<T>(w, s.k, s.n, s.k, ws + q.w_off, st))) return rc;
   Gemm g{};
-  g.a = q.stage_x ? make_operand(ws + q.x_off, s.m, s.k, round8(s.k), q.parts)
-                  : make_operand(x, s.m, s.k, s.ldx, 1);
-  g.b = q.stage_w ? make_operand(ws + q.w_off, s.n, s.k, round8(s.k), q.parts)
-                  : make_operand(w, s.n, s.k, s.k, 1);
+  g.a = q.stage_x ? Operand{ws + q.x_off, s.m, s.k, round8(s.k)}
+                  : Operand{x, s.m, s.k, s.ldx};
+  g.b = q.stage_w ? Operand{ws + q.w_off, s.n, s.k, round8(s.k)}
+                  : Operand{w, s.n, s.k, s.k};
   g.M = s.m;
   g.N = s.n;
   g.K = s.k;
@@ -1219,10 +1300,10 @@ int backward(const LinearShape& s, const LinearPlan& q, const void* x, const voi
     return rc;
   if (q.stage_w && (recompute || gx) && (rc = stage<T>(w, s.k, s.n, s.k, ws + q.w_off, st)))
     return rc;
-  const Operand xo = q.stage_x ? make_operand(ws + q.x_off, s.m, s.k, round8(s.k), q.parts)
-                               : make_operand(x, s.m, s.k, s.ldx, 1);
-  const Operand wo = q.stage_w ? make_operand(ws + q.w_off, s.n, s.k, round8(s.k), q.parts)
-                               : make_operand(w, s.n, s.k, s.k, 1);
+  const Operand xo = q.stage_x ? Operand{ws + q.x_off, s.m, s.k, round8(s.k)}
+                               : Operand{x, s.m, s.k, s.ldx};
+  const Operand wo = q.stage_w ? Operand{ws + q.w_off, s.n, s.k, round8(s.k)}
+                               : Operand{w, s.n, s.k, s.k};
   float* colsum = reinterpret_cast<float*>(ws + q.colsum_off);
   const void* dz = dy;
   long long ld_dz = s.n;
@@ -1257,10 +1338,10 @@ int backward(const LinearShape& s, const LinearPlan& q, const void* x, const voi
     DDPM_CHECK_LAUNCH("linear_fold_rows_kernel");
   }
   if (!gx && !gw) return DDPM_OK;
-  Operand zo = make_operand(dz, s.m, s.n, ld_dz, 1);
+  Operand zo = Operand{dz, s.m, s.n, ld_dz};
   if (q.stage_dz) {
     if ((rc = stage<T>(dz, ld_dz, s.m, s.n, ws + q.dzp_off, st))) return rc;
-    zo = make_operand(ws + q.dzp_off, s.m, s.n, round8(s.n), q.parts);
+    zo = Operand{ws + q.dzp_off, s.m, s.n, round8(s.n)};
   }
   if (gx) {
     Gemm g{};

@@ -97,6 +97,15 @@ def test_long_sums(dtype):
     _run(*_case(200, 72, 6000, dtype, seed=5), "gelu")
 
 
+@pytest.mark.parametrize("dtype", ops.DTYPES)
+@pytest.mark.parametrize("m,n,k", [(5000, 1500, 300), (2600, 2049, 96), (20_000, 256, 264)])
+def test_several_tiles_a_block(m, n, k, dtype):
+    """Tiles of pairs of blocks, blocks with several tiles, ragged last tiles."""
+    x, w, b, res, dy = _case(m, n, k, dtype, seed=8)
+    _run(x, w, b, res, dy, "gelu")
+    _run(x, w, None, None, dy, None)
+
+
 def test_float32_keeps_its_digits():
     """The 2-norm of the error stays near a single-precision product's, not at
     the 2^-17 of two bf16 parts."""
@@ -242,6 +251,26 @@ def test_same_bits_every_time_and_on_other_streams():
     torch.cuda.synchronize()
     for got in results:
         assert all(torch.equal(a, e) for a, e in zip(got, want))
+
+
+def test_calls_from_new_threads():
+    """A thread whose first CUDA call is the operator's, once everything that is
+    looked up once has been looked up."""
+    import threading
+
+    from dynamicconvolutionoperator_b200 import linear_act
+
+    x, w, b, _, _ = _case(300, 64, 64, torch.bfloat16)
+    want = linear_act(x, w, b)
+    torch.cuda.synchronize()
+    got = []
+    threads = [threading.Thread(target=lambda: got.append(linear_act(x, w, b))) for _ in range(3)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert len(got) == 3 and all(torch.equal(g, want) for g in got)
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.float16])

@@ -97,7 +97,7 @@ def test_linear_abi_argument_errors_without_gpu():
     assert fwd(x=None) == -1 and b"null" in lib.ddpm_last_error()
     assert fwd(x=17) == -1 and b"misaligned" in lib.ddpm_last_error()
     assert fwd(ws=8) == -1 and b"workspace" in lib.ddpm_last_error()
-    assert fwd(dt=0, nbytes=64) == -4 and b"workspace" in lib.ddpm_last_error()
+    assert fwd(dt=0, x=20, nbytes=64) == -4 and b"workspace" in lib.ddpm_last_error()
     assert fwd(x=18, nbytes=64) == -4  # rows that TMA cannot address are copied
     assert fwd(m=1 << 33) == -2
     assert fwd(m=0) == 0
