@@ -18,7 +18,7 @@
 //             columns and k are zero filled, which covers every ragged size
 //   issue     tcgen05.mma of 128 x BN x 16 by one thread; two TMEM
 //             accumulators, so the epilogue of a tile overlaps the next one
-//   epilogue  eight warps (lane = row, two column halves): TMEM -> registers,
+//   epilogue  8 or 16 warps (lane = row, 2 or 4 column parts): TMEM -> registers,
 //             bias, activation, residual -> 128-byte x 32-row boxes in shared
 //             memory -> TMA store. The residual (or dy) comes through the same
 //             boxes by TMA, several boxes ahead.
@@ -32,8 +32,8 @@
 // FP32 data: the tensor cores multiply bf16, so every value is split into three
 // bf16 parts that hold its 24 bits, x = x0 + x1 + x2, and a K step issues the six
 // products whose size is above 2^-24 of x0 y0 (exponents stay in range: bf16 has
-// FP32's). The epilogue's warps split the operands on their way: FP32 tiles come
-// by TMA, their parts go to a second ring as core matrices (16 bytes = 8 values
+// FP32's). Eight more warps split the operands on their way: FP32 tiles come by
+// TMA, their parts go to a second ring as core matrices (16 bytes = 8 values
 // along the contiguous axis). A split in a pass of its own moved 2.5 times the
 // bytes (65536 x 256 -> 64, training: 199 us). Each K block has an accumulator
 // of its own, and the epilogue's registers add the blocks: a chain of 384
@@ -64,12 +64,15 @@ namespace {
 
 constexpr int kBM = 128;
 __host__ __device__ constexpr int block_k(int parts) { return parts == 3 ? 32 : 64; }
-constexpr int kEpiWarps = 8;
 constexpr int kFirstEpi = 4;  // warps 0-3: TMA, MMA, TMEM allocation, none
-constexpr int kThreads = 32 * (kFirstEpi + kEpiWarps);
+constexpr int kSplitWarps = 8;  // FP32 data: warps that split operands, behind the epilogue's
+__host__ __device__ constexpr int gemm_threads(int parts, int ew) {
+  return 32 * (kFirstEpi + ew + (parts == 3 ? kSplitWarps : 0));
+}
 constexpr int kMaxStages = 8, kMaxBufs = 8;
 constexpr uint64_t kWaitNs = 2000000000ull;
 constexpr int kGemvRows = 8;
+constexpr int kShortK = 8;  // K blocks
 
 enum Epi { kOut, kDz, kPartial };
 
@@ -87,21 +90,24 @@ struct GemmParams {
   int* status;
 };
 
-// A box of the epilogue: 32 rows x 128 bytes (64 where half a tile is no wider).
-__host__ __device__ constexpr int box_row(int bn, int es) { return bn / 2 * es < 128 ? 64 : 128; }
+// A box of the epilogue: 32 rows x 128 bytes (64 where a warp has no more
+// columns: a quarter of the warps share each quarter of the rows).
+__host__ __device__ constexpr int box_row(int bn, int ew, int es) {
+  return bn / (ew / 4) * es < 128 ? 64 : 128;
+}
 
 struct SmemLayout {
   uint32_t stage, planes, boxes, bias, total;
 };
-__host__ __device__ inline SmemLayout smem_layout(int cg, int parts, int bn, int row, int stages,
-                                                  int nbuf) {
+__host__ __device__ inline SmemLayout smem_layout(int cg, int parts, int bn, int ew, int row,
+                                                  int stages, int nbuf) {
   SmemLayout L;
   // a stage: 64 k of 16-bit values or 32 of FP32; FP32: two sets of parts
   L.stage = (uint32_t)(kBM + bn / cg) * 128;
   L.planes = L.stage * stages;
   L.boxes = L.planes + (parts == 3 ? 2 * 3 * (kBM + bn) * 64 : 0);
-  L.bias = L.boxes + kEpiWarps * nbuf * 32 * row;
-  L.total = L.bias + (parts == 3 ? 0 : kEpiWarps * (bn / 2) * 4) + 1024;  // + alignment
+  L.bias = L.boxes + ew * nbuf * 32 * row;
+  L.total = L.bias + (parts == 3 ? 0 : bn * 16) + 1024;  // + alignment
   return L;
 }
 
@@ -262,16 +268,17 @@ __device__ __forceinline__ void tile_at(const GemmParams& p, int t, int& tm, int
 
 // T: the type of out, in and bias (kPartial: out is FP32). PARTS: 1, or 3 for
 // FP32 data, split into bf16 parts. CG: blocks that share a tile.
-template <typename T, int BN, int PARTS, Epi kEpi, int CG>
-__global__ void __launch_bounds__(kThreads, 1)
+template <typename T, int BN, int PARTS, Epi kEpi, int CG, int EW>
+__global__ void __launch_bounds__(gemm_threads(PARTS, EW), 1)
 linear_gemm_kernel(const __grid_constant__ GemmParams p) {
   using To = typename std::conditional<kEpi == kPartial, float, T>::type;
   constexpr bool kFast = sizeof(T) == 2;
-  constexpr int kHalf = BN / 2;                    // columns of a warp's part of a tile
-  constexpr int kRow = box_row(BN, sizeof(To));    // bytes of a box row
+  constexpr int kCols = BN / (EW / 4);             // columns of a warp's part of a tile
+  constexpr int kRow = box_row(BN, EW, sizeof(To));  // bytes of a box row
+  constexpr int kFirstSplit = kFirstEpi + EW;
   constexpr int kBox = 32 * kRow;
   constexpr int kCB = kRow / (int)sizeof(To);      // columns of a box
-  constexpr int kBoxes = kHalf / kCB;
+  constexpr int kBoxes = kCols / kCB;
   constexpr int kSub = kCB / 32;                   // steps of 32 columns
   constexpr int kBK = block_k(PARTS);
   constexpr int kRows64 = PARTS == 3 ? 32 : 64;    // MN-major: contiguous values of a box
@@ -280,12 +287,12 @@ linear_gemm_kernel(const __grid_constant__ GemmParams p) {
   extern __shared__ uint8_t smem_raw[];
   __shared__ uint64_t full[kMaxStages], empty[kMaxStages], acc_full[2], acc_empty[2];
   __shared__ uint64_t parts_full[2], parts_empty[2];
-  __shared__ uint64_t in_full[kEpiWarps][kMaxBufs], drained;
+  __shared__ uint64_t in_full[EW][kMaxBufs], drained;
   __shared__ uint32_t tmem_base_s;
   __shared__ int abort_s;
   uint8_t* smem = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-  const SmemLayout L = smem_layout(CG, PARTS, BN, kRow, p.stages, p.nbuf);
+  const SmemLayout L = smem_layout(CG, PARTS, BN, EW, kRow, p.stages, p.nbuf);
   // a shuffle, so that the compiler knows the warp's number to be uniform
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const uint32_t rank = CG == 2 ? cluster_rank() : 0;
@@ -295,15 +302,15 @@ linear_gemm_kernel(const __grid_constant__ GemmParams p) {
   if (threadIdx.x == 0) {
     for (int i = 0; i < p.stages; ++i) {
       tc::mbar_init(&full[i], 1);
-      tc::mbar_init(&empty[i], PARTS == 3 ? kEpiWarps : 1);
+      tc::mbar_init(&empty[i], PARTS == 3 ? 4 : 1);
     }
     for (int i = 0; i < 2; ++i) {
       tc::mbar_init(&acc_full[i], 1);
-      tc::mbar_init(&acc_empty[i], CG * kEpiWarps);
-      tc::mbar_init(&parts_full[i], kEpiWarps);
+      tc::mbar_init(&acc_empty[i], CG * EW);
+      tc::mbar_init(&parts_full[i], 4);
       tc::mbar_init(&parts_empty[i], 1);
     }
-    for (int w = 0; w < kEpiWarps; ++w)
+    for (int w = 0; w < EW; ++w)
       for (int i = 0; i < p.nbuf; ++i) tc::mbar_init(&in_full[w][i], 1);
     tc::mbar_init(&drained, 1);
     abort_s = 0;
@@ -464,12 +471,73 @@ linear_gemm_kernel(const __grid_constant__ GemmParams p) {
       warp_wait(&drained, 0, nullptr);
     }
     __syncwarp();
+  } else if (PARTS == 3 && warp >= kFirstSplit) {  // ---- parts of FP32 operands ----
+    // Two groups of four warps take the K blocks in turn, each into its own set
+    // of parts. A 16-byte row of a part holds 8 values along the contiguous axis;
+    // rows lie along the other one.
+    const int team = (warp - kFirstSplit) >> 2;
+    const int me = ((warp - kFirstSplit) & 3) * 32 + lane;
+    const bool lead = tc::elect_one();
+    uint32_t blocks = 0;
+    for (int t = first_tile; t < p.num_tiles; t += tile_step) {
+      const int sp = t / (p.tiles_m * p.tiles_n);
+      blocks += (uint32_t)((long long)p.kblocks * (sp + 1) / p.splits) -
+                (uint32_t)((long long)p.kblocks * sp / p.splits);
+    }
+    auto split_operand = [&](const uint8_t* raw, uint8_t* dst, bool mn, auto width) {
+      constexpr int kW = decltype(width)::value;  // rows (columns) of the operand
+      constexpr uint32_t kPart = kW * kBK * 2;
+#pragma unroll 4
+      for (int item = me; item < kW * kBK / 8; item += 128) {
+        // K-major: [k / 8][row]; MN-major: [row / 8][k]
+        const int o = mn ? item % kBK : item % kW, g = mn ? item / kBK : item / kW;
+        const uint8_t* line = raw + (mn ? (g / 4) * kBK * 128 + o * 128 : o * 128);
+        const int c = mn ? (g % 4) * 2 : g * 2;
+        const float4 lo = *reinterpret_cast<const float4*>(line + ((c ^ (o & 7)) * 16));
+        const float4 hi = *reinterpret_cast<const float4*>(line + (((c + 1) ^ (o & 7)) * 16));
+        const float v[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+        uint32_t part[3][4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          // the first part is cut off, not rounded: it cannot overflow
+          const uint32_t a = __float_as_uint(v[2 * e]), b = __float_as_uint(v[2 * e + 1]);
+          part[0][e] = __byte_perm(a, b, 0x7632);
+          const float ra = v[2 * e] - __uint_as_float(a & 0xffff0000u);
+          const float rb = v[2 * e + 1] - __uint_as_float(b & 0xffff0000u);
+          part[1][e] = pack2<__nv_bfloat16>(ra, rb);
+          const float2 h = unpack2<__nv_bfloat16>(part[1][e]);
+          part[2][e] = pack2<__nv_bfloat16>(ra - h.x, rb - h.y);
+        }
+#pragma unroll
+        for (int q = 0; q < 3; ++q)
+          *reinterpret_cast<uint4*>(dst + q * kPart + item * 16) =
+              make_uint4(part[q][0], part[q][1], part[q][2], part[q][3]);
+      }
+    };
+    uint8_t* dst = smem + L.planes + team * 3 * (kPartA + kPartB);
+    for (uint32_t i = team; i < blocks; i += 2) {
+      const uint32_t s = i % p.stages;
+      if (!warp_wait(&full[s], (i / p.stages) & 1, abort_flag) ||
+          !warp_wait(&parts_empty[team], ((i >> 1) & 1) ^ 1, abort_flag)) {
+        if (lead) give_up(abort_flag, p.status, 96);
+        break;
+      }
+      const uint8_t* raw = smem + s * L.stage;
+      split_operand(raw, dst, p.a_mn, std::integral_constant<int, kBM>());
+      split_operand(raw + kStageA, dst + 3 * kPartA, p.b_mn, std::integral_constant<int, kBNb>());
+      tc::fence_proxy_async_smem();
+      __syncwarp();
+      if (lead) {
+        tc::mbar_arrive(&empty[s]);
+        tc::mbar_arrive(&parts_full[team]);
+      }
+    }
   } else if (warp >= kFirstEpi) {  // ---- epilogue ----
     const int ew = warp - kFirstEpi;
     const bool lead = tc::elect_one();  // copies, stores and arrivals of the warp
-    const int quad = warp & 3, half = ew >> 2;
+    const int quad = warp & 3, part = ew >> 2;  // rows and columns of the warp
     uint8_t* boxes = smem + L.boxes + ew * p.nbuf * kBox;
-    float* bias_s = reinterpret_cast<float*>(smem + L.bias) + ew * kHalf;
+    float* bias_s = reinterpret_cast<float*>(smem + L.bias) + ew * kCols;
     const To* in = static_cast<const To*>(p.in_ptr);
     const T* bias = static_cast<const T*>(p.bias);
     To* out = static_cast<To*>(p.out_ptr);
@@ -491,7 +559,7 @@ linear_gemm_kernel(const __grid_constant__ GemmParams p) {
       if (lt >= p.num_tiles) return;
       int tm, tn, sp;
       tile_at(p, lt, tm, tn, sp);
-      const int c = tn * BN + half * kHalf + lj * kCB, r = (tm * CG + rank) * kBM + quad * 32;
+      const int c = tn * BN + part * kCols + lj * kCB, r = (tm * CG + rank) * kBM + quad * 32;
       const int b = lq % p.nbuf;
       if (c < p.N && r < p.M) {
         tc::mbar_arrive_expect_tx(&in_full[ew][b], kBox);
@@ -508,105 +576,33 @@ linear_gemm_kernel(const __grid_constant__ GemmParams p) {
     if (p.tma_io && has_in && lead)
       for (int i = 0; i < ahead; ++i) load_next();
     bool ok = true;
-    // FP32 data: the K blocks of this block's tiles in order, each split by all
-    // eight warps; a 16-byte row of a part holds 8 values along the contiguous
-    // axis, rows lie along the other one
-    uint32_t done = 0, blocks = 0;  // split so far, and in all
-    if constexpr (PARTS == 3) {
-      for (int t = first_tile; t < p.num_tiles; t += tile_step) {
-        const int sp = t / (p.tiles_m * p.tiles_n);
-        blocks += (uint32_t)((long long)p.kblocks * (sp + 1) / p.splits) -
-                  (uint32_t)((long long)p.kblocks * sp / p.splits);
-      }
-    }
-    int stage = 0;
-    uint32_t turn = 0;
-    auto split_operand = [&](const uint8_t* raw, uint8_t* dst, bool mn, auto width) {
-      constexpr int kW = decltype(width)::value;  // rows (columns) of the operand
-      constexpr uint32_t kPart = kW * kBK * 2;
-#pragma unroll
-      for (int i = 0; i < kW * kBK / 8; i += 32 * kEpiWarps) {
-        const int item = i + ew * 32 + lane;
-        // K-major: [k / 8][row]; MN-major: [row / 8][k]
-        const int o = mn ? item % kBK : item % kW, g = mn ? item / kBK : item / kW;
-        const uint8_t* line = raw + (mn ? (g / 4) * kBK * 128 + o * 128 : o * 128);
-        const int c = mn ? (g % 4) * 2 : g * 2;
-        float v[8];
-        *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(line + ((c ^ (o & 7)) * 16));
-        *reinterpret_cast<float4*>(v + 4) =
-            *reinterpret_cast<const float4*>(line + (((c + 1) ^ (o & 7)) * 16));
-        uint32_t part[3][4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          // the first part is cut off, not rounded: it cannot overflow
-          const uint32_t a = __float_as_uint(v[2 * e]), b = __float_as_uint(v[2 * e + 1]);
-          part[0][e] = __byte_perm(a, b, 0x7632);
-          const float ra = v[2 * e] - __uint_as_float(a & 0xffff0000u);
-          const float rb = v[2 * e + 1] - __uint_as_float(b & 0xffff0000u);
-          part[1][e] = pack2<__nv_bfloat16>(ra, rb);
-          const float2 h = unpack2<__nv_bfloat16>(part[1][e]);
-          part[2][e] = pack2<__nv_bfloat16>(ra - h.x, rb - h.y);
-        }
-#pragma unroll
-        for (int q3 = 0; q3 < 3; ++q3)
-          *reinterpret_cast<uint4*>(dst + q3 * kPart + item * 16) =
-              make_uint4(part[q3][0], part[q3][1], part[q3][2], part[q3][3]);
-      }
-    };
-    auto split_next = [&]() -> bool {
-      if (done == blocks) return true;
-      const int b = done & 1;
-      if (!warp_wait(&full[stage], turn, abort_flag) ||
-          !warp_wait(&parts_empty[b], ((done >> 1) & 1) ^ 1, abort_flag))
-        return false;
-      const uint8_t* raw = smem + stage * L.stage;
-      uint8_t* dst = smem + L.planes + b * 3 * (kPartA + kPartB);
-      split_operand(raw, dst, p.a_mn, std::integral_constant<int, kBM>());
-      split_operand(raw + kStageA, dst + 3 * kPartA, p.b_mn, std::integral_constant<int, kBNb>());
-      tc::fence_proxy_async_smem();
-      __syncwarp();
-      if (lead) {
-        tc::mbar_arrive(&empty[stage]);
-        tc::mbar_arrive(&parts_full[b]);
-      }
-      ++done;
-      if (++stage == p.stages) {
-        stage = 0;
-        turn ^= 1;
-      }
-      return true;
-    };
-    if constexpr (PARTS == 3) ok = split_next();
     for (int t = first_tile; t < p.num_tiles && ok; t += tile_step) {
       int tm, tn, sp;
       tile_at(p, t, tm, tn, sp);
       const int row0 = (tm * CG + rank) * kBM + quad * 32;
       const int row = row0 + lane;
-      const int col0 = tn * BN + half * kHalf;
-      const uint32_t tcol = tmem + ((uint32_t)(quad * 32) << 16) + half * kHalf;
+      const int col0 = tn * BN + part * kCols;
+      const uint32_t tcol = tmem + ((uint32_t)(quad * 32) << 16) + part * kCols;
       if constexpr (kEpi != kPartial && PARTS == 1) {
         if (bias != nullptr) {
 #pragma unroll
-          for (int i = lane; i < kHalf; i += 32)
+          for (int i = lane; i < kCols; i += 32)
             bias_s[i] = col0 + i < p.N ? ldg_f32<T>(bias + col0 + i) : 0.f;
           __syncwarp();
         }
       }
-      float sum[PARTS == 3 ? kHalf : 1];  // FP32 data: the K blocks added up
+      float sum[PARTS == 3 ? kCols : 1];  // FP32 data: the K blocks added up
       if constexpr (PARTS == 3) {
         const int kb0 = (int)((long long)p.kblocks * sp / p.splits);
         const int kb1 = (int)((long long)p.kblocks * (sp + 1) / p.splits);
 #pragma unroll
-        for (int i = 0; i < kHalf; ++i) sum[i] = 0.f;
-        // the parts of the next block (the next tile's at the end) are made
-        // while this one is multiplied
+        for (int i = 0; i < kCols; ++i) sum[i] = 0.f;
         for (int kb = kb0; kb < kb1; ++kb, ++ti) {
-          ok = split_next();
-          ok = ok && warp_wait(&acc_full[ti & 1], (ti >> 1) & 1, abort_flag);
+          ok = warp_wait(&acc_full[ti & 1], (ti >> 1) & 1, abort_flag);
           if (!ok) break;
           tc::tc_fence_after();
 #pragma unroll
-          for (int i = 0; i < kHalf; i += 32) {
+          for (int i = 0; i < kCols; i += 32) {
             float v[32];
             tc::tmem_ld16(tcol + (ti & 1) * BN + i, *reinterpret_cast<float(*)[16]>(v));
             tc::tmem_ld16(tcol + (ti & 1) * BN + i + 16, *reinterpret_cast<float(*)[16]>(v + 16));
@@ -961,9 +957,9 @@ int stage(const void* src, long long ld, long long rows, int cols, void* dst, cu
   return DDPM_OK;
 }
 
-// Tile of a product: columns and blocks that share it.
+// Tile of a product: columns, blocks that share it, epilogue warps.
 struct Tile {
-  int bn, cg;
+  int bn, cg, ew;
 };
 
 // The tile with the least estimated time: rounds of tiles over the SMs, each
@@ -973,7 +969,7 @@ struct Tile {
 Tile pick_tile(long long m, int n, long long k, int parts, int splits) {
   const int sms = gencat::num_sms(), bk = block_k(parts);
   const long long kb = ((k + bk - 1) / bk + splits - 1) / splits;
-  Tile best{64, 1};
+  Tile best{64, 1, 8};
   double least = 0;
   for (int cg = 1; cg <= (parts == 3 ? 1 : 2); ++cg)
     for (int bn = parts == 3 ? 128 : 256; bn >= (cg == 2 ? 256 : 64); bn /= 2) {
@@ -987,23 +983,26 @@ Tile pick_tile(long long m, int n, long long k, int parts, int splits) {
       const double t = rounds * (kb * block + 1000.0 + 4.0 * bn);
       if (least == 0 || t < least) {
         least = t;
-        best = Tile{bn, cg};
+        // a short K loop leaves the epilogue as the longest part of a tile: twice
+        // the warps there (65536 x 64 -> 1728: 94 -> 78 us), which a long one
+        // would pay for with a stage
+        best = Tile{bn, cg, bn == 256 && kb <= kShortK ? 16 : 8};
       }
     }
   return best;
 }
 
-template <typename T, int BN, int PARTS, Epi kEpi, int CG>
+template <typename T, int BN, int PARTS, Epi kEpi, int CG, int EW>
 int launch_gemm_as(GemmParams& p, cudaStream_t st) {
-  auto fn = linear_gemm_kernel<T, BN, PARTS, kEpi, CG>;
-  constexpr int kRow = box_row(BN, kEpi == kPartial ? 4 : (int)sizeof(T));
+  auto fn = linear_gemm_kernel<T, BN, PARTS, kEpi, CG, EW>;
+  constexpr int kRow = box_row(BN, EW, kEpi == kPartial ? 4 : (int)sizeof(T));
   const int tiles_k = (p.kblocks + p.splits - 1) / p.splits;
   const int limit = gencat::max_smem_optin() - 2048;  // static shared memory
   // As many stages as the K loop can use, at least two; what is left goes to
   // the epilogue's boxes, eight a warp at most, two at least.
   p.nbuf = 2;
   int stages = kMaxStages;
-  auto total = [&](int s, int b) { return (int)smem_layout(CG, PARTS, BN, kRow, s, b).total; };
+  auto total = [&](int s, int b) { return (int)smem_layout(CG, PARTS, BN, EW, kRow, s, b).total; };
   // a persistent block streams several tiles through the ring: twice a tile's
   // steps is as far ahead as it needs to look
   const int useful = tiles_k * 2 < 2 ? 2 : tiles_k * 2;
@@ -1022,11 +1021,11 @@ int launch_gemm_as(GemmParams& p, cudaStream_t st) {
   const int units = gencat::num_sms() / CG;
   const int grid = (p.num_tiles < units ? p.num_tiles : units) * CG;
   if constexpr (CG == 1) {
-    fn<<<grid, kThreads, smem, st>>>(p);
+    fn<<<grid, gemm_threads(PARTS, EW), smem, st>>>(p);
   } else {
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(grid);
-    cfg.blockDim = dim3(kThreads);
+    cfg.blockDim = dim3(gemm_threads(PARTS, EW));
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
     cudaLaunchAttribute at{};
@@ -1044,13 +1043,16 @@ int launch_gemm_as(GemmParams& p, cudaStream_t st) {
 template <typename T, Epi kEpi>
 int launch_gemm(GemmParams& p, Tile t, cudaStream_t st) {
   if constexpr (sizeof(T) == 4) {
-    return t.bn == 128 ? launch_gemm_as<T, 128, 3, kEpi, 1>(p, st)
-                       : launch_gemm_as<T, 64, 3, kEpi, 1>(p, st);
+    return t.bn == 128 ? launch_gemm_as<T, 128, 3, kEpi, 1, 8>(p, st)
+                       : launch_gemm_as<T, 64, 3, kEpi, 1, 8>(p, st);
+  } else if (t.bn == 256 && t.ew == 16) {
+    return t.cg == 2 ? launch_gemm_as<T, 256, 1, kEpi, 2, 16>(p, st)
+                     : launch_gemm_as<T, 256, 1, kEpi, 1, 16>(p, st);
   } else {
-    return t.cg == 2     ? launch_gemm_as<T, 256, 1, kEpi, 2>(p, st)
-           : t.bn == 256 ? launch_gemm_as<T, 256, 1, kEpi, 1>(p, st)
-           : t.bn == 128 ? launch_gemm_as<T, 128, 1, kEpi, 1>(p, st)
-                         : launch_gemm_as<T, 64, 1, kEpi, 1>(p, st);
+    return t.cg == 2     ? launch_gemm_as<T, 256, 1, kEpi, 2, 8>(p, st)
+           : t.bn == 256 ? launch_gemm_as<T, 256, 1, kEpi, 1, 8>(p, st)
+           : t.bn == 128 ? launch_gemm_as<T, 128, 1, kEpi, 1, 8>(p, st)
+                         : launch_gemm_as<T, 64, 1, kEpi, 1, 8>(p, st);
   }
 }
 
@@ -1136,7 +1138,7 @@ int run_gemm(const Gemm& g, cudaStream_t st) {
   if (rc) return rc;
   rc = operand_map(&p.b, g.b, g.b_mn, bn / g.tile.cg, (int)sizeof(T), kBf16);
   if (rc) return rc;
-  const int row = box_row(bn, es);
+  const int row = box_row(bn, sizeof(T) == 4 ? 8 : g.tile.ew, es);
   if (p.tma_io) {
     rc = io_map(&p.out, g.out, es, kBf16, g.M, g.N, g.ld_out, g.splits, row);
     if (rc) return rc;
@@ -1218,7 +1220,7 @@ LinearPlan plan_linear(const LinearShape& s, bool bwd) {
       if (splits > kb / 4) splits = kb / 4;
       if (splits > 1) {
         q.splits_w = (int)splits;
-        q.tile_w = Tile{bn, 1};
+        q.tile_w = Tile{bn, 1, 8};
       }
     }
     if (q.splits_w > 1) q.part_off = take((size_t)q.splits_w * s.n * ((s.k + 3) / 4 * 4) * 4);
