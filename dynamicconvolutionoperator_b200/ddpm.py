@@ -25,6 +25,10 @@ import torch.nn.functional as F
 from torch import nn
 
 from . import _fuseconv, _kernels
+from ._dropout import dropout as _dropout
+from ._linear import linear_act
+from ._norm import group_norm_act
+from ._op import activation_code
 
 _DEFAULT_DILATIONS = (1, 3, 5)
 
@@ -67,6 +71,19 @@ class DDPM(nn.Module):
         native_fuse: Run the 3x3 ``fuse`` convolution on this library's
             tensor-core kernels (C <= 64; single rounding of conv + bias, no
             TF32). ``False`` keeps the reference's cuDNN call.
+
+    The remaining arguments add a head behind ``fuse``, on the library's
+    channel-last operators; without them the module is the reference's. Its
+    output has channel-last memory, and it is
+    ``project(dropout(act(norm(fuse(...))))) + x`` with the parts asked for:
+
+        norm_groups: Group norm over this many groups (``norm.weight``,
+            ``norm.bias``), then ``activation``.
+        activation: "relu", "silu", "gelu", "gelu_tanh" or None; needs ``norm_groups``.
+        dropout: Probability of dropping a value, in training mode.
+        out_dim: 1x1 projection to this many channels (``project.weight``,
+            ``project.bias``).
+        residual: Add ``x``; needs as many channels out as in.
     """
 
     def __init__(
@@ -80,12 +97,28 @@ class DDPM(nn.Module):
         fused_generator_inference: bool = True,
         fused_generator_training: bool | None = None,
         native_fuse: bool = True,
+        norm_groups: int | None = None,
+        activation: str | None = None,
+        dropout: float = 0.0,
+        out_dim: int | None = None,
+        residual: bool = False,
     ) -> None:
         super().__init__()
         if kernel_size < 1 or kernel_size % 2 == 0:
             raise ValueError(f"kernel_size must be a positive odd integer, got {kernel_size}")
         if dim < 1:
             raise ValueError(f"dim must be positive, got {dim}")
+        if norm_groups is not None and (norm_groups < 1 or dim % norm_groups):
+            raise ValueError(f"norm_groups must divide dim, got {norm_groups} for {dim}")
+        activation_code(activation)
+        if activation is not None and norm_groups is None:
+            raise ValueError("activation needs norm_groups")
+        if not 0.0 <= dropout <= 1.0:
+            raise ValueError(f"dropout must be between 0 and 1, got {dropout}")
+        if out_dim is not None and out_dim < 1:
+            raise ValueError(f"out_dim must be positive, got {out_dim}")
+        if residual and out_dim not in (None, dim):
+            raise ValueError(f"residual needs out_dim == dim, got {out_dim} and {dim}")
 
         self.dim = dim
         self.kernel_size = kernel_size
@@ -98,6 +131,11 @@ class DDPM(nn.Module):
         self.dilations = _DEFAULT_DILATIONS
         self.generator = nn.Conv2d(dim, 3 * dim * kernel_size**2, 1)
         self.fuse = nn.Conv2d(4 * dim, dim, 3, 1, 1)
+        self.activation = activation
+        self.dropout = float(dropout)
+        self.residual = bool(residual)
+        self.norm = nn.GroupNorm(norm_groups, dim) if norm_groups is not None else None
+        self.project = nn.Conv2d(dim, out_dim, 1) if out_dim is not None else None
 
     # ------------------------------------------------------------ dispatch --
     def _fused_generator_ok(self, x: torch.Tensor, y: torch.Tensor,
@@ -144,7 +182,42 @@ class DDPM(nn.Module):
         )
         return _kernels.fused_dynamic_cat(x, kernels, self.kernel_size, self.dilations)
 
-    def forward(self, x: torch.Tensor, y: torch.Tensor) -> torch.Tensor:
+    def forward(self, x: torch.Tensor, y: torch.Tensor,
+                seed: int | torch.Tensor | None = None) -> torch.Tensor:
+        """``seed``: key of the head's dropout (see ``dropout``); None draws one
+        from torch's default CPU generator, which a captured graph cannot do."""
+        out = self._body(x, y)
+        if self.norm is None and self.project is None and not self.residual and not self.dropout:
+            return out
+        return self._head(out, x, seed)
+
+    def _head(self, out: torch.Tensor, x: torch.Tensor, seed) -> torch.Tensor:
+        dt = out.dtype
+        with torch.autocast("cuda", enabled=False):
+            if self.norm is not None:
+                # FP32 parameters go with 16-bit data as they are
+                w, b = (p if p.dtype in (dt, torch.float32) else p.to(dt)
+                        for p in (self.norm.weight, self.norm.bias))
+                out = group_norm_act(out, self.norm.num_groups, w, b, self.norm.eps,
+                                     activation=self.activation)
+            out = out.permute(0, 2, 3, 1)
+            res = x.to(dt).permute(0, 2, 3, 1) if self.residual else None
+            if self.dropout and self.training:
+                if seed is None:
+                    if torch.cuda.is_current_stream_capturing():
+                        raise RuntimeError("a captured DDPM with dropout needs a seed tensor")
+                    seed = int(torch.randint(1 << 62, ()))
+                # numbered in channel-last order; the last step adds the residual
+                out = _dropout(out, self.dropout, seed,
+                               residual=res if self.project is None else None)
+            elif self.project is None and res is not None:
+                out = out + res
+            if self.project is not None:
+                w, b = (p.to(dt) for p in (self.project.weight, self.project.bias))
+                out = linear_act(out, w, b, residual=res)
+            return out.permute(0, 3, 1, 2)
+
+    def _body(self, x: torch.Tensor, y: torch.Tensor) -> torch.Tensor:
         _check_inputs(x, y, self.dim)
         if not x.is_cuda:
             raise RuntimeError(

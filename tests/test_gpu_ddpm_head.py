@@ -1,0 +1,157 @@
+"""The DDPM with its optional head (group norm + activation, dropout, 1x1
+projection, residual) against the float64 oracle with the same head, and the
+parts of the head called one after the other."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from oracle import ddpm_oracle as orc
+from tests import _operators as ops
+from tests._parity import compare
+
+pytestmark = pytest.mark.gpu
+
+HEADS = [
+    dict(norm_groups=4, activation="silu"),
+    dict(norm_groups=2, activation="gelu", dropout=0.25, out_dim=16, residual=True),
+    dict(dropout=0.5, residual=True),
+    dict(out_dim=24),
+    dict(residual=True),
+]
+
+
+def _gold(m, ref, x, y, grad, seed):
+    """Output and gradients in float64 on the CPU."""
+    ref = ref.double()
+    head = {n: p.detach().double().cpu().requires_grad_() for n, p in m.named_parameters()
+            if n.startswith(("norm.", "project."))}
+    xd, yd = x.double().requires_grad_(), y.double().requires_grad_()
+    out = ref(xd, yd)
+    if m.norm is not None:
+        out = torch.nn.functional.group_norm(out, m.norm.num_groups, head["norm.weight"],
+                                             head["norm.bias"], m.norm.eps)
+        out = ops.act(out, m.activation)
+    if m.dropout and m.training:
+        cl = out.permute(0, 2, 3, 1)
+        mask = ops.kept(cl.numel(), m.dropout, seed, 0).view(cl.shape)
+        out = torch.where(mask, cl / (1 - m.dropout), torch.zeros_like(cl)).permute(0, 3, 1, 2)
+    if m.project is not None:
+        out = torch.nn.functional.conv2d(out, head["project.weight"], head["project.bias"])
+    if m.residual:
+        out = out + xd
+    leaves = {"x": xd, "y": yd, **dict(ref.named_parameters()), **head}
+    grads = torch.autograd.grad(out, list(leaves.values()), grad.double())
+    return out.detach(), dict(zip(leaves, grads))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("head", HEADS)
+def test_matches_float64(head, dtype):
+    from dynamicconvolutionoperator_b200 import DDPM, _lib
+
+    seed = 1234
+    ref = orc.make_model(16, 3, dtype=dtype, seed=3)
+    m = DDPM(16, 3, **head)
+    m.load_state_dict(ref.state_dict(), strict=False)
+    if m.norm is not None:
+        torch.nn.init.uniform_(m.norm.weight, 0.5, 1.5)
+        torch.nn.init.uniform_(m.norm.bias, -0.5, 0.5)
+    m = m.cuda().to(dtype)
+    shape = (2, 16, 11, 13)
+    x, y, _ = orc.make_inputs(shape, dtype=dtype, seed=5)
+    oc = head.get("out_dim") or 16
+    grad = torch.randn((2, oc, 11, 13), generator=torch.Generator().manual_seed(6)).to(dtype)
+    xd, yd = (t.cuda().requires_grad_() for t in (x, y))
+    out = m(xd, yd, seed=seed)
+    assert out.shape == grad.shape
+    named = dict(m.named_parameters())
+    got = torch.autograd.grad(out, [xd, yd, *named.values()], grad.cuda())
+    got = {k: v.cpu() for k, v in zip(["x", "y", *named], got)}
+    gold, want = _gold(m, ref, x, y, grad, seed)
+    stats, fails = compare(out.detach().cpu(), got, gold, want, dtype)
+    assert not fails, "\n".join(fails) + f"\n{stats}"
+    assert _lib.device_status() == 0
+
+
+def test_without_a_head_nothing_changes():
+    from dynamicconvolutionoperator_b200 import DDPM
+
+    m = DDPM(16, 3).cuda()
+    assert set(m.state_dict()) == {"generator.weight", "generator.bias", "fuse.weight", "fuse.bias"}
+    x, y = torch.randn(2, 2, 16, 9, 10, device="cuda")
+    assert torch.equal(m(x, y), m._body(x, y))
+
+
+def test_head_is_its_operators_in_a_row():
+    from dynamicconvolutionoperator_b200 import DDPM, dropout, group_norm_act, linear_act
+
+    m = DDPM(16, 3, norm_groups=4, activation="gelu", dropout=0.3, out_dim=16, residual=True).cuda()
+    x, y = torch.randn(2, 2, 16, 20, 24, device="cuda")
+    body = m._body(x, y)
+    z = group_norm_act(body, 4, m.norm.weight, m.norm.bias, m.norm.eps, activation="gelu")
+    z = dropout(z.permute(0, 2, 3, 1), 0.3, 99)
+    z = linear_act(z, m.project.weight, m.project.bias, residual=x.permute(0, 2, 3, 1))
+    assert torch.equal(m(x, y, seed=99), z.permute(0, 3, 1, 2))
+    m.eval()
+    assert torch.equal(m(x, y, seed=1), m(x, y, seed=2))
+
+
+def test_drawn_seeds_follow_the_default_generator():
+    from dynamicconvolutionoperator_b200 import DDPM
+
+    m = DDPM(16, 3, dropout=0.5).cuda()
+    x, y = torch.randn(2, 1, 16, 8, 8, device="cuda")
+    torch.manual_seed(5)
+    a, b = m(x, y), m(x, y)
+    torch.manual_seed(5)
+    assert torch.equal(m(x, y), a) and not torch.equal(a, b)
+
+
+def test_autocast_runs_the_head_in_the_autocast_type():
+    from dynamicconvolutionoperator_b200 import DDPM
+
+    m = DDPM(16, 3, norm_groups=4, activation="silu", out_dim=8).cuda()
+    x, y = torch.randn(2, 1, 16, 12, 16, device="cuda", requires_grad=True)
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        out = m(x, y)
+    assert out.dtype == torch.bfloat16
+    out.float().square().mean().backward()
+    for p in m.parameters():
+        assert p.grad is not None and p.grad.dtype == torch.float32 and p.grad.isfinite().all()
+
+
+def test_training_step_with_the_head_captured_and_replayed():
+    from dynamicconvolutionoperator_b200 import DDPM
+
+    m = DDPM(16, 3, norm_groups=4, activation="silu", dropout=0.2, out_dim=16, residual=True,
+             fused_generator_training=True).cuda().to(torch.bfloat16)
+    x, y, g = torch.randn(3, 2, 16, 16, 24, device="cuda").to(torch.bfloat16)
+    seed = torch.tensor([7], device="cuda")
+    params = list(m.parameters())
+
+    def once():
+        out = m(x, y, seed=seed)
+        return [out.detach(), *torch.autograd.grad(out, params, g)]
+
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        once()
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = once()
+    for value in (7, 8):
+        seed.fill_(value)
+        graph.replay()
+        torch.cuda.synchronize()
+        # the generator's backward adds with FP32 atomics, whose order is free
+        for a, b in zip(held, once()):
+            scale = b.float().abs().max() + 1e-6
+            assert ((a.float() - b.float()).abs().max() / scale).item() < 2e-2
+        assert torch.equal(held[0], m(x, y, seed=seed))
+    with pytest.raises(RuntimeError, match="seed"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            m(x, y)

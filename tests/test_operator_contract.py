@@ -150,3 +150,19 @@ def test_group_norm_workspace_covers_every_alignment(bwd):
         for n, px in ((3, 1000), (5, 100_000)):
             assert size(n, px, c, g, 1, bwd, 0) >= size(n, px, c, g, 1, bwd, 1)
         assert size(5, 100_000, c, g, 1, bwd, 1) > 0
+
+
+@pytest.mark.parametrize("kwargs,match", [
+    (dict(norm_groups=3), "norm_groups"),
+    (dict(norm_groups=0), "norm_groups"),
+    (dict(activation="relu"), "needs norm_groups"),
+    (dict(norm_groups=2, activation="swish"), "activation"),
+    (dict(dropout=1.5), "dropout"),
+    (dict(out_dim=0), "out_dim"),
+    (dict(out_dim=5, residual=True), "residual"),
+])
+def test_ddpm_head_refusals(kwargs, match):
+    from dynamicconvolutionoperator_b200 import DDPM
+
+    with pytest.raises(ValueError, match=match):
+        DDPM(4, 3, **kwargs)
