@@ -11,8 +11,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from ._kernels import _require_cuda
-from ._op import first_order, ptr
+from ._op import first_order, on_one_device, ptr
 
 _U64 = (1 << 64) - 1
 
@@ -91,7 +90,7 @@ def dropout(x: torch.Tensor, p: float, seed: int | torch.Tensor, offset: int = 0
         if residual.shape != x.shape or residual.dtype != x.dtype:
             raise ValueError(f"residual must have x's shape and dtype, got {tuple(residual.shape)} "
                              f"of {residual.dtype} for {tuple(x.shape)} of {x.dtype}")
-    _require_cuda(x, *[t for t in (seed, residual) if isinstance(t, torch.Tensor)])
+    on_one_device(x, seed if isinstance(seed, torch.Tensor) else None, residual)
     _lib.dtype_code(x.dtype)
     x = x.contiguous()
     residual = residual.contiguous() if residual is not None else None

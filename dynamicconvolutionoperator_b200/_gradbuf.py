@@ -54,12 +54,17 @@ def view_of(param: torch.Tensor) -> torch.Tensor | None:
     return None
 
 
+def attached() -> bool:
+    """Whether any parameter has a view attached."""
+    return bool(_views)
+
+
 def grad_buffer(param: torch.Tensor | None, shape, dtype: torch.dtype,
                 device: torch.device) -> torch.Tensor:
     """Tensor of ``shape`` for the backward to write ``param``'s gradient into:
     the attached view when one is armed and ``param.grad`` is ``None``, else a
     fresh allocation."""
-    if param is not None:
+    if param is not None and _views:
         ent = _views.get(id(param))
         if ent is not None and ent[0]() is param and ent[2] and param.grad is None:
             view = ent[1]
@@ -90,5 +95,5 @@ def grads_written(params, buffers) -> None:
         fn(tuple(params), tuple(buffers))
 
 
-__all__ = ["add_listener", "arm", "attach", "detach", "grad_buffer", "grads_written",
+__all__ = ["add_listener", "arm", "attach", "attached", "detach", "grad_buffer", "grads_written",
            "remove_listener", "view_of"]

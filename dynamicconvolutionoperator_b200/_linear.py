@@ -13,9 +13,8 @@ import functools
 import torch
 
 from . import _lib
-from ._gradbuf import grad_buffer
-from ._kernels import _require_cuda
-from ._op import activation_code, aligned, first_order, ptr, workspace
+from ._op import (activation_code, aligned, first_order, on_one_device, param_grad, ptr,
+                  workspace)
 
 
 def _rows(x: torch.Tensor) -> torch.Tensor:
@@ -84,8 +83,8 @@ class _LinearAct(torch.autograd.Function):
         n = w.shape[0]
         dev, dt = flat.device, flat.dtype
         gx = torch.empty((m, k), dtype=dt, device=dev) if need_x else None
-        gw = grad_buffer(weight, weight.shape, dt, dev) if need_w else None
-        gb = grad_buffer(bias, bias.shape, dt, dev) if need_b else None
+        gw = param_grad(weight) if need_w else None
+        gb = param_grad(bias) if need_b else None
         if m == 0:
             for g in (gw, gb):
                 if g is not None:
@@ -127,23 +126,26 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None 
     act = activation_code(activation)
     if x.ndim < 1:
         raise ValueError("x must have at least one dimension [..., k]")
-    shape = tuple(weight.shape)
-    if not (len(shape) == 2 or (len(shape) == 4 and shape[2:] == (1, 1))) or shape[1] != x.shape[-1]:
-        raise ValueError(f"weight must be [n, {x.shape[-1]}] or [n, {x.shape[-1]}, 1, 1], got {shape}")
+    shape = weight.shape
+    if not (len(shape) == 2 or (len(shape) == 4 and shape[2] == shape[3] == 1)) or shape[1] != x.shape[-1]:
+        raise ValueError(f"weight must be [n, {x.shape[-1]}] or [n, {x.shape[-1]}, 1, 1], "
+                         f"got {tuple(shape)}")
     n = shape[0]
     if n < 1 or shape[1] < 1:
-        raise ValueError(f"weight must not be empty, got {shape}")
-    if bias is not None and tuple(bias.shape) != (n,):
+        raise ValueError(f"weight must not be empty, got {tuple(shape)}")
+    if bias is not None and bias.shape != (n,):
         raise ValueError(f"bias must have shape ({n},), got {tuple(bias.shape)}")
-    if residual is not None and tuple(residual.shape) != (*x.shape[:-1], n):
+    if residual is not None and residual.shape != (*x.shape[:-1], n):
         raise ValueError(f"residual must have shape {(*x.shape[:-1], n)}, got {tuple(residual.shape)}")
-    given = [t for t in (weight, bias, residual) if t is not None]
-    for t in given:
-        if t.dtype != x.dtype:
-            raise ValueError(f"all tensors must have one dtype, got {x.dtype} and {t.dtype}")
-    _require_cuda(x, *given)
+    needs_grad = x.requires_grad
+    for t in (weight, bias, residual):
+        if t is not None:
+            if t.dtype is not x.dtype:
+                raise ValueError(f"all tensors must have one dtype, got {x.dtype} and {t.dtype}")
+            needs_grad = needs_grad or t.requires_grad
+    on_one_device(x, weight, bias, residual)
     _lib.dtype_code(x.dtype)
-    if torch.is_grad_enabled() and (x.requires_grad or any([t.requires_grad for t in given])):
+    if needs_grad and torch.is_grad_enabled():
         return _LinearAct.apply(x, weight, bias, residual, act)
     flat = _rows(x)
     out = _forward(flat, _matrix(weight, (n, flat.shape[1])),

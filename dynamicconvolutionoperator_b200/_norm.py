@@ -15,17 +15,20 @@ import math
 import torch
 
 from . import _lib
-from ._gradbuf import grad_buffer
-from ._kernels import _require_cuda
-from ._op import activation_code, aligned, first_order, ptr, workspace
+from ._op import (activation_code, aligned, first_order, on_one_device, param_grad, ptr,
+                  workspace)
 
 
 def _channel_last(t: torch.Tensor) -> torch.Tensor:
     """[N, C, *] as contiguous [N, *, C] (no copy for channel-last memory)."""
+    if t.ndim == 4:
+        return t.permute(0, 2, 3, 1).contiguous()
     return (t.movedim(1, -1) if t.ndim > 2 else t).contiguous()
 
 
 def _channel_first(t: torch.Tensor) -> torch.Tensor:
+    if t.ndim == 4:
+        return t.permute(0, 3, 1, 2)
     return t.movedim(-1, 1) if t.ndim > 2 else t
 
 
@@ -76,8 +79,8 @@ class _GroupNormAct(torch.autograd.Function):
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
         dev = xl.device
         gx = torch.empty_like(xl) if need_x else None
-        gw = grad_buffer(weight, weight.shape, weight.dtype, dev) if need_w else None
-        gb = grad_buffer(bias, bias.shape, bias.dtype, dev) if need_b else None
+        gw = param_grad(weight) if need_w else None
+        gb = param_grad(bias) if need_b else None
         if xl.numel() == 0:
             for g in (gw, gb):
                 if g is not None:
@@ -124,16 +127,18 @@ def group_norm_act(x: torch.Tensor, num_groups: int, weight: torch.Tensor | None
         raise ValueError(f"num_groups must divide the channels, got {num_groups} for {c}")
     if not eps >= 0:
         raise ValueError(f"eps must not be negative, got {eps}")
-    for name, t in (("weight", weight), ("bias", bias)):
+    for t in (weight, bias):
         if t is None:
             continue
-        if tuple(t.shape) != (c,):
-            raise ValueError(f"{name} must have shape ({c},), got {tuple(t.shape)}")
-        if t.dtype not in (x.dtype, torch.float32):
-            raise ValueError(f"{name} must have x's dtype or float32, got {t.dtype} for {x.dtype}")
+        if t.shape != (c,):
+            raise ValueError(f"{'weight' if t is weight else 'bias'} must have shape ({c},), "
+                             f"got {tuple(t.shape)}")
+        if t.dtype is not x.dtype and t.dtype is not torch.float32:
+            raise ValueError(f"{'weight' if t is weight else 'bias'} must have x's dtype or "
+                             f"float32, got {t.dtype} for {x.dtype}")
     if weight is not None and bias is not None and weight.dtype != bias.dtype:
         raise ValueError(f"weight and bias must have one dtype, got {weight.dtype} and {bias.dtype}")
-    _require_cuda(x, *(t for t in (weight, bias) if t is not None))
+    on_one_device(x, weight, bias)
     _lib.dtype_code(x.dtype)
     if torch.is_grad_enabled() and (x.requires_grad
                                     or (weight is not None and weight.requires_grad)

@@ -7,6 +7,9 @@ import functools
 import torch
 from torch.autograd.function import once_differentiable
 
+from . import _gradbuf
+from ._kernels import _require_cuda
+
 ACTIVATIONS = {None: 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}
 
 
@@ -30,6 +33,24 @@ def aligned(*pointers: int | None) -> bool:
     return bits % 16 == 0
 
 
+def param_grad(param: torch.Tensor) -> torch.Tensor:
+    """Where the backward writes ``param``'s gradient (contiguous): an attached
+    buffer, or a new tensor."""
+    if _gradbuf.attached():
+        return _gradbuf.grad_buffer(param, param.shape, param.dtype, param.device)
+    return torch.empty_like(param, memory_format=torch.contiguous_format)
+
+
+def on_one_device(x: torch.Tensor, *others: torch.Tensor | None) -> None:
+    """Raise unless every tensor is on ``x``'s CUDA device."""
+    if not x.is_cuda:
+        _require_cuda(x)
+    index = x.get_device()
+    for t in others:
+        if t is not None and t.get_device() != index:
+            _require_cuda(x, t)
+
+
 def workspace(nbytes: int, device: torch.device) -> torch.Tensor | None:
     return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
 
@@ -46,4 +67,5 @@ def first_order(backward):
     return run
 
 
-__all__ = ["ACTIVATIONS", "activation_code", "aligned", "first_order", "ptr", "workspace"]
+__all__ = ["ACTIVATIONS", "activation_code", "aligned", "first_order", "on_one_device",
+           "param_grad", "ptr", "workspace"]
