@@ -393,7 +393,12 @@ __global__ void __launch_bounds__(kThreads, kBwd ? 2 : 3) norm_kernel(const Norm
         }
       }
       if constexpr (kCluster) {
-        asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+        // one cluster, one sample (S > 1); a block alone may have several
+        if (p.S > 1)
+          asm volatile("barrier.cluster.arrive.release.aligned;\n\t"
+                       "barrier.cluster.wait.acquire.aligned;" ::: "memory");
+        else
+          __syncthreads();
         const float total = (float)p.P * (float)p.cg;
         for (int g = warp; g < p.G; g += kWarps) {
           const bool in = lane < p.S;
@@ -414,7 +419,7 @@ __global__ void __launch_bounds__(kThreads, kBwd ? 2 : 3) norm_kernel(const Norm
         }
         __syncthreads();
         // the peers' reads of this block's partials are over before it ends
-        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+        if (p.S > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
       } else {
         __syncthreads();
         if (tid == 0) {
@@ -507,7 +512,9 @@ __global__ void __launch_bounds__(kThreads, kBwd ? 2 : 3) norm_kernel(const Norm
       }
     }
   }
-  if constexpr (kCluster) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  if constexpr (kCluster) {
+    if (p.S > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  }
   if constexpr (kBwd) {
     if (p.wsum != nullptr) {
       __syncthreads();
@@ -1113,19 +1120,21 @@ int make_plan(Plan* q, long long n, long long P, int C, int G, int dt, bool bwd,
   q->TY = kThreads / q->TX;
   q->U = q->CT == 1 ? G : C;
   q->uw = q->CT == 1 ? C / G : 1;
-  // Small samples: a cluster each, at least a row of pixels for every thread
-  // row and at most 64 KB of x a block (16 x 16 x 64 FP32 forward: 9.0 -> 4.6 us,
-  // and two calls fewer on the host).
+  // Small samples: a cluster each (a single block that takes several in turn
+  // where there are many), at least a row of pixels for every thread row and at
+  // most 64 KB of x a block: 16 x 16 x 64 FP32 forward 9.0 -> 7.5 us, and two
+  // calls fewer on the host.
   if (q->CT == 1) {
+    const int blocks = 3 * gencat::num_sms();
     for (int cl = 8; cl >= 1 && !q->cluster; cl /= 2) {
       const long long r = (P + cl - 1) / cl;
-      if ((cl - 1) * r >= P || n * cl > 3 * gencat::num_sms() || (cl > 1 && r < q->TY)) continue;
+      if (cl > 1 && ((cl - 1) * r >= P || n * cl > blocks || r < q->TY)) continue;
       if ((double)r * C * es > 65536.0) break;
       q->cluster = true;
       q->R = (int)r;
       q->S = cl;
       q->chunks = n * cl;
-      q->grid = (int)q->chunks;
+      q->grid = (int)(q->chunks < blocks ? q->chunks : blocks);
       q->lag = 0;
     }
     if (q->cluster) {

@@ -141,3 +141,22 @@ def test_replayed_graph_draws_by_the_seed_tensor():
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(held, once()))
         assert torch.equal(held[0] != 0, held[1] != 0)
+
+
+def test_more_values_than_32_bits_count():
+    from dynamicconvolutionoperator_b200 import dropout
+
+    n = (1 << 32) + 4099
+    if torch.cuda.mem_get_info()[0] < 5 * n:
+        pytest.skip("needs 22 GB")
+    x = torch.ones(n, dtype=torch.bfloat16, device="cuda")
+    out = dropout(x, 0.5, 3)
+    for at in (0, 1 << 31, (1 << 32) - 500, n - 1001):
+        assert torch.equal(out[at:at + 1000], dropout(x[at:at + 1000], 0.5, 3, at))
+
+
+def test_seed_on_another_device_is_refused():
+    from dynamicconvolutionoperator_b200 import dropout
+
+    with pytest.raises(RuntimeError, match="CUDA"):
+        dropout(torch.ones(4, device="cuda"), 0.5, torch.tensor([1]))

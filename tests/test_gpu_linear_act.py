@@ -324,3 +324,46 @@ def test_gradients_land_in_attached_buffers():
             ops.check(key, got, r, ops.bound(r, s, _steps(64, x.dtype) + _steps(16, x.dtype), x.dtype))
     finally:
         _gradbuf.detach(w), _gradbuf.detach(b)
+
+
+def test_more_outputs_than_32_bits_count():
+    from dynamicconvolutionoperator_b200 import linear_act
+
+    if torch.cuda.mem_get_info()[0] < 24 << 30:
+        pytest.skip("needs 24 GB")
+    m = 1 << 20
+    x, w, b, _, _ = _case(m, 2056, 16, torch.bfloat16)
+    out = linear_act(x, w, b, "silu")
+    assert out.numel() > 2 ** 31
+    assert torch.equal(out[-300:], linear_act(x[-300:], w, b, "silu"))
+    xa = x[-300:].clone().requires_grad_()
+    gy = torch.zeros_like(out)
+    gy[-300:] = torch.randn(300, 2056, device="cuda").bfloat16()
+    xb = x.requires_grad_()
+    gx, = torch.autograd.grad(linear_act(xb, w, b, "silu"), xb, gy)
+    ga, = torch.autograd.grad(linear_act(xa, w, b, "silu"), xa, gy[-300:])
+    assert torch.equal(gx[-300:], ga) and not gx[:1000].any()
+
+
+def test_vectors_and_batches():
+    from dynamicconvolutionoperator_b200 import linear_act
+
+    x, w, b, res, _ = _case(12, 24, 40, torch.float32)
+    want = linear_act(x, w, b, "gelu", res)
+    got = linear_act(x.view(3, 2, 2, 40), w, b, "gelu", res.view(3, 2, 2, 24))
+    assert torch.equal(got.view(12, 24), want)
+    v = x[0].clone().requires_grad_()
+    out = linear_act(v, w, b)
+    assert out.shape == (24,)
+    g, = torch.autograd.grad(out.sum(), v)
+    torch.testing.assert_close(g, w.sum(0), rtol=1e-5, atol=1e-5)
+
+
+def test_second_derivative_is_refused():
+    from dynamicconvolutionoperator_b200 import linear_act
+
+    x, w, _, _, _ = _case(12, 24, 40, torch.float32)
+    x.requires_grad_()
+    g, = torch.autograd.grad(linear_act(x, w, None, "silu").sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable|not require grad"):
+        g.sum().backward()

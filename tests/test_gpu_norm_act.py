@@ -64,6 +64,8 @@ SHAPES = [
     ((300, 16, 5, 3), 2),         # more samples than blocks
     ((2, 2304, 6, 5), 9),         # channels of several tiles, groups across them
     ((2, 515, 17), 5),            # several tiles of single channels
+    ((3000, 24), 3),              # rows without pixels, more than blocks
+    ((1500, 40, 6), 5),
     ((1, 8, 3, 4, 5), 4),         # three spatial dimensions
 ]
 
@@ -217,14 +219,70 @@ def test_same_bits_every_time_and_on_other_streams():
         assert all(torch.equal(a, e) for a, e in zip(got, want))
 
 
-def test_captured_and_replayed():
+@pytest.mark.parametrize("shape", [(4, 64, 96, 96), (3, 63, 96, 96), (3, 60, 20, 20)])
+def test_calls_of_one_stream_overlap_with_another_kernels(shape):
+    """Blocks that wait for one another beside other work on the device."""
+    from dynamicconvolutionoperator_b200 import group_norm_act, linear_act
+
+    x, w, b, _ = _case(shape, torch.float16, 3 if shape[1] % 3 == 0 else 4)
+    groups = 3 if shape[1] % 3 == 0 else 4
+    want = group_norm_act(x, groups, w, b)
+    a, wa = (torch.randn(4096, 512, device="cuda").bfloat16() for _ in range(2))
+    other = linear_act(a, wa)
+    torch.cuda.synchronize()
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    outs = []
+    for _ in range(20):
+        with torch.cuda.stream(s1):
+            outs.append((group_norm_act(x, groups, w, b), want))
+        with torch.cuda.stream(s2):
+            outs.append((linear_act(a, wa), other))
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, e) for g, e in outs)
+
+
+def test_more_values_than_32_bits_count():
     from dynamicconvolutionoperator_b200 import group_norm_act
 
-    x, w, b, dy = _case((2, 64, 64, 64), torch.bfloat16, 8)
+    if torch.cuda.mem_get_info()[0] < 24 << 30:
+        pytest.skip("needs 24 GB")
+    x = torch.randn(36, 1000, 1000, 64, device="cuda", dtype=torch.bfloat16).permute(0, 3, 1, 2)
+    assert x.numel() > 2 ** 31
+    xa = x.requires_grad_()
+    out = group_norm_act(xa, 8, activation="silu")
+    last = x[-1:].detach().requires_grad_()
+    want = group_norm_act(last, 8, activation="silu")
+    # the same sums in other chunks: the last digit of the rounding may differ
+    torch.testing.assert_close(out[-1:], want, rtol=2 ** -7, atol=1e-5)
+    dy = torch.randn_like(last)
+    g = torch.zeros_like(x)
+    g[-1:] = dy
+    gx, = torch.autograd.grad(out, xa, g)
+    gl, = torch.autograd.grad(want, last, dy)
+    torch.testing.assert_close(gx[-1:], gl, rtol=2 ** -7, atol=1e-5)
+    assert not gx[0].any()
+
+
+def test_second_derivative_is_refused():
+    from dynamicconvolutionoperator_b200 import group_norm_act
+
+    x = torch.randn(2, 8, 4, 4, device="cuda", requires_grad=True)
+    g, = torch.autograd.grad(group_norm_act(x, 2).square().sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable|not require grad"):
+        g.sum().backward()
+
+
+@pytest.mark.parametrize("shape", [(2, 64, 64, 64), (2, 64, 200, 200), (2, 63, 200, 200)])
+def test_captured_and_replayed(shape):
+    """A kernel of each kind: clusters, the ring, blocks that wait for one another."""
+    from dynamicconvolutionoperator_b200 import group_norm_act
+
+    groups = 8 if shape[1] == 64 else 7
+    x, w, b, dy = _case(shape, torch.bfloat16, groups)
     xa, wa, ba = (t.clone().requires_grad_() for t in (x, w, b))
 
     def once():
-        out = group_norm_act(xa, 8, wa, ba, activation="silu")
+        out = group_norm_act(xa, groups, wa, ba, activation="silu")
         return [out.detach(), *torch.autograd.grad(out, (xa, wa, ba), dy)]
 
     s = torch.cuda.Stream()
@@ -236,7 +294,7 @@ def test_captured_and_replayed():
     with torch.cuda.graph(graph):
         held = once()
     for seed in (1, 2):
-        x2 = _case((2, 64, 64, 64), torch.bfloat16, 8, seed=seed)[0]
+        x2 = _case(shape, torch.bfloat16, groups, seed=seed)[0]
         with torch.no_grad():
             xa.copy_(x2)
         graph.replay()
