@@ -323,6 +323,15 @@ linear_gemm_kernel(const __grid_constant__ GemmParams p) {
   tc::tc_fence_after();
   const uint32_t tmem = tmem_base_s;
 
+  auto total_blocks = [&]() {  // K blocks of all of this block's tiles
+    uint32_t n = 0;
+    for (int t = first_tile; t < p.num_tiles; t += tile_step) {
+      const int sp = t / (p.tiles_m * p.tiles_n);
+      n += (uint32_t)((long long)p.kblocks * (sp + 1) / p.splits) -
+           (uint32_t)((long long)p.kblocks * sp / p.splits);
+    }
+    return n;
+  };
   // bytes of A in a stage; of one part of A and of B
   constexpr uint32_t kStageA = kBM * 128, kPartA = kBM * kBK * 2, kPartB = kBNb * kBK * 2;
   if (warp == 0) {
@@ -465,11 +474,21 @@ linear_gemm_kernel(const __grid_constant__ GemmParams p) {
           ++ti;
         }
       }
-      // every product issued has completed before the tensor memory is freed
       if (lead) commit<CG>(&drained);
       __syncwarp();
-      warp_wait(&drained, 0, nullptr);
     }
+    // Every product has completed before the tensor memory is freed, and every
+    // arrival that a commit promised to this block's barriers, those that nobody
+    // else waits for among them, has come before its shared memory goes. (The
+    // last phases are awaited behind `drained`: by then no barrier is more than
+    // one phase behind them, so their parity tells.)
+    warp_wait(&drained, 0, rank == 0 ? nullptr : abort_flag);
+    const uint32_t n = total_blocks();
+    const uint32_t ring = PARTS == 3 ? 2 : p.stages;
+    for (uint32_t j = n > ring ? n - ring : 0; j < n; ++j)
+      if (!warp_wait(PARTS == 3 ? &parts_empty[j % ring] : &empty[j % ring], (j / ring) & 1,
+                     abort_flag))
+        break;
     __syncwarp();
   } else if (PARTS == 3 && warp >= kFirstSplit) {  // ---- parts of FP32 operands ----
     // Two groups of four warps take the K blocks in turn, each into its own set
@@ -478,12 +497,7 @@ linear_gemm_kernel(const __grid_constant__ GemmParams p) {
     const int team = (warp - kFirstSplit) >> 2;
     const int me = ((warp - kFirstSplit) & 3) * 32 + lane;
     const bool lead = tc::elect_one();
-    uint32_t blocks = 0;
-    for (int t = first_tile; t < p.num_tiles; t += tile_step) {
-      const int sp = t / (p.tiles_m * p.tiles_n);
-      blocks += (uint32_t)((long long)p.kblocks * (sp + 1) / p.splits) -
-                (uint32_t)((long long)p.kblocks * sp / p.splits);
-    }
+    const uint32_t blocks = total_blocks();
     auto split_operand = [&](const uint8_t* raw, uint8_t* dst, bool mn, auto width) {
       constexpr int kW = decltype(width)::value;  // rows (columns) of the operand
       constexpr uint32_t kPart = kW * kBK * 2;
