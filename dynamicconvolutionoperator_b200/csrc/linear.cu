@@ -679,7 +679,7 @@ linear_gemm_kernel(const __grid_constant__ GemmParams p) {
             for (int cc = 0; cc < kCB; cc += 32) {
               const int c = cc + lane;
               if (c0 + c < p.N) {
-#pragma unroll 8
+#pragma unroll 16
                 for (int r = 0; r < 32; ++r)
                   if (row0 + r < p.M)
                     *reinterpret_cast<To*>(box + value_at(r, c)) =
@@ -856,40 +856,51 @@ __global__ void __launch_bounds__(256) linear_colsum_kernel(const T* __restrict_
   }
 }
 
-// out[i] = sum over `count` partials [count][size], in order.
+// out[r][c] = sum over `count` partials [count][rows][pitch].
+struct Fold {
+  const float* part;
+  long long rows, pitch;
+  int count, cols, blocks;
+  void* out;
+};
+
+// A thread per value, the partials in order: few of them, many values.
 template <typename T>
-__global__ void __launch_bounds__(256) linear_fold_kernel(const float* __restrict__ part, int count,
-                                                          long long rows, int cols, int pitch,
-                                                          T* __restrict__ out) {
-  const long long total = rows * cols;
+__global__ void __launch_bounds__(256) linear_fold_kernel(const Fold f) {
+  const long long total = f.rows * f.cols;
   for (long long i = blockIdx.x * (long long)blockDim.x + threadIdx.x; i < total;
        i += (long long)gridDim.x * blockDim.x) {
-    const long long r = i / cols;
-    const float* s = part + r * pitch + (i - r * cols);
+    const long long r = i / f.cols;
+    const float* s = f.part + r * f.pitch + (i - r * f.cols);
     float a = 0.f;
 #pragma unroll 8
-    for (int k = 0; k < count; ++k) a += s[(long long)k * rows * pitch];
-    out[i] = from_f32<T>(a);
+    for (int k = 0; k < f.count; ++k) a += s[(long long)k * f.rows * f.pitch];
+    static_cast<T*>(f.out)[i] = from_f32<T>(a);
   }
 }
 
-// Column totals of [rows][cols] FP32 partials: 32 columns a block.
+// 32 values a block, whose 32 warps share the partials: many of them. Two sums
+// in one launch (the bias's and the weight's gradient).
 template <typename T>
-__global__ void __launch_bounds__(1024) linear_fold_rows_kernel(const float* __restrict__ part,
-                                                                long long rows, int cols,
-                                                                T* __restrict__ out) {
+__global__ void __launch_bounds__(1024) linear_fold_long_kernel(const Fold f0, const Fold f1) {
   __shared__ float sh[32][33];
+  const bool second = (int)blockIdx.x >= f0.blocks;
+  const Fold& f = second ? f1 : f0;
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  const int c = blockIdx.x * 32 + lane;
+  const long long i = (blockIdx.x - (second ? f0.blocks : 0)) * 32LL + lane;
+  const long long total = f.rows * f.cols, step = f.rows * f.pitch;
   float a = 0.f;
-  if (c < cols)
-#pragma unroll 4
-    for (long long r = w; r < rows; r += 32) a += part[r * cols + c];
+  if (i < total) {
+    const long long r = i / f.cols;
+    const float* s = f.part + r * f.pitch + (i - r * f.cols);
+#pragma unroll 8
+    for (int k = w; k < f.count; k += 32) a += s[(long long)k * step];
+  }
   sh[w][lane] = a;
   __syncthreads();
-  if (w == 0 && c < cols) {
-    for (int i = 1; i < 32; ++i) a += sh[i][lane];
-    out[c] = from_f32<T>(a);
+  if (w == 0 && i < total) {
+    for (int k = 1; k < 32; ++k) a += sh[k][lane];
+    static_cast<T*>(f.out)[i] = from_f32<T>(a);
   }
 }
 
@@ -1348,14 +1359,8 @@ int backward(const LinearShape& s, const LinearPlan& q, const void* x, const voi
                                                   q.colsum_chunk, colsum);
     DDPM_CHECK_LAUNCH("linear_colsum_kernel");
   }
-  if (gb) {
-    linear_fold_rows_kernel<T><<<(s.n + 31) / 32, 1024, 0, st>>>(colsum, q.colsum_rows, s.n,
-                                                                 static_cast<T*>(gb));
-    DDPM_CHECK_LAUNCH("linear_fold_rows_kernel");
-  }
-  if (!gx && !gw) return DDPM_OK;
   Operand zo = Operand{dz, s.m, s.n, ld_dz};
-  if (q.stage_dz) {
+  if (q.stage_dz && (gx || gw)) {
     if ((rc = stage<T>(dz, ld_dz, s.m, s.n, ws + q.dzp_off, st))) return rc;
     zo = Operand{ws + q.dzp_off, s.m, s.n, round8(s.n)};
   }
@@ -1384,19 +1389,35 @@ int backward(const LinearShape& s, const LinearPlan& q, const void* x, const voi
     g.splits = q.splits_w;
     g.tile = q.tile_w;
     if (q.splits_w > 1) {
-      const int pitch = (s.k + 3) / 4 * 4;
       g.out = ws + q.part_off;
-      g.ld_out = pitch;
+      g.ld_out = (s.k + 3) / 4 * 4;
       if ((rc = run_gemm<T, kPartial>(g, st))) return rc;
-      linear_fold_kernel<T><<<small_grid((long long)s.n * s.k), 256, 0, st>>>(
-          reinterpret_cast<const float*>(ws + q.part_off), q.splits_w, s.n, s.k, pitch,
-          static_cast<T*>(gw));
-      DDPM_CHECK_LAUNCH("linear_fold_kernel");
     } else {
       g.out = gw;
       g.ld_out = s.k;
       if ((rc = run_gemm<T, kOut>(g, st))) return rc;
     }
+  }
+  // the sums over partials: of the bias, and of the weight where it was split
+  auto blocks = [](const Fold& f) { return (int)((f.rows * f.cols + 31) / 32); };
+  Fold fb{}, fw{};
+  if (gb) {
+    fb = Fold{colsum, 1, s.n, (int)q.colsum_rows, s.n, 0, gb};
+    fb.blocks = blocks(fb);
+  }
+  if (gw && q.splits_w > 1) {
+    fw = Fold{reinterpret_cast<const float*>(ws + q.part_off), s.n, (s.k + 3) / 4 * 4, q.splits_w,
+              s.k, 0, gw};
+    if (q.splits_w < 16) {
+      linear_fold_kernel<T><<<small_grid(fw.rows * fw.cols), 256, 0, st>>>(fw);
+      DDPM_CHECK_LAUNCH("linear_fold_kernel");
+    } else {
+      fw.blocks = blocks(fw);
+    }
+  }
+  if (fb.blocks + fw.blocks > 0) {
+    linear_fold_long_kernel<T><<<fb.blocks + fw.blocks, 1024, 0, st>>>(fb, fw);
+    DDPM_CHECK_LAUNCH("linear_fold_kernel");
   }
   return DDPM_OK;
 }
