@@ -578,7 +578,7 @@ constexpr int kWork = 32 * kWorkWarps;
 constexpr int kRingThreads = kWork + 32 * (kMergeWarps + kFoldWarps + 1);
 constexpr int kMaxSlots = 8, kRingGroups = 64;
 constexpr int kRingSmem = 196608;     // bytes of the ring
-constexpr int kSlack = 3;             // steps
+constexpr int kSlack = 2;             // steps
 constexpr double kRingBytes = 4e6;    // least size of x
 
 struct RingParams {
