@@ -6,6 +6,9 @@ linked into ``dynamicconvolutionoperator_b200/libddpm_b200.so``. The library is
 a plain C-ABI shared object (see ``include/ddpm_b200.h``); Python loads it with
 ctypes, so no torch headers or torch ABI are involved.
 
+``csrc/torch/*.cpp`` (the operators' autograd side, against torch's headers) goes
+into ``_operators.so`` beside it, which links the library.
+
 Usage: ``python -m dynamicconvolutionoperator_b200._build [--force] [--debug]``.
 """
 
@@ -25,6 +28,7 @@ CSRC = PKG_DIR / "csrc"
 INCLUDE = REPO_DIR / "include"
 BUILD_DIR = REPO_DIR / "_build"
 LIB_PATH = PKG_DIR / "libddpm_b200.so"
+OPERATORS_PATH = PKG_DIR / "_operators.so"
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 BASE_FLAGS = [
@@ -53,6 +57,49 @@ def _stale(obj: Path, src: Path, deps: list[Path]) -> bool:
         return True
     t = obj.stat().st_mtime
     return any(p.stat().st_mtime > t for p in [src, *deps])
+
+
+def _build_operators(force: bool, verbose: bool) -> None:
+    """Compile and link ``_operators.so`` (needs the library)."""
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension
+
+    cuda = Path(_nvcc()).resolve().parents[1]
+    includes = [*cpp_extension.include_paths(), str(cuda / "include"),
+                sysconfig.get_paths()["include"]]
+    flags = ["-std=c++17", "-O2", "-fPIC", "-fvisibility=hidden",
+             "-DTORCH_EXTENSION_NAME=_operators", "-DTORCH_API_INCLUDE_EXTENSION_H",
+             f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+             *(f"-isystem{p}" for p in includes)]
+
+    def run(cmd: list[str], what: str) -> None:
+        if verbose:
+            print(" ".join(cmd), flush=True)
+        res = subprocess.run(cmd, capture_output=True, text=True)
+        if res.returncode != 0:
+            raise RuntimeError(f"{what} failed:\n{res.stdout}\n{res.stderr}")
+
+    cxx = os.environ.get("CXX") or shutil.which("g++") or "g++"
+    objs = []
+    for src in sorted((CSRC / "torch").glob("*.cpp")):
+        obj = BUILD_DIR / "torch" / (src.stem + ".o")
+        obj.parent.mkdir(exist_ok=True)
+        if force or _stale(obj, src, sorted(INCLUDE.glob("*.h"))):
+            run([cxx, *flags, "-c", str(src), "-o", str(obj)], f"compiling {src.name}")
+        objs.append(obj)
+    if force or not OPERATORS_PATH.exists() or any(
+        o.stat().st_mtime > OPERATORS_PATH.stat().st_mtime for o in objs
+    ):
+        tmp = OPERATORS_PATH.with_suffix(".so.tmp")
+        libs = [f"-L{p}" for p in cpp_extension.library_paths()]
+        # the shared C++ runtime by name: a second, static one (all that some images
+        # have for linking) would not catch torch's exceptions, nor torch this one's
+        run([cxx, "-shared", "-o", str(tmp), *map(str, objs), f"-L{PKG_DIR}", f"-l:{LIB_PATH.name}",
+             *libs, "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch", "-ltorch_python",
+             "-l:libstdc++.so.6", "-Wl,-rpath,$ORIGIN"], "linking _operators.so")
+        os.replace(tmp, OPERATORS_PATH)
 
 
 def build(force: bool = False, debug: bool = False, verbose: bool = False) -> Path:
@@ -92,6 +139,7 @@ def build(force: bool = False, debug: bool = False, verbose: bool = False) -> Pa
         if res.returncode != 0:
             raise RuntimeError(f"link failed:\n{res.stdout}\n{res.stderr}")
         os.replace(tmp, LIB_PATH)
+    _build_operators(force, verbose)
     return LIB_PATH
 
 

@@ -10,43 +10,9 @@ from __future__ import annotations
 
 import torch
 
-from . import _lib
-from ._op import first_order, on_one_device, ptr
+from ._op import operators
 
 _U64 = (1 << 64) - 1
-
-
-def _launch(x, residual, p, seed, offset):
-    """``x`` (and ``residual``) contiguous; ``seed`` a number or a tensor."""
-    out = torch.empty_like(x)
-    number, held = (0, seed.data_ptr()) if isinstance(seed, torch.Tensor) else (seed, None)
-    _lib.call_on(x.device, "ddpm_dropout", x.data_ptr(), ptr(residual), out.data_ptr(), x.numel(),
-                 p, number, held, offset, _lib.dtype_code(x.dtype))
-    return out
-
-
-class _Dropout(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, residual, p, seed, offset):
-        # a seed on the device is saved, so that writing to it before the
-        # backward (which has to draw the same mask) raises
-        if isinstance(seed, torch.Tensor):
-            ctx.save_for_backward(seed)
-            ctx.args = (p, None, offset)
-        else:
-            ctx.args = (p, seed, offset)
-        return _launch(x, residual, p, seed, offset)
-
-    @staticmethod
-    @first_order
-    def backward(ctx, grad_out):
-        p, seed, offset = ctx.args
-        gx = None
-        if ctx.needs_input_grad[0]:
-            if seed is None:
-                seed, = ctx.saved_tensors
-            gx = _launch(grad_out.contiguous(), None, p, seed, offset)
-        return gx, grad_out if ctx.needs_input_grad[1] else None, None, None, None
 
 
 def dropout(x: torch.Tensor, p: float, seed: int | torch.Tensor, offset: int = 0,
@@ -74,30 +40,17 @@ def dropout(x: torch.Tensor, p: float, seed: int | torch.Tensor, offset: int = 0
     p = float(p)
     if not 0.0 <= p <= 1.0:
         raise ValueError(f"p must be between 0 and 1, got {p}")
+    held = None
     if isinstance(seed, torch.Tensor):
-        if seed.numel() != 1 or seed.dtype != torch.int64:
-            raise ValueError("a seed tensor must hold one int64 value, got "
-                             f"{tuple(seed.shape)} of {seed.dtype}")
+        seed, held = 0, seed
     else:
         seed = int(seed)
         if not -(1 << 63) <= seed <= _U64:
             raise ValueError(f"seed must fit 64 bits, got {seed}")
-        seed &= _U64
     offset = int(offset)
     if not 0 <= offset <= _U64:
         raise ValueError(f"offset must fit 64 bits and not be negative, got {offset}")
-    if residual is not None:
-        if residual.shape != x.shape or residual.dtype != x.dtype:
-            raise ValueError(f"residual must have x's shape and dtype, got {tuple(residual.shape)} "
-                             f"of {residual.dtype} for {tuple(x.shape)} of {x.dtype}")
-    on_one_device(x, seed if isinstance(seed, torch.Tensor) else None, residual)
-    _lib.dtype_code(x.dtype)
-    x = x.contiguous()
-    residual = residual.contiguous() if residual is not None else None
-    if torch.is_grad_enabled() and (x.requires_grad
-                                    or (residual is not None and residual.requires_grad)):
-        return _Dropout.apply(x, residual, p, seed, offset)
-    return _launch(x, residual, p, seed, offset)
+    return operators().dropout(x, p, seed & _U64, held, offset, residual)
 
 
 __all__ = ["dropout"]

@@ -24,6 +24,8 @@ import torch
 
 # id(param) -> [weakref to param, view, armed]
 _views: dict[int, list] = {}
+# told whether any view is attached (the compiled operators ask for buffers only then)
+_observer = None
 # callables (params, buffers) told when a backward has written gradients
 _listeners: list = []
 
@@ -34,10 +36,21 @@ def attach(param: torch.Tensor, view: torch.Tensor) -> None:
     if view.numel() != param.numel() or view.dtype != param.dtype or view.device != param.device:
         raise ValueError("a gradient view must match its parameter's size, dtype and device")
     _views[id(param)] = [weakref.ref(param), view, True]
+    if _observer is not None:
+        _observer(True)
 
 
 def detach(param: torch.Tensor) -> None:
     _views.pop(id(param), None)
+    if _observer is not None:
+        _observer(bool(_views))
+
+
+def observe(fn) -> None:
+    """Have ``fn(whether any view is attached)`` called now and on every change."""
+    global _observer
+    _observer = fn
+    fn(bool(_views))
 
 
 def arm(param: torch.Tensor) -> None:
@@ -54,9 +67,17 @@ def view_of(param: torch.Tensor) -> torch.Tensor | None:
     return None
 
 
-def attached() -> bool:
-    """Whether any parameter has a view attached."""
-    return bool(_views)
+def take_view(param: torch.Tensor, dtype: torch.dtype | None = None,
+              device: torch.device | None = None) -> torch.Tensor | None:
+    """The attached view of ``param`` when one is armed and ``param.grad`` is
+    ``None`` (handed out once per arming), else ``None``."""
+    ent = _views.get(id(param))
+    if ent is not None and ent[0]() is param and ent[2] and param.grad is None:
+        view = ent[1]
+        if view.dtype == (dtype or param.dtype) and view.device == (device or param.device):
+            ent[2] = False
+            return view
+    return None
 
 
 def grad_buffer(param: torch.Tensor | None, shape, dtype: torch.dtype,
@@ -64,14 +85,8 @@ def grad_buffer(param: torch.Tensor | None, shape, dtype: torch.dtype,
     """Tensor of ``shape`` for the backward to write ``param``'s gradient into:
     the attached view when one is armed and ``param.grad`` is ``None``, else a
     fresh allocation."""
-    if param is not None and _views:
-        ent = _views.get(id(param))
-        if ent is not None and ent[0]() is param and ent[2] and param.grad is None:
-            view = ent[1]
-            if view.dtype == dtype and view.device == device:
-                ent[2] = False
-                return view.view(shape)
-    return torch.empty(shape, dtype=dtype, device=device)
+    view = take_view(param, dtype, device) if param is not None else None
+    return torch.empty(shape, dtype=dtype, device=device) if view is None else view.view(shape)
 
 
 def add_listener(fn) -> None:
@@ -95,5 +110,5 @@ def grads_written(params, buffers) -> None:
         fn(tuple(params), tuple(buffers))
 
 
-__all__ = ["add_listener", "arm", "attach", "attached", "detach", "grad_buffer", "grads_written",
-           "remove_listener", "view_of"]
+__all__ = ["add_listener", "arm", "attach", "detach", "grad_buffer", "grads_written", "observe",
+           "remove_listener", "take_view", "view_of"]

@@ -148,7 +148,6 @@ _SIGNATURES: dict[str, tuple[object, list[object]]] = {
 
 _lock = threading.Lock()
 _lib: ctypes.CDLL | None = None
-_calls: dict[str, object] = {}  # entry points by name
 
 
 def exported_symbols() -> list[str]:
@@ -180,29 +179,11 @@ def load() -> ctypes.CDLL:
 
 def call(name: str, *args) -> None:
     """Invoke an entry point; a non-zero return raises RuntimeError with its message."""
-    fn = _calls.get(name)
-    if fn is None:
-        fn = _calls[name] = getattr(load(), name)
-    rc = fn(*args)
+    lib = load()
+    rc = getattr(lib, name)(*args)
     if rc != 0:
-        msg = load().ddpm_last_error().decode(errors="replace")
+        msg = lib.ddpm_last_error().decode(errors="replace")
         raise RuntimeError(f"{name} failed (code {rc}): {msg}")
-
-
-# torch's current stream without the stream object around it
-_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
-    lambda index: torch.cuda.current_stream(index).cuda_stream)
-
-
-def call_on(device: torch.device, name: str, *args) -> None:
-    """``call`` with ``device`` current and torch's current stream on it as the
-    last argument."""
-    index = device.index
-    if torch.cuda.current_device() == index:
-        call(name, *args, _raw_stream(index))
-    else:
-        with torch.cuda.device(index):
-            call(name, *args, _raw_stream(index))
 
 
 def device_status(reset: bool = True) -> int:

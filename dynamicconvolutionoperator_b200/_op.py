@@ -1,16 +1,22 @@
-"""What the channel-last operators share on the host."""
+"""What the channel-last operators share on the host: the compiled module
+``_operators.so`` (``csrc/torch/operators.cpp``), which checks arguments,
+allocates and calls the C ABI for autograd, and the activations' names.
+
+Like the kernels' library it is loaded from this package only; there is no
+fallback. Build both with ``python -m dynamicconvolutionoperator_b200._build``.
+"""
 
 from __future__ import annotations
 
-import functools
+import importlib
 
 import torch
-from torch.autograd.function import once_differentiable
 
-from . import _gradbuf
-from ._kernels import _require_cuda
+from . import _gradbuf, _lib
 
 ACTIVATIONS = {None: 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}
+
+_module = None
 
 
 def activation_code(activation: str | None) -> int:
@@ -21,51 +27,25 @@ def activation_code(activation: str | None) -> int:
                          f"None, got {activation!r}") from None
 
 
-def ptr(t: torch.Tensor | None) -> int | None:
-    return t.data_ptr() if t is not None else None
+def _grad_buffer(param: torch.Tensor) -> torch.Tensor | None:
+    view = _gradbuf.take_view(param)
+    return None if view is None else view.view(param.shape)
 
 
-def aligned(*pointers: int | None) -> bool:
-    """Whether every address is on a 16-byte boundary."""
-    bits = 0
-    for p in pointers:
-        bits |= p or 0
-    return bits % 16 == 0
+def operators():
+    """The compiled module (loaded once)."""
+    global _module
+    if _module is None:
+        _lib.load()
+        try:
+            module = importlib.import_module("._operators", __package__)
+        except ImportError as e:
+            raise RuntimeError(
+                "_operators.so is not built or does not load; run "
+                f"`python -m dynamicconvolutionoperator_b200._build` ({e})") from e
+        _gradbuf.observe(lambda attached: module.set_grad_buffer(_grad_buffer if attached else None))
+        _module = module
+    return _module
 
 
-def param_grad(param: torch.Tensor) -> torch.Tensor:
-    """Where the backward writes ``param``'s gradient (contiguous): an attached
-    buffer, or a new tensor."""
-    if _gradbuf.attached():
-        return _gradbuf.grad_buffer(param, param.shape, param.dtype, param.device)
-    return torch.empty_like(param, memory_format=torch.contiguous_format)
-
-
-def on_one_device(x: torch.Tensor, *others: torch.Tensor | None) -> None:
-    """Raise unless every tensor is on ``x``'s CUDA device."""
-    if not x.is_cuda:
-        _require_cuda(x)
-    index = x.get_device()
-    for t in others:
-        if t is not None and t.get_device() != index:
-            _require_cuda(x, t)
-
-
-def workspace(nbytes: int, device: torch.device) -> torch.Tensor | None:
-    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
-
-
-def first_order(backward):
-    """``once_differentiable`` (a second derivative raises), at no cost where
-    the graph of the backward is not recorded."""
-    recorded = once_differentiable(backward)
-
-    @functools.wraps(backward)
-    def run(ctx, *grads):
-        return recorded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
-
-    return run
-
-
-__all__ = ["ACTIVATIONS", "activation_code", "aligned", "first_order", "on_one_device",
-           "param_grad", "ptr", "workspace"]
+__all__ = ["ACTIVATIONS", "activation_code", "operators"]
