@@ -16,6 +16,11 @@
 // integer multiplies close behind for 16-bit data: 20 32x32->64-bit products
 // per four values. Hence one Philox block serves four neighbouring values and
 // a thread handles 16 bytes (one or two blocks) per step.
+//
+// Measured, 268M values: bf16 264 us (4.1 TB/s; the pipe of the wide multiplies is
+// 80 % busy, and neither more resident warps nor a longer grid changes it), with a
+// residual 284 us (5.7 TB/s), FP32 402 us (5.3 TB/s; a copy: 329 us). An offset
+// that is no multiple of four: 405 us.
 #include "act.cuh"
 #include "common.cuh"
 

@@ -573,6 +573,14 @@ __global__ void __launch_bounds__(256) norm_param_kernel(const float2* __restric
 // no role waits for another's round trip: the counting is a reduction without
 // an answer, and every block folds the samples that it writes, all in the same
 // order. A slot holds a chunk of x (backward: of x and dy).
+//
+// Measured, 64 x 256 x 256 x 64 bf16 with silu: forward 281 us (3.8 TB/s of the
+// 1.07 GB it has to move), backward 535 us (3.0 TB/s); the other kernel took 908
+// and 2306. Neither a unit nor HBM is the limit but the steps' chains (copy, sums,
+// merge, count, fold, write): larger slots (three of 64 KB instead of four of 48:
+// 335 -> 290 us) help, fewer work warps (12 instead of 20) cost nothing, and a
+// lag of two steps beyond what the sums need hides the folds (none: 435 us),
+// while a longer one leaves L2 (195 MB read for 134 at three).
 constexpr int kWorkWarps = 20, kMergeWarps = 4, kFoldWarps = 4;
 constexpr int kWork = 32 * kWorkWarps;
 constexpr int kRingThreads = kWork + 32 * (kMergeWarps + kFoldWarps + 1);

@@ -42,8 +42,16 @@
 // dweight sums over all rows: its K axis is split over the SMs left without a
 // tile, FP32 partials are added in a fixed order.
 //
+// Measured (bf16): 16384 x 1024 -> 4096 107 us (1280 TFLOP/s, 0.76 of the
+// measured peak; without its copies 98 us), with gelu 121 us; 8192^3 760 us (1450
+// TFLOP/s); 65536 x 64 -> 1728 78 us (3.0 TB/s, bound by the epilogue's chain: its
+// warps' TMEM loads, stores to the boxes, fences). FP32: 8192 x 2048 -> 2048 540 us
+// (127 TFLOP/s of FP32 products; bound by shared memory, through which a K block
+// moves 208 KB, and by the splitting), 65536 x 256 -> 64 41 us.
+//
 // Up to eight rows, forward: a dot-product kernel reads the weight once at the
-// memory's rate; a tensor-core tile would be 15/16 empty and its K loop serial.
+// memory's rate; a tensor-core tile would be 15/16 empty and its K loop serial (1024 -> 4096
+// bf16: 3.2 us, 2.6 TB/s).
 #include <atomic>
 #include <type_traits>
 
