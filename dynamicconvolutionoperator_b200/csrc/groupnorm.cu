@@ -574,13 +574,14 @@ __global__ void __launch_bounds__(256) norm_param_kernel(const float2* __restric
 // an answer, and every block folds the samples that it writes, all in the same
 // order. A slot holds a chunk of x (backward: of x and dy).
 //
-// Measured, 64 x 256 x 256 x 64 bf16 with silu: forward 281 us (3.8 TB/s of the
-// 1.07 GB it has to move), backward 535 us (3.0 TB/s); the other kernel took 908
+// Measured, 64 x 256 x 256 x 64 bf16 with silu: forward 271 us (4.0 TB/s of the
+// 1.07 GB it has to move), backward 527 us (3.1 TB/s); the other kernel took 908
 // and 2306. Neither a unit nor HBM is the limit but the steps' chains (copy, sums,
 // merge, count, fold, write): larger slots (three of 64 KB instead of four of 48:
 // 335 -> 290 us) help, fewer work warps (12 instead of 20) cost nothing, and a
-// lag of two steps beyond what the sums need hides the folds (none: 435 us),
-// while a longer one leaves L2 (195 MB read for 134 at three).
+// lag of two steps beyond what the sums need hides the folds (none: 435 us). The
+// copies' L2 policies keep a chunk until its second reading (backward of a fourth
+// of that size: 399 -> 271 MB read from HBM, of 268).
 constexpr int kWorkWarps = 20, kMergeWarps = 4, kFoldWarps = 4;
 constexpr int kWork = 32 * kWorkWarps;
 constexpr int kRingThreads = kWork + 32 * (kMergeWarps + kFoldWarps + 1);
@@ -632,6 +633,17 @@ template <typename T> __device__ __forceinline__ void store4(T* p, const F2 (&v)
     __stcs(reinterpret_cast<float4*>(p), make_float4(a.x, a.y, b.x, b.y));
   else
     __stcs(reinterpret_cast<uint2*>(p), make_uint2(pack2<T>(a.x, a.y), pack2<T>(b.x, b.y)));
+}
+
+// Bulk copy with an L2 policy: a chunk that is read again a few steps later is
+// to stay, the second reading lets it go.
+__device__ __forceinline__ void bulk_g2s_hint(void* dst, const void* src, uint32_t bytes,
+                                              uint64_t* bar, uint64_t policy) {
+  asm volatile(
+      "cp.async.bulk.shared::cta.global.mbarrier::complete_tx::bytes.L2::cache_hint"
+      " [%0], [%1], %2, [%3], %4;" ::"r"(tc::smem_u32(dst)),
+      "l"(src), "r"(bytes), "r"(tc::smem_u32(bar)), "l"(policy)
+      : "memory");
 }
 
 // Warp-uniform bounded wait (the clock is read only in a long one).
@@ -703,7 +715,11 @@ __global__ void __launch_bounds__(kRingThreads, 1) norm_ring_kernel(const RingPa
     int s = 0;             // the next slot, and the parity of its next copy
     uint32_t turn = 0;
     Walk first(p), second(p);
-    auto fetch = [&](Walk& walk) {
+    uint64_t keep, drop;
+    asm("createpolicy.fractional.L2::evict_last.b64 %0, 1.0;" : "=l"(keep));
+    asm("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(drop));
+    if (rp.resident || !write) keep = drop;  // read once
+    auto fetch = [&](Walk& walk, uint64_t policy) {
       if (!ring_wait(&sh.empty[s], turn ^ 1, abort_flag)) {
         fail(96);
         ok = false;
@@ -715,10 +731,10 @@ __global__ void __launch_bounds__(kRingThreads, 1) norm_ring_kernel(const RingPa
         uint8_t* slot = ring + (size_t)s * rp.slot_bytes;
         const long long at = k.at * p.C * (long long)sizeof(T);
         tc::mbar_expect_tx(&sh.full[s], kBwd ? 2 * bytes : bytes);
-        tc::bulk_g2s(slot, static_cast<const uint8_t*>(p.x) + at, bytes, &sh.full[s]);
+        bulk_g2s_hint(slot, static_cast<const uint8_t*>(p.x) + at, bytes, &sh.full[s], policy);
         if constexpr (kBwd)
-          tc::bulk_g2s(slot + rp.slot_bytes / 2, static_cast<const uint8_t*>(p.dy) + at, bytes,
-                       &sh.full[s]);
+          bulk_g2s_hint(slot + rp.slot_bytes / 2, static_cast<const uint8_t*>(p.dy) + at, bytes,
+                        &sh.full[s], policy);
       }
       if constexpr (kBwd) {
         for (int g = lane; g < p.G; g += 32) sh.stat1[s][g] = __ldg(&p.stats[(long long)k.n * p.G + g]);
@@ -732,8 +748,8 @@ __global__ void __launch_bounds__(kRingThreads, 1) norm_ring_kernel(const RingPa
       }
     };
     for (int i = 0; i < steps && ok; ++i) {
-      if (i < mine) fetch(first);
-      if (ok && !rp.resident && write && i >= p.lag) fetch(second);
+      if (i < mine) fetch(first, keep);
+      if (ok && !rp.resident && write && i >= p.lag) fetch(second, drop);
     }
     if (!ok || *abort_flag) {  // what is in flight lands first
       const uint32_t n = q < (uint32_t)rp.slots ? q : (uint32_t)rp.slots;
