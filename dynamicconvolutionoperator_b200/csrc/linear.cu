@@ -18,7 +18,8 @@
 //             columns and k are zero filled, which covers every ragged size
 //   issue     tcgen05.mma of 128 x BN x 16 by one thread; two TMEM
 //             accumulators, so the epilogue of a tile overlaps the next one
-//   epilogue  8 or 16 warps (lane = row, 2 or 4 column parts): TMEM -> registers,
+//   epilogue  one or two groups of 8 warps (lane = row, two column halves; two
+//             groups take the tiles in turn): TMEM -> registers,
 //             bias, activation, residual -> 128-byte x 32-row boxes in shared
 //             memory -> TMA store. The residual (or dy) comes through the same
 //             boxes by TMA, several boxes ahead.
@@ -44,7 +45,7 @@
 //
 // Measured (bf16): 16384 x 1024 -> 4096 107 us (1280 TFLOP/s, 0.76 of the
 // measured peak; without its copies 98 us), with gelu 121 us; 8192^3 760 us (1450
-// TFLOP/s); 65536 x 64 -> 1728 78 us (3.0 TB/s, bound by the epilogue's chain: its
+// TFLOP/s); 65536 x 64 -> 1728 72 us (3.3 TB/s, bound by the epilogue's chain: its
 // warps' TMEM loads, stores to the boxes, fences). FP32: 8192 x 2048 -> 2048 540 us
 // (127 TFLOP/s of FP32 products; bound by shared memory, through which a K block
 // moves 208 KB, and by the splitting), 65536 x 256 -> 64 41 us.
@@ -98,11 +99,8 @@ struct GemmParams {
   int* status;
 };
 
-// A box of the epilogue: 32 rows x 128 bytes (64 where a warp has no more
-// columns: a quarter of the warps share each quarter of the rows).
-__host__ __device__ constexpr int box_row(int bn, int ew, int es) {
-  return bn / (ew / 4) * es < 128 ? 64 : 128;
-}
+// A box of the epilogue: 32 rows x 128 bytes (64 where half a tile is no wider).
+__host__ __device__ constexpr int box_row(int bn, int es) { return bn / 2 * es < 128 ? 64 : 128; }
 
 struct SmemLayout {
   uint32_t stage, planes, boxes, bias, total;
@@ -115,7 +113,7 @@ __host__ __device__ inline SmemLayout smem_layout(int cg, int parts, int bn, int
   L.planes = L.stage * stages;
   L.boxes = L.planes + (parts == 3 ? 2 * 3 * (kBM + bn) * 64 : 0);
   L.bias = L.boxes + ew * nbuf * 32 * row;
-  L.total = L.bias + (parts == 3 ? 0 : bn * 16) + 1024;  // + alignment
+  L.total = L.bias + (parts == 3 ? 0 : ew * (bn / 2) * 4) + 1024;  // + alignment
   return L;
 }
 
@@ -281,8 +279,9 @@ __global__ void __launch_bounds__(gemm_threads(PARTS, EW), 1)
 linear_gemm_kernel(const __grid_constant__ GemmParams p) {
   using To = typename std::conditional<kEpi == kPartial, float, T>::type;
   constexpr bool kFast = sizeof(T) == 2;
-  constexpr int kCols = BN / (EW / 4);             // columns of a warp's part of a tile
-  constexpr int kRow = box_row(BN, EW, sizeof(To));  // bytes of a box row
+  constexpr int kGroups = EW / 8;                  // groups of 8 warps take the tiles in turn
+  constexpr int kCols = BN / 2;                    // columns of a warp's part of a tile
+  constexpr int kRow = box_row(BN, sizeof(To));    // bytes of a box row
   constexpr int kFirstSplit = kFirstEpi + EW;
   constexpr int kBox = 32 * kRow;
   constexpr int kCB = kRow / (int)sizeof(To);      // columns of a box
@@ -314,7 +313,7 @@ linear_gemm_kernel(const __grid_constant__ GemmParams p) {
     }
     for (int i = 0; i < 2; ++i) {
       tc::mbar_init(&acc_full[i], 1);
-      tc::mbar_init(&acc_empty[i], CG * EW);
+      tc::mbar_init(&acc_empty[i], CG * 8);
       tc::mbar_init(&parts_full[i], 4);
       tc::mbar_init(&parts_empty[i], 1);
     }
@@ -557,7 +556,7 @@ linear_gemm_kernel(const __grid_constant__ GemmParams p) {
   } else if (warp >= kFirstEpi) {  // ---- epilogue ----
     const int ew = warp - kFirstEpi;
     const bool lead = tc::elect_one();  // copies, stores and arrivals of the warp
-    const int quad = warp & 3, part = ew >> 2;  // rows and columns of the warp
+    const int group = ew >> 3, quad = warp & 3, part = (ew >> 2) & 1;
     uint8_t* boxes = smem + L.boxes + ew * p.nbuf * kBox;
     float* bias_s = reinterpret_cast<float*>(smem + L.bias) + ew * kCols;
     const To* in = static_cast<const To*>(p.in_ptr);
@@ -573,9 +572,9 @@ linear_gemm_kernel(const __grid_constant__ GemmParams p) {
     auto value_at = [&](int r, int c) {
       return chunk_at(r, c / kPer) + (c % kPer) * (int)sizeof(To);
     };
-    uint32_t ti = 0, q = 0;
+    uint32_t ti = group, q = 0;
     // the load cursor: box `lj` of tile `lt`
-    int lt = first_tile, lj = 0;
+    int lt = first_tile + group * tile_step, lj = 0;
     uint32_t lq = 0;
     auto load_next = [&]() {  // the elected lane
       if (lt >= p.num_tiles) return;
@@ -592,13 +591,14 @@ linear_gemm_kernel(const __grid_constant__ GemmParams p) {
       ++lq;
       if (++lj == kBoxes) {
         lj = 0;
-        lt += tile_step;
+        lt += kGroups * tile_step;
       }
     };
     if (p.tma_io && has_in && lead)
       for (int i = 0; i < ahead; ++i) load_next();
     bool ok = true;
-    for (int t = first_tile; t < p.num_tiles && ok; t += tile_step) {
+    for (int t = first_tile + group * tile_step; t < p.num_tiles && ok;
+         t += kGroups * tile_step) {
       int tm, tn, sp;
       tile_at(p, t, tm, tn, sp);
       const int row0 = (tm * CG + rank) * kBM + quad * 32;
@@ -795,7 +795,7 @@ linear_gemm_kernel(const __grid_constant__ GemmParams p) {
         if (p.tma_io && lead) tc::bulk_commit();
       }
       if (!ok) break;
-      if constexpr (PARTS == 1) ++ti;
+      if constexpr (PARTS == 1) ti += kGroups;
     }
     if (p.tma_io && lead) {
       if (!ok || *abort_flag) {  // loads ahead of the failure land first
@@ -1017,7 +1017,7 @@ Tile pick_tile(long long m, int n, long long k, int parts, int splits) {
       if (least == 0 || t < least) {
         least = t;
         // a short K loop leaves the epilogue as the longest part of a tile: twice
-        // the warps there (65536 x 64 -> 1728: 94 -> 78 us), which a long one
+        // the warps there (65536 x 64 -> 1728: 94 -> 72 us), which a long one
         // would pay for with a stage
         best = Tile{bn, cg, bn == 256 && kb <= kShortK ? 16 : 8};
       }
@@ -1028,7 +1028,7 @@ Tile pick_tile(long long m, int n, long long k, int parts, int splits) {
 template <typename T, int BN, int PARTS, Epi kEpi, int CG, int EW>
 int launch_gemm_as(GemmParams& p, cudaStream_t st) {
   auto fn = linear_gemm_kernel<T, BN, PARTS, kEpi, CG, EW>;
-  constexpr int kRow = box_row(BN, EW, kEpi == kPartial ? 4 : (int)sizeof(T));
+  constexpr int kRow = box_row(BN, kEpi == kPartial ? 4 : (int)sizeof(T));
   const int tiles_k = (p.kblocks + p.splits - 1) / p.splits;
   const int limit = gencat::max_smem_optin() - 2048;  // static shared memory
   // As many stages as the K loop can use, at least two; what is left goes to
@@ -1171,7 +1171,7 @@ int run_gemm(const Gemm& g, cudaStream_t st) {
   if (rc) return rc;
   rc = operand_map(&p.b, g.b, g.b_mn, bn / g.tile.cg, (int)sizeof(T), kBf16);
   if (rc) return rc;
-  const int row = box_row(bn, sizeof(T) == 4 ? 8 : g.tile.ew, es);
+  const int row = box_row(bn, es);
   if (p.tma_io) {
     rc = io_map(&p.out, g.out, es, kBf16, g.M, g.N, g.ld_out, g.splits, row);
     if (rc) return rc;
