@@ -43,6 +43,13 @@
 // dweight sums over all rows: its K axis is split over the SMs left without a
 // tile, FP32 partials are added in a fixed order.
 //
+// 16-bit data, long sums: an addition in the tensor cores cuts off what lies below
+// the sum's last bit, so that a chain of them is biased towards zero by up to 2^-23
+// of the sum an addition (16 values of k). Same-sign fp16 data measured -3.9e-4 of
+// the sum at 65536 values and -6.2e-3 at 2^20, more than half a step of bf16. An
+// accumulator takes kChain values of k at most (-1.0e-4); longer sums are split, and
+// their FP32 partials added (and the epilogue applied) by a kernel of its own.
+//
 // Measured (bf16): 16384 x 1024 -> 4096 107 us (1280 TFLOP/s, 0.76 of the
 // measured peak; without its copies 98 us), with gelu 121 us; 8192^3 760 us (1450
 // TFLOP/s); 65536 x 64 -> 1728 72 us (3.3 TB/s, bound by the epilogue's chain: its
@@ -82,6 +89,7 @@ constexpr int kMaxStages = 8, kMaxBufs = 8;
 constexpr uint64_t kWaitNs = 2000000000ull;
 constexpr int kGemvRows = 8;
 constexpr int kShortK = 8;  // K blocks
+constexpr int kChain = 16384;  // values of k an accumulator sums (16-bit data)
 
 enum Epi { kOut, kDz, kPartial };
 
@@ -912,6 +920,55 @@ __global__ void __launch_bounds__(1024) linear_fold_long_kernel(const Fold f0, c
   }
 }
 
+// The epilogue of a product whose K axis was split: the partials [splits][M][pitch]
+// in order, then what the product's own epilogue does. 32 rows of 256 columns a
+// block, a column a thread (kDz: its sum over the 32 rows is one of `colsum`).
+struct Finish {
+  const float* part;
+  long long M, pitch;
+  int splits, N, tiles_n, act;
+  const void* bias;  // nullable
+  const void* in;    // residual (kOut, nullable) or dy (kDz), [M][N]
+  void* out;
+  long long ld_out;
+  float* colsum;     // nullable
+};
+template <typename T, Epi kEpi>
+__global__ void __launch_bounds__(256) linear_finish_kernel(const Finish f) {
+  const int tm = (int)(blockIdx.x / (unsigned)f.tiles_n);
+  const int c = (int)(blockIdx.x - (unsigned)tm * f.tiles_n) * 256 + (int)threadIdx.x;
+  if (c >= f.N) return;
+  const long long row0 = tm * 32LL;
+  const int rows = (int)min(32LL, f.M - row0);
+  const float bias = f.bias ? to_f32<T>(static_cast<const T*>(f.bias)[c]) : 0.f;
+  const T* in = static_cast<const T*>(f.in);
+  T* out = static_cast<T*>(f.out);
+  float total = 0.f;
+  for (int r = 0; r < rows; r += 2) {
+    float v[2] = {0.f, 0.f};
+    for (int k = 0; k < f.splits; ++k)
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        if (r + e < rows) v[e] += f.part[(k * f.M + row0 + r + e) * f.pitch + c];
+    v[0] += bias;
+    v[1] += bias;
+    if constexpr (kEpi == kOut) act_values<sizeof(T) == 2, 2>(f.act, v);
+    else act_slopes<sizeof(T) == 2, 2>(f.act, v);
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+      if (r + e < rows) {
+        const long long row = row0 + r + e;
+        if (in != nullptr) {
+          const float u = to_f32<T>(in[row * f.N + c]);
+          v[e] = kEpi == kOut ? v[e] + u : v[e] * u;
+        }
+        out[row * f.ld_out + c] = from_f32<T>(v[e]);
+        total += v[e];
+      }
+  }
+  if (kEpi == kDz && f.colsum != nullptr) f.colsum[(long long)tm * f.N + c] = total;
+}
+
 // Forward of up to kGemvRows rows: a warp per output column, V values of the
 // weight a lane and load, FP32 products.
 template <typename T, int V, int MR>
@@ -1183,11 +1240,46 @@ int run_gemm(const Gemm& g, cudaStream_t st) {
   return launch_gemm<T, kEpi>(p, g.tile, st);
 }
 
+long long pitch4(int n) { return (n + 3) / 4 * 4; }
+
+// A product with an epilogue, over `part` (FP32 partials) where it is split.
+template <typename T, Epi kEpi>
+int run_product(Gemm g, float* part, cudaStream_t st) {
+  if constexpr (sizeof(T) == 2) {  // FP32 data needs no splits here
+    if (g.splits > 1) {
+      Finish f{};
+      f.part = part;
+      f.M = g.M;
+      f.pitch = pitch4(g.N);
+      f.splits = g.splits;
+      f.N = g.N;
+      f.tiles_n = (g.N + 255) / 256;
+      f.act = g.act;
+      f.bias = g.bias;
+      f.in = g.in;
+      f.out = g.out;
+      f.ld_out = g.ld_out;
+      f.colsum = g.colsum;
+      g.out = part;
+      g.ld_out = f.pitch;
+      g.bias = g.in = nullptr;
+      g.colsum = nullptr;
+      const int rc = run_gemm<T, kPartial>(g, st);
+      if (rc) return rc;
+      const long long blocks = (g.M + 31) / 32 * f.tiles_n;
+      linear_finish_kernel<T, kEpi><<<(unsigned)blocks, 256, 0, st>>>(f);
+      DDPM_CHECK_LAUNCH("linear_finish_kernel");
+      return DDPM_OK;
+    }
+  }
+  return run_gemm<T, kEpi>(g, st);
+}
+
 // What a call has to lay out in its workspace.
 struct LinearPlan {
   bool rows_path;            // the dot-product kernel
   bool stage_x, stage_w, stage_dz;
-  int parts, splits_w;
+  int parts, splits_z, splits_x, splits_w;
   Tile tile_z, tile_x, tile_w;
   long long colsum_rows, colsum_chunk;
   size_t x_off, w_off, dz_off, dzp_off, colsum_off, part_off, total;
@@ -1220,14 +1312,25 @@ LinearPlan plan_linear(const LinearShape& s, bool bwd) {
     q.x_off = q.stage_x ? take(staged_bytes(s.m, s.k, es)) : 0;
     q.w_off = q.stage_w ? take(staged_bytes(s.n, s.k, es)) : 0;
   }
-  q.tile_z = pick_tile(s.m, s.n, s.k, q.parts, 1);
+  // splits that a sum over k values needs
+  auto chains = [&](long long k) { return f32 ? 1 : (int)((k + kChain - 1) / kChain); };
+  q.splits_z = chains(s.k);
+  q.tile_z = pick_tile(s.m, s.n, s.k, q.parts, q.splits_z);
+  size_t part = 0;  // the products use the partials' memory one after the other
+  auto partials = [&](int splits, long long rows, int cols) {
+    const size_t bytes = splits > 1 ? (size_t)splits * rows * pitch4(cols) * 4 : 0;
+    if (bytes > part) part = bytes;
+  };
+  if (!q.rows_path && (!bwd || s.act != DDPM_ACT_NONE)) partials(q.splits_z, s.m, s.n);
   if (bwd) {
     const bool recompute = s.act != DDPM_ACT_NONE;
     // dz: recomputed, or dy, copied where TMA cannot address it
     if (recompute) q.dz_off = take((size_t)s.m * round8(s.n) * es);
     q.stage_dz = !recompute && (!s.aligned || s.n % (16 / es));
     q.dzp_off = q.stage_dz ? take(staged_bytes(s.m, s.n, es)) : 0;
-    q.tile_x = pick_tile(s.m, s.k, s.n, q.parts, 1);
+    q.splits_x = chains(s.n);
+    q.tile_x = pick_tile(s.m, s.k, s.n, q.parts, q.splits_x);
+    partials(q.splits_x, s.m, s.k);
     if (recompute) {
       q.colsum_rows = (s.m + 31) / 32;  // a row of sums for every 32 rows
     } else {
@@ -1251,13 +1354,19 @@ LinearPlan plan_linear(const LinearShape& s, bool bwd) {
       const long long tiles = (long long)((s.n + kBM - 1) / kBM) * ((s.k + bn - 1) / bn);
       long long splits = gencat::num_sms() / tiles;
       if (splits > kb / 4) splits = kb / 4;
+      const int need = chains(s.m);
       if (splits > 1) {
-        q.splits_w = (int)splits;
+        // whole rounds of the SMs where the sum needs more splits
+        q.splits_w = (int)((need + splits - 1) / splits * splits);
         q.tile_w = Tile{bn, 1, 8};
+      } else if (need > 1) {
+        q.splits_w = need;
+        q.tile_w = pick_tile(s.n, s.k, s.m, q.parts, need);
       }
     }
-    if (q.splits_w > 1) q.part_off = take((size_t)q.splits_w * s.n * ((s.k + 3) / 4 * 4) * 4);
+    partials(q.splits_w, s.n, s.k);
   }
+  if (part > 0) q.part_off = take(part);
   q.total = at;
   return q;
 }
@@ -1320,9 +1429,9 @@ int forward(const LinearShape& s, const LinearPlan& q, const void* x, const void
   g.out = out;
   g.ld_out = s.n;
   g.act = s.act;
-  g.splits = 1;
+  g.splits = q.splits_z;
   g.tile = q.tile_z;
-  return run_gemm<T, kOut>(g, st);
+  return run_product<T, kOut>(g, reinterpret_cast<float*>(ws + q.part_off), st);
 }
 
 template <typename T>
@@ -1340,6 +1449,7 @@ int backward(const LinearShape& s, const LinearPlan& q, const void* x, const voi
   const Operand wo = q.stage_w ? Operand{ws + q.w_off, s.n, s.k, round8(s.k)}
                                : Operand{w, s.n, s.k, s.k};
   float* colsum = reinterpret_cast<float*>(ws + q.colsum_off);
+  float* part = reinterpret_cast<float*>(ws + q.part_off);
   const void* dz = dy;
   long long ld_dz = s.n;
   if (recompute) {
@@ -1356,9 +1466,9 @@ int backward(const LinearShape& s, const LinearPlan& q, const void* x, const voi
     g.ld_out = round8(s.n);
     g.act = s.act;
     g.colsum = gb ? colsum : nullptr;
-    g.splits = 1;
+    g.splits = q.splits_z;
     g.tile = q.tile_z;
-    if ((rc = run_gemm<T, kDz>(g, st))) return rc;
+    if ((rc = run_product<T, kDz>(g, part, st))) return rc;
     dz = g.out;
     ld_dz = g.ld_out;
   } else if (gb) {
@@ -1382,9 +1492,9 @@ int backward(const LinearShape& s, const LinearPlan& q, const void* x, const voi
     g.K = s.n;
     g.out = gx;
     g.ld_out = s.k;
-    g.splits = 1;
+    g.splits = q.splits_x;
     g.tile = q.tile_x;
-    if ((rc = run_gemm<T, kOut>(g, st))) return rc;
+    if ((rc = run_product<T, kOut>(g, part, st))) return rc;
   }
   if (gw) {
     Gemm g{};
@@ -1397,8 +1507,8 @@ int backward(const LinearShape& s, const LinearPlan& q, const void* x, const voi
     g.splits = q.splits_w;
     g.tile = q.tile_w;
     if (q.splits_w > 1) {
-      g.out = ws + q.part_off;
-      g.ld_out = (s.k + 3) / 4 * 4;
+      g.out = part;
+      g.ld_out = pitch4(s.k);
       if ((rc = run_gemm<T, kPartial>(g, st))) return rc;
     } else {
       g.out = gw;
@@ -1414,8 +1524,7 @@ int backward(const LinearShape& s, const LinearPlan& q, const void* x, const voi
     fb.blocks = blocks(fb);
   }
   if (gw && q.splits_w > 1) {
-    fw = Fold{reinterpret_cast<const float*>(ws + q.part_off), s.n, (s.k + 3) / 4 * 4, q.splits_w,
-              s.k, 0, gw};
+    fw = Fold{part, s.n, pitch4(s.k), q.splits_w, s.k, 0, gw};
     if (q.splits_w < 16) {
       linear_fold_kernel<T><<<small_grid(fw.rows * fw.cols), 256, 0, st>>>(fw);
       DDPM_CHECK_LAUNCH("linear_fold_kernel");
