@@ -127,6 +127,15 @@ bool recorded(std::initializer_list<Tensor> tensors) {
   return false;
 }
 
+// The operators have no forward-mode derivative: an output without a tangent
+// would count as one whose derivative is zero.
+void no_tangents(std::initializer_list<Tensor> tensors) {
+  if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+  for (const Tensor& t : tensors)
+    TORCH_CHECK(!t.defined() || !t._fw_grad(0).defined(),
+                "the DDPM B200 operators have no forward-mode derivative");
+}
+
 // -------------------------------------------------------------- group norm ----
 // [N, C, *] as contiguous [N, *, C] (no copy for channel-last memory), and back.
 Tensor channel_last(const Tensor& t) {
@@ -182,6 +191,7 @@ struct GroupNormAct : torch::autograd::Function<GroupNormAct> {
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    no_tangents({grads[0]});
     const variable_list saved = ctx->get_saved_variables();
     const Tensor &xl = saved[0], &weight = saved[1], &bias = saved[2];
     const int groups = (int)ctx->saved_data["groups"].toInt();
@@ -215,6 +225,7 @@ struct GroupNormAct : torch::autograd::Function<GroupNormAct> {
 Tensor group_norm_act(const Tensor& x, int64_t groups, const Maybe& weight,
                       const Maybe& bias, double eps, int64_t act) {
   const Tensor w = or_none(weight), b = or_none(bias);
+  no_tangents({x, w, b});
   CHECK_VALUE(x.dim() >= 2, "x must have at least two dimensions [N, C, *], got ", x.sizes());
   const int64_t c = x.size(1);
   CHECK_VALUE(groups >= 1 && c >= 1 && c % groups == 0,
@@ -293,6 +304,7 @@ struct LinearAct : torch::autograd::Function<LinearAct> {
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    no_tangents({grads[0]});
     const variable_list saved = ctx->get_saved_variables();
     const Tensor &flat = saved[0], &weight = saved[1], &bias = saved[2];
     const int act = (int)ctx->saved_data["act"].toInt();
@@ -328,6 +340,7 @@ struct LinearAct : torch::autograd::Function<LinearAct> {
 Tensor linear_act(const Tensor& x, const Tensor& weight, const Maybe& bias,
                   int64_t act, const Maybe& residual) {
   const Tensor b = or_none(bias), res = or_none(residual);
+  no_tangents({x, weight, b, res});
   CHECK_VALUE(x.dim() >= 1, "x must have at least one dimension [..., k]");
   const int64_t k = x.size(-1), dims = weight.dim();
   CHECK_VALUE((dims == 2 || (dims == 4 && weight.size(2) == 1 && weight.size(3) == 1)) &&
@@ -381,6 +394,7 @@ struct Dropout : torch::autograd::Function<Dropout> {
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    no_tangents({grads[0]});
     const bool residual = ctx->saved_data["residual"].toBool();
     const auto need = needed(ctx, {true, residual});
     Tensor gx;
@@ -395,6 +409,7 @@ struct Dropout : torch::autograd::Function<Dropout> {
 Tensor dropout(const Tensor& x, double p, uint64_t seed, const Maybe& seed_tensor,
                uint64_t offset, const Maybe& residual) {
   const Tensor held = or_none(seed_tensor), res = or_none(residual);
+  no_tangents({x, res});
   if (held.defined())
     CHECK_VALUE(held.numel() == 1 && held.scalar_type() == at::kLong,
                       "a seed tensor must hold one int64 value, got ", held.sizes(), " of ",

@@ -160,3 +160,19 @@ def test_seed_on_another_device_is_refused():
 
     with pytest.raises(RuntimeError, match="CUDA"):
         dropout(torch.ones(4, device="cuda"), 0.5, torch.tensor([1]))
+
+
+@pytest.mark.parametrize("requires_grad", [False, True])
+def test_forward_mode_is_refused(requires_grad):
+    from torch.autograd import forward_ad
+
+    from dynamicconvolutionoperator_b200 import dropout
+
+    x = torch.randn(40, device="cuda", requires_grad=requires_grad)
+    with forward_ad.dual_level():
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            dropout(forward_ad.make_dual(x, torch.ones_like(x)), 0.5, 1)
+        if requires_grad:  # forward over reverse
+            out = dropout(x, 0.5, 1)
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                torch.autograd.grad(out, x, forward_ad.make_dual(torch.ones_like(x), x.detach()))

@@ -367,3 +367,20 @@ def test_second_derivative_is_refused():
     g, = torch.autograd.grad(linear_act(x, w, None, "silu").sum(), x, create_graph=True)
     with pytest.raises(RuntimeError, match="once_differentiable|not require grad"):
         g.sum().backward()
+
+
+@pytest.mark.parametrize("requires_grad", [False, True])
+def test_forward_mode_is_refused(requires_grad):
+    from torch.autograd import forward_ad
+
+    from dynamicconvolutionoperator_b200 import linear_act
+
+    x, w, _, _, dy = _case(12, 24, 40, torch.float32)
+    x.requires_grad_(requires_grad)
+    with forward_ad.dual_level():
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            linear_act(forward_ad.make_dual(x, torch.ones_like(x)), w)
+        if requires_grad:  # forward over reverse
+            out = linear_act(x, w, None, "silu")
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                torch.autograd.grad(out, x, forward_ad.make_dual(dy, torch.ones_like(dy)))

@@ -313,3 +313,19 @@ def test_nan_stays_in_its_group():
     got = group_norm_act(x, 2, w, b, activation="relu")
     assert got[0, :4].isnan().all() and got[1, 4:].isnan().all()
     assert torch.equal(got[0, 4:], want[0, 4:]) and torch.equal(got[1, :4], want[1, :4])
+
+
+@pytest.mark.parametrize("requires_grad", [False, True])
+def test_forward_mode_is_refused(requires_grad):
+    from torch.autograd import forward_ad
+
+    from dynamicconvolutionoperator_b200 import group_norm_act
+
+    x = torch.randn(2, 8, 4, 4, device="cuda", requires_grad=requires_grad)
+    with forward_ad.dual_level():
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            group_norm_act(forward_ad.make_dual(x, torch.ones_like(x)), 2)
+        if requires_grad:  # forward over reverse
+            out = group_norm_act(x, 2)
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                torch.autograd.grad(out, x, forward_ad.make_dual(torch.ones_like(x), x.detach()))

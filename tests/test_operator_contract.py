@@ -166,3 +166,34 @@ def test_ddpm_head_refusals(kwargs, match):
 
     with pytest.raises(ValueError, match=match):
         DDPM(4, 3, **kwargs)
+
+
+def _calls():
+    """Every operator as a function of one argument that may carry a derivative."""
+    x, w, v = torch.randn(2, 4, 3, 3), torch.randn(5, 3), torch.randn(4)
+    return {
+        "norm x": (lambda t: group_norm_act(t, 2), x),
+        "norm weight": (lambda t: group_norm_act(x, 2, t), v),
+        "norm bias": (lambda t: group_norm_act(x, 2, None, t), v),
+        "linear x": (lambda t: linear_act(t, w), x),
+        "linear weight": (lambda t: linear_act(x, t), w),
+        "linear bias": (lambda t: linear_act(x, w, t), torch.randn(5)),
+        "linear residual": (lambda t: linear_act(x, w, None, "relu", t), torch.randn(2, 4, 3, 5)),
+        "dropout x": (lambda t: dropout(t, 0.5, 1), x),
+        "dropout residual": (lambda t: dropout(x, 0.5, 1, residual=t), x),
+    }
+
+
+@pytest.mark.parametrize("requires_grad", [False, True])
+@pytest.mark.parametrize("name", list(_calls()))
+def test_forward_mode_derivatives_are_refused(name, requires_grad):
+    """An output without a tangent would pass for one with a zero derivative."""
+    from torch.autograd import forward_ad
+
+    call, t = _calls()[name]
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(t.requires_grad_(requires_grad), torch.ones_like(t))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            call(dual)
+        with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
+            call(dual)
