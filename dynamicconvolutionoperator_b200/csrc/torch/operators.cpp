@@ -7,10 +7,12 @@
 // A parameter's gradient is written into the caller's buffer where one is
 // attached (`_gradbuf.py`), else into a new tensor.
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
 
 #include <atomic>
 
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 
@@ -127,6 +129,17 @@ bool recorded(std::initializer_list<Tensor> tensors) {
   return false;
 }
 
+// A tracer would record the allocation of an output and not the kernel that
+// fills it: the operators are no ops of torch's.
+void not_traced() {
+  using c10::impl::TorchDispatchModeKey;
+  using Modes = c10::impl::TorchDispatchModeTLS;
+  TORCH_CHECK(!torch::jit::tracer::isTracing() &&
+                  !Modes::get_mode(TorchDispatchModeKey::PROXY) &&
+                  !Modes::get_mode(TorchDispatchModeKey::FAKE),
+              "the DDPM B200 operators cannot be traced (capture a CUDA graph instead)");
+}
+
 // The operators have no forward-mode derivative: an output without a tangent
 // would count as one whose derivative is zero.
 void no_tangents(std::initializer_list<Tensor> tensors) {
@@ -191,6 +204,7 @@ struct GroupNormAct : torch::autograd::Function<GroupNormAct> {
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    not_traced();
     no_tangents({grads[0]});
     const variable_list saved = ctx->get_saved_variables();
     const Tensor &xl = saved[0], &weight = saved[1], &bias = saved[2];
@@ -225,6 +239,7 @@ struct GroupNormAct : torch::autograd::Function<GroupNormAct> {
 Tensor group_norm_act(const Tensor& x, int64_t groups, const Maybe& weight,
                       const Maybe& bias, double eps, int64_t act) {
   const Tensor w = or_none(weight), b = or_none(bias);
+  not_traced();
   no_tangents({x, w, b});
   CHECK_VALUE(x.dim() >= 2, "x must have at least two dimensions [N, C, *], got ", x.sizes());
   const int64_t c = x.size(1);
@@ -304,6 +319,7 @@ struct LinearAct : torch::autograd::Function<LinearAct> {
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    not_traced();
     no_tangents({grads[0]});
     const variable_list saved = ctx->get_saved_variables();
     const Tensor &flat = saved[0], &weight = saved[1], &bias = saved[2];
@@ -340,6 +356,7 @@ struct LinearAct : torch::autograd::Function<LinearAct> {
 Tensor linear_act(const Tensor& x, const Tensor& weight, const Maybe& bias,
                   int64_t act, const Maybe& residual) {
   const Tensor b = or_none(bias), res = or_none(residual);
+  not_traced();
   no_tangents({x, weight, b, res});
   CHECK_VALUE(x.dim() >= 1, "x must have at least one dimension [..., k]");
   const int64_t k = x.size(-1), dims = weight.dim();
@@ -394,6 +411,7 @@ struct Dropout : torch::autograd::Function<Dropout> {
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    not_traced();
     no_tangents({grads[0]});
     const bool residual = ctx->saved_data["residual"].toBool();
     const auto need = needed(ctx, {true, residual});
@@ -409,6 +427,7 @@ struct Dropout : torch::autograd::Function<Dropout> {
 Tensor dropout(const Tensor& x, double p, uint64_t seed, const Maybe& seed_tensor,
                uint64_t offset, const Maybe& residual) {
   const Tensor held = or_none(seed_tensor), res = or_none(residual);
+  not_traced();
   no_tangents({x, res});
   if (held.defined())
     CHECK_VALUE(held.numel() == 1 && held.scalar_type() == at::kLong,

@@ -155,3 +155,19 @@ def test_training_step_with_the_head_captured_and_replayed():
     with pytest.raises(RuntimeError, match="seed"):
         with torch.cuda.graph(torch.cuda.CUDAGraph()):
             m(x, y)
+
+
+def test_tracing_is_refused():
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    from dynamicconvolutionoperator_b200 import DDPM, linear_act
+
+    x, y = torch.randn(2, 1, 16, 9, 10, device="cuda")
+    m = DDPM(16, 3, norm_groups=4, activation="silu", out_dim=8).cuda().eval()
+    with torch.no_grad(), pytest.raises(RuntimeError, match="cannot be traced"):
+        torch.jit.trace(m, (x, y), check_trace=False)
+    # a backward on its own
+    a, w = torch.randn(2, 12, 12, device="cuda", requires_grad=True)
+    out = linear_act(a, w, None, "silu")
+    with pytest.raises(RuntimeError, match="cannot be traced"):
+        make_fx(lambda g: torch.autograd.grad(out, a, g))(torch.ones_like(out))

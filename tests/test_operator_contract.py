@@ -197,3 +197,28 @@ def test_forward_mode_derivatives_are_refused(name, requires_grad):
             call(dual)
         with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
             call(dual)
+
+
+def _jit(call, t):
+    torch.jit.trace(call, (t,), check_trace=False)
+
+
+def _fx(call, t):
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    make_fx(call)(t)
+
+
+def _fake(call, t):
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    with FakeTensorMode(allow_non_fake_inputs=True):
+        call(torch.empty(t.shape))
+
+
+@pytest.mark.parametrize("tracer", [_jit, _fx, _fake])
+@pytest.mark.parametrize("name", ["norm x", "linear x", "dropout x"])
+def test_tracing_is_refused(name, tracer):
+    """A trace would hold the output's allocation without the kernel."""
+    with pytest.raises(RuntimeError, match="cannot be traced"):
+        tracer(*_calls()[name])
