@@ -84,6 +84,9 @@ class DDPM(nn.Module):
         out_dim: 1x1 projection to this many channels (``project.weight``,
             ``project.bias``).
         residual: Add ``x``; needs as many channels out as in.
+
+    A ``norm`` or ``project`` that is replaced by a layer of another kind or
+    configuration, or that has hooks, runs its own forward.
     """
 
     def __init__(
@@ -193,13 +196,17 @@ class DDPM(nn.Module):
 
     def _head(self, out: torch.Tensor, x: torch.Tensor, seed) -> torch.Tensor:
         dt = out.dtype
+        caller = torch.get_autocast_dtype("cuda") if _autocast_enabled() else None
         with torch.autocast("cuda", enabled=False):
             if self.norm is not None:
-                # FP32 parameters go with 16-bit data as they are
-                w, b = (p if p.dtype in (dt, torch.float32) else p.to(dt)
-                        for p in (self.norm.weight, self.norm.bias))
-                out = group_norm_act(out, self.norm.num_groups, w, b, self.norm.eps,
-                                     activation=self.activation)
+                if _is_standard_norm(self.norm):
+                    # FP32 parameters go with 16-bit data as they are
+                    w, b = (p if p is None or p.dtype in (dt, torch.float32) else p.to(dt)
+                            for p in (self.norm.weight, self.norm.bias))
+                    out = group_norm_act(out, self.norm.num_groups, w, b, self.norm.eps,
+                                         activation=self.activation)
+                else:
+                    out = _ACTIVATIONS[self.activation](_own_forward(self.norm, out, caller))
             out = out.permute(0, 2, 3, 1)
             res = x.to(dt).permute(0, 2, 3, 1) if self.residual else None
             if self.dropout and self.training:
@@ -213,8 +220,13 @@ class DDPM(nn.Module):
             elif self.project is None and res is not None:
                 out = out + res
             if self.project is not None:
-                w, b = (p.to(dt) for p in (self.project.weight, self.project.bias))
-                out = linear_act(out, w, b, residual=res)
+                if _is_standard_project(self.project):
+                    w, b = (p if p is None else p.to(dt)
+                            for p in (self.project.weight, self.project.bias))
+                    out = linear_act(out, w, b, residual=res)
+                else:
+                    out = _own_forward(self.project, out.permute(0, 3, 1, 2), caller)
+                    return out if res is None else out + res.permute(0, 3, 1, 2)
             return out.permute(0, 3, 1, 2)
 
     def _body(self, x: torch.Tensor, y: torch.Tensor) -> torch.Tensor:
@@ -275,6 +287,50 @@ def _is_standard_fuse(fuse: nn.Module) -> bool:
         and fuse.groups == 1
         and fuse.padding_mode == "zeros"
     )
+
+
+def _has_hooks(module: nn.Module) -> bool:
+    """Hooks run when the module is called (old-style weight norm, for one,
+    makes its weight in such a hook)."""
+    return bool(module._forward_pre_hooks or module._forward_hooks
+                or module._backward_pre_hooks or module._backward_hooks)
+
+
+def _is_standard_norm(norm: nn.Module) -> bool:
+    """``norm`` is the head's own kind of layer, whose parameters say all."""
+    return type(norm) is nn.GroupNorm and not _has_hooks(norm)
+
+
+def _is_standard_project(project: nn.Module) -> bool:
+    """``project`` is the head's own kind of layer: a 1x1 ``nn.Conv2d`` with
+    stride 1, no padding and one group."""
+    return (
+        type(project) is nn.Conv2d
+        and tuple(project.kernel_size) == (1, 1)
+        and tuple(project.stride) == (1, 1)
+        and project.padding in ((0, 0), "valid", "same")
+        and project.groups == 1
+        and not _has_hooks(project)
+    )
+
+
+_ACTIVATIONS = {
+    None: lambda t: t,
+    "relu": F.relu,
+    "silu": F.silu,
+    "gelu": F.gelu,
+    "gelu_tanh": lambda t: F.gelu(t, approximate="tanh"),
+}
+
+
+def _own_forward(module: nn.Module, x: torch.Tensor,
+                 autocast_dtype: torch.dtype | None) -> torch.Tensor:
+    """A layer of the head that the operators do not cover: its own forward, in
+    its parameters' dtype (under the caller's autocast, if there was one)."""
+    dt = next((p.dtype for p in module.parameters() if p.is_floating_point()), x.dtype)
+    with torch.autocast("cuda", enabled=autocast_dtype is not None,
+                        dtype=autocast_dtype or torch.bfloat16):
+        return module(x.to(dt)).to(x.dtype)
 
 
 _BIAS_LANES = 8  # extra input channels carrying the folded bias (keeps Cin % 8 == 0)

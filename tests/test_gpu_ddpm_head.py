@@ -171,3 +171,70 @@ def test_tracing_is_refused():
     out = linear_act(a, w, None, "silu")
     with pytest.raises(RuntimeError, match="cannot be traced"):
         make_fx(lambda g: torch.autograd.grad(out, a, g))(torch.ones_like(out))
+
+
+def _head_of(dtype=torch.float32, **kwargs):
+    from dynamicconvolutionoperator_b200 import DDPM
+
+    m = DDPM(16, 3, norm_groups=4, activation="silu", out_dim=16, residual=True, **kwargs).cuda()
+    x, y = torch.randn(2, 2, 16, 10, 12, device="cuda").to(dtype)
+    return m.to(dtype), x, y
+
+
+def test_hooks_of_the_heads_layers_run():
+    m, x, y = _head_of()
+    want = m(x, y)
+    seen = []
+    for name in ("norm", "project"):
+        layer = getattr(m, name)
+        layer.register_forward_pre_hook(lambda mod, args, name=name: seen.append(name))
+        layer.register_forward_hook(lambda mod, args, out, name=name: seen.append((name, out)))
+    got = m(x, y)
+    assert [s if isinstance(s, str) else s[0] for s in seen] == ["norm", "norm", "project", "project"]
+    body = m._body(x, y)
+    z = m.project(torch.nn.functional.silu(m.norm(body)))
+    assert torch.equal(got, z + x)
+    # the library's convolution may round its operands to TF32 (2^-11 each)
+    assert (got - want).abs().max() < 2 ** -9 * want.abs().max()
+    # hooks that make the weight: a step on their parameters reaches the result
+    m, x, y = _head_of()
+    torch.nn.utils.weight_norm(m.project)
+    before = m(x, y) - x
+    with torch.no_grad():
+        m.project.weight_g.mul_(2)
+        m.project.bias.mul_(2)
+    assert ((m(x, y) - x) - 2 * before).abs().max() < 2 ** -9 * before.abs().max()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_layers_without_parameters_of_their_own(dtype):
+    from dynamicconvolutionoperator_b200 import group_norm_act, linear_act
+
+    m, x, y = _head_of(dtype)
+    m.norm = torch.nn.GroupNorm(4, 16, affine=False)
+    m.project = torch.nn.Conv2d(16, 16, 1, bias=False).cuda().to(dtype)
+    z = group_norm_act(m._body(x, y), 4, activation="silu").permute(0, 2, 3, 1)
+    want = linear_act(z, m.project.weight, residual=x.permute(0, 2, 3, 1)).permute(0, 3, 1, 2)
+    assert torch.equal(m(x, y), want)
+
+
+@pytest.mark.parametrize("layer", [
+    lambda: torch.nn.Conv2d(16, 8, 1, stride=2),
+    lambda: torch.nn.Conv2d(16, 8, 3, padding=1),
+    lambda: torch.nn.Conv2d(16, 8, 1, groups=4),
+    lambda: torch.nn.Conv2d(16, 8, 1, padding=1),
+    lambda: torch.nn.Sequential(torch.nn.Conv2d(16, 8, 1), torch.nn.ReLU()),
+])
+def test_replaced_projections_run_their_own_forward(layer):
+    m, x, y = _head_of()
+    m.residual, m.project = False, layer().cuda()
+    m.norm = torch.nn.BatchNorm2d(16).cuda().eval()
+    want = m.project(torch.nn.functional.silu(m.norm(m._body(x, y))))
+    got = m(x, y)
+    assert got.shape == want.shape and torch.equal(got, want)
+    # FP32 layers behind a 16-bit body
+    m.generator.bfloat16(), m.fuse.bfloat16()
+    out = m(x.bfloat16(), y.bfloat16())
+    assert out.dtype == torch.bfloat16 and out.shape == want.shape
+    with torch.autocast("cuda", dtype=torch.float16):
+        assert m.float()(x, y).dtype == torch.float16
