@@ -4,8 +4,9 @@
 //   gelu       z * Phi(z), Phi the normal distribution function (erf form)
 //   gelu_tanh  z/2 * (1 + tanh(sqrt(2/pi) (z + 0.044715 z^3)))
 // kFast (16-bit data) takes the hardware's approximate exponential and
-// reciprocal and a fitted Phi, with errors far below the rounding to 16 bits.
-// FP32 data takes the full-precision functions.
+// reciprocal and a fitted Phi, with errors far below the rounding to 16 bits (of
+// gelu: 1.7e-5 of the value, over the whole range). FP32 data takes the
+// full-precision functions.
 #pragma once
 
 #include "common.cuh"
@@ -89,36 +90,40 @@ __device__ __forceinline__ float exp2_fast(float t) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
   return e;
 }
+__device__ __forceinline__ float rcp_fast(float d) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d));
+  return r;
+}
 __device__ __forceinline__ F2 logistic2(F2 t) {
   const float2 u = split(t);
   const float2 d = split(f2(exp2_fast(u.x), exp2_fast(u.y)) + f2(1.f));
-  float rx, ry;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(rx) : "f"(d.x));
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(ry) : "f"(d.y));
-  return f2(rx, ry);
+  return f2(rcp_fast(d.x), rcp_fast(d.y));
 }
 
 constexpr float kLog2e = 1.4426950408889634f;
 
-// Phi(z) = 1 / (1 + e^-s(z)) with s(z) = log(Phi(z) / Phi(-z)) = z p(z^2). p is a
-// polynomial of degree 7 over z^2 <= 25 (constant beyond), fitted here for the
-// least maximum of Phi's relative error below zero, 1.6e-5; |z Phi(z)| is off
-// by at most 2.8e-6. A 16-bit value's half step is 2.4e-4 or more of it. The
-// coefficients hold the factor -log2(e).
-__device__ __forceinline__ F2 normal_cdf(F2 z) {
-  const float2 sq = split(z * z);
-  const F2 u = f2(fminf(sq.x, 25.f), fminf(sq.y, 25.f));
-  F2 q = fma2(u, f2(7.628720572e-11f), f2(-8.903303872e-09f));
-  q = fma2(u, q, f2(4.363843402e-07f));
-  q = fma2(u, q, f2(-1.140831500e-05f));
-  q = fma2(u, q, f2(1.531346206e-04f));
-  q = fma2(u, q, f2(1.431668934e-04f));
-  q = fma2(u, q, f2(-1.049632579e-01f));
-  q = fma2(u, q, f2(-2.302116394e+00f));
-  return logistic2(z * q);
+// -Phi(-|z|), and e = e^(-z^2 / 2). Phi(-t) = e G(t), where G falls slowly (as
+// 1 / t far out): a polynomial of degree 5 in 1 / (1 + 0.36 t), fitted here for the
+// least maximum of its relative error over 0 <= t <= 13.3, 1.1e-5; with the FP32
+// roundings 1.7e-5. So Phi keeps its digits down to -13.2, where bf16 has its least
+// values of z Phi(z) (a fit of log(Phi(z) / Phi(-z)) over z^2 <= 25 was 13 times off at
+// -6); beyond, the exponential gives 0. The coefficients hold the factor -1.
+__device__ __forceinline__ F2 normal_tail(F2 z, F2& e) {
+  const float2 x = split(z * z * f2(-0.5f * kLog2e)), u = split(z);
+  e = f2(exp2_fast(x.x), exp2_fast(x.y));
+  const float2 d = split(fma2(f2(fabsf(u.x), fabsf(u.y)), f2(0.36f), f2(1.f)));
+  const F2 k = f2(rcp_fast(d.x), rcp_fast(d.y));
+  F2 g = fma2(k, f2(9.919366325e-02f), f2(-2.561782224e-01f));
+  g = fma2(k, g, f2(-3.334195208e-02f));
+  g = fma2(k, g, f2(-1.695141690e-01f));
+  g = fma2(k, g, f2(-1.399494276e-01f));
+  g = fma2(k, g, f2(-2.050534351e-04f));
+  return e * g;
 }
 
-// Factors of the forms that are z / (1 + e^-s(z)): Phi and its like.
+// Factors of the forms that are z / (1 + e^-s(z)): Phi and its like. (16-bit gelu
+// goes by normal_tail.)
 template <int A> __device__ __forceinline__ float act_gate(float z) {  // FP32 data
   if constexpr (A == DDPM_ACT_SILU) return 1.f / (1.f + expf(-z));
   // erfc keeps the relative precision of the tail below zero
@@ -128,7 +133,6 @@ template <int A> __device__ __forceinline__ float act_gate(float z) {  // FP32 d
 }
 template <int A> __device__ __forceinline__ F2 act_gate(F2 z) {  // 16-bit data
   if constexpr (A == DDPM_ACT_SILU) return logistic2(z * f2(-kLog2e));
-  else if constexpr (A == DDPM_ACT_GELU) return normal_cdf(z);
   else return logistic2(z * fma2(z * z, f2(-kLog2e * 0.07135481627f), f2(-kLog2e * 1.59576912161f)));
 }
 
@@ -139,7 +143,13 @@ template <bool kFast, int A> __device__ __forceinline__ F2 act_value(F2 z) {
     const float2 u = split(z);
     if constexpr (A == DDPM_ACT_RELU)
       return f2(u.x < 0.f ? 0.f : u.x, u.y < 0.f ? 0.f : u.y);  // keeps a NaN
-    else if constexpr (kFast)
+    else if constexpr (kFast && A == DDPM_ACT_GELU) {
+      // max(z, 0) - |z| Phi(-|z|); 14 in place of |z| keeps infinity times 0 out above
+      F2 e;
+      const F2 tail = normal_tail(z, e);
+      return fma2(f2(fmaxf(-u.x, fminf(u.x, 14.f)), fmaxf(-u.y, fminf(u.y, 14.f))), tail,
+                  f2(fmaxf(u.x, 0.f), fmaxf(u.y, 0.f)));
+    } else if constexpr (kFast)
       return z * act_gate<A>(z);
     else
       return z * f2(act_gate<A>(u.x), act_gate<A>(u.y));
@@ -154,24 +164,25 @@ template <bool kFast, int A> __device__ __forceinline__ F2 act_slope(F2 z) {
     if constexpr (A == DDPM_ACT_RELU) {
       return f2(u.x > 0.f ? 1.f : 0.f, u.y > 0.f ? 1.f : 0.f);
     } else {
-      F2 g;
-      if constexpr (kFast) g = act_gate<A>(z);
-      else g = f2(act_gate<A>(u.x), act_gate<A>(u.y));
-      const F2 rest = fma2(g, f2(-1.f), f2(1.f));
-      if constexpr (A == DDPM_ACT_SILU) {
-        return g * fma2(z, rest, f2(1.f));
-      } else if constexpr (A == DDPM_ACT_GELU) {
+      if constexpr (kFast && A == DDPM_ACT_GELU) {
         F2 e;
-        if constexpr (kFast) {
-          const float2 x = split(z * z * f2(-0.5f * kLog2e));
-          e = f2(exp2_fast(x.x), exp2_fast(x.y));
-        } else {
-          e = f2(expf(-0.5f * u.x * u.x), expf(-0.5f * u.y * u.y));
-        }
+        const float2 tail = split(normal_tail(z, e));
+        const F2 g = f2(u.x < 0.f ? -tail.x : 1.f + tail.x, u.y < 0.f ? -tail.y : 1.f + tail.y);
         return fma2(z * f2(0.39894228040143268f), e, g);
       } else {
-        const F2 du = fma2(z * z, f2(0.21406444881f), f2(1.59576912161f));
-        return fma2(z * g, rest * du, g);
+        F2 g;
+        if constexpr (kFast) g = act_gate<A>(z);
+        else g = f2(act_gate<A>(u.x), act_gate<A>(u.y));
+        const F2 rest = fma2(g, f2(-1.f), f2(1.f));
+        if constexpr (A == DDPM_ACT_SILU) {
+          return g * fma2(z, rest, f2(1.f));
+        } else if constexpr (A == DDPM_ACT_GELU) {
+          const F2 e = f2(expf(-0.5f * u.x * u.x), expf(-0.5f * u.y * u.y));
+          return fma2(z * f2(0.39894228040143268f), e, g);
+        } else {
+          const F2 du = fma2(z * z, f2(0.21406444881f), f2(1.59576912161f));
+          return fma2(z * g, rest * du, g);
+        }
       }
     }
   }

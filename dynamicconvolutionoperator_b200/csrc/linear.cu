@@ -51,7 +51,7 @@
 // their FP32 partials added (and the epilogue applied) by a kernel of its own.
 //
 // Measured (bf16): 16384 x 1024 -> 4096 107 us (1280 TFLOP/s, 0.76 of the
-// measured peak; without its copies 98 us), with gelu 121 us; 8192^3 760 us (1450
+// measured peak; without its copies 98 us), with gelu 118 us; 8192^3 760 us (1450
 // TFLOP/s); 65536 x 64 -> 1728 72 us (3.3 TB/s, bound by the epilogue's chain: its
 // warps' TMEM loads, stores to the boxes, fences). FP32: 8192 x 2048 -> 2048 540 us
 // (127 TFLOP/s of FP32 products; bound by shared memory, through which a K block
