@@ -180,7 +180,10 @@ template <bool kFast, int A> __device__ __forceinline__ F2 act_slope(F2 z) {
           const F2 e = f2(expf(-0.5f * u.x * u.x), expf(-0.5f * u.y * u.y));
           return fma2(z * f2(0.39894228040143268f), e, g);
         } else {
-          const F2 du = fma2(z * z, f2(0.21406444881f), f2(1.59576912161f));
+          // beyond |z| = 100 one of g and 1 - g is 0: a z^2 past FP32 must not meet it
+          const float2 sq = split(z * z);
+          const F2 du = fma2(f2(fminf(sq.x, 1e4f), fminf(sq.y, 1e4f)), f2(0.21406444881f),
+                             f2(1.59576912161f));
           return fma2(z * g, rest * du, g);
         }
       }

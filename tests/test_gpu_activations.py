@@ -94,3 +94,19 @@ def test_infinities(name, dtype, rows):
     big = torch.tensor([float("inf"), float("nan")], device="cuda", dtype=dtype)
     out = linear_act(big.repeat(rows // 2)[:, None], one, activation=name).view(-1, 2)
     assert (out[:, 0] == float("inf")).all() and out[:, 1].isnan().all()
+
+
+@pytest.mark.parametrize("rows", [4, 200])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("name", ops.ACTS)
+def test_slopes_of_large_values(name, dtype, rows):
+    """Far out an activation is z or 0 and its slope 1 or 0, also where z^2 overflows."""
+    from dynamicconvolutionoperator_b200 import linear_act
+
+    z = torch.tensor([1e20, -1e20, 3e38, -3e38, 1e10, -1e10, 150., -150.], device="cuda", dtype=dtype)
+    x = z.repeat(rows)[:, None].requires_grad_()
+    out = linear_act(x, torch.ones(1, 1, dtype=dtype, device="cuda"), activation=name)
+    slope, = torch.autograd.grad(out, x, torch.ones_like(out))
+    want = torch.ones_like(z) if name is None else (z > 0).to(dtype)
+    assert torch.equal(slope.view(-1, 8), want.expand(rows, 8))
+    assert torch.equal(out.detach().view(-1, 8), (z * want).expand(rows, 8))
