@@ -34,7 +34,7 @@ def dropout(x: torch.Tensor, p: float, seed: int | torch.Tensor, offset: int = 0
             device, read when the kernel runs: a captured graph draws a new
             mask on every replay once the tensor is written in between. It
             must not change between the forward and its backward.
-        offset: Position of the first value (64 bits).
+        offset: Position of the first value; every position fits 64 bits.
         residual: Added after the scaling; same shape, dtype and device as ``x``.
     """
     p = float(p)

@@ -169,6 +169,8 @@ int dropout(const void* x, const void* residual, void* out, long long n, double 
   DDPM_CHECK_ARG(p >= 0.0 && p <= 1.0, "p must be between 0 and 1, got %g", p);
   DDPM_CHECK_ARG(dtype_size(dt) > 0, "unknown dtype code %d", dt);
   if (n == 0) return DDPM_OK;
+  DDPM_CHECK_ARG(offset <= UINT64_MAX - (unsigned long long)(n - 1),
+                 "the positions must fit 64 bits, got offset %llu", offset);
   DDPM_CHECK_ARG(x && out, "null pointer");
   const uintptr_t es = (uintptr_t)dtype_size(dt);
   const uintptr_t at = (uintptr_t)x | (uintptr_t)residual | (uintptr_t)out;

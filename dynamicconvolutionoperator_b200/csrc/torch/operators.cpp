@@ -437,6 +437,8 @@ Tensor dropout(const Tensor& x, double p, uint64_t seed, const Maybe& seed_tenso
     CHECK_VALUE(res.sizes() == x.sizes() && res.scalar_type() == x.scalar_type(),
                       "residual must have x's shape and dtype, got ", res.sizes(), " of ",
                       res.dtype(), " for ", x.sizes(), " of ", x.dtype());
+  CHECK_VALUE(x.numel() == 0 || offset <= UINT64_MAX - ((uint64_t)x.numel() - 1),
+              "the positions must fit 64 bits, got offset ", offset, " for ", x.numel(), " values");
   on_one_device(x, {held, res});
   dtype_code(x);
   const Tensor xc = x.contiguous(), rc = dense(res);

@@ -438,7 +438,8 @@ DDPM_API int ddpm_linear_bwd(const void* x, long long ldx, const void* weight, c
  * else 0; plus residual[i] where `residual` is not NULL. Position q is kept iff
  * word q % 4 of Philox-4x32-10 with counter (q / 4, 0) and key `seed` is at
  * least round(p * 2^32). `seed_ptr` (device, 8-byte aligned) replaces `seed`
- * when not NULL and is read when the kernel runs. The gradient of x is the same
+ * when not NULL and is read when the kernel runs. Positions fit 64 bits: offset +
+ * size past 2^64 is refused. The gradient of x is the same
  * call on the gradient. `out` may be `x` or `residual`.
  */
 DDPM_API int ddpm_dropout(const void* x, const void* residual, void* out, long long size, double p,

@@ -176,3 +176,12 @@ def test_forward_mode_is_refused(requires_grad):
             out = dropout(x, 0.5, 1)
             with pytest.raises(RuntimeError, match="forward-mode"):
                 torch.autograd.grad(out, x, forward_ad.make_dual(torch.ones_like(x), x.detach()))
+
+
+@pytest.mark.parametrize("size", [1, 6, 4099])
+def test_last_positions(size):
+    from dynamicconvolutionoperator_b200 import dropout
+
+    x = torch.ones(size, device="cuda")
+    offset = (1 << 64) - size
+    assert torch.equal(dropout(x, 0.5, 9, offset) != 0, ops.kept(size, 0.5, 9, offset).cuda())

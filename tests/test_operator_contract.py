@@ -222,3 +222,19 @@ def test_tracing_is_refused(name, tracer):
     """A trace would hold the output's allocation without the kernel."""
     with pytest.raises(RuntimeError, match="cannot be traced"):
         tracer(*_calls()[name])
+
+
+def test_dropout_positions_past_64_bits_are_refused():
+    """The generator's counter would leave the 2^64 positions that a seed has."""
+    x, most = torch.randn(8), (1 << 64) - 1
+    for offset in (most, most - 6):
+        with pytest.raises(ValueError, match="fit 64 bits"):
+            dropout(x, 0.5, 1, offset)
+    for offset in (most - 7, 0):
+        with pytest.raises(RuntimeError, match="CUDA"):
+            dropout(x, 0.5, 1, offset)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        dropout(x[:0], 0.5, 1, most)
+    lib = _lib.load()
+    assert lib.ddpm_dropout(16, None, 16, 8, 0.5, 1, None, most - 6, 0, None) == -1
+    assert b"64 bits" in lib.ddpm_last_error()
