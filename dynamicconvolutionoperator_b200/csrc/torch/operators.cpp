@@ -245,6 +245,7 @@ Tensor group_norm_act(const Tensor& x, int64_t groups, const Maybe& weight,
   const int64_t c = x.size(1);
   CHECK_VALUE(groups >= 1 && c >= 1 && c % groups == 0,
                     "num_groups must divide the channels, got ", groups, " for ", c);
+  TORCH_CHECK(c <= 65536, "group norm supports C <= 65536 (got ", c, ")");  // sizes below are int
   CHECK_VALUE(eps >= 0, "eps must not be negative, got ", eps);
   auto param = [&](const Tensor& t, const char* name) {
     if (!t.defined()) return;

@@ -238,3 +238,13 @@ def test_dropout_positions_past_64_bits_are_refused():
     lib = _lib.load()
     assert lib.ddpm_dropout(16, None, 16, 8, 0.5, 1, None, most - 6, 0, None) == -1
     assert b"64 bits" in lib.ddpm_last_error()
+
+
+@pytest.mark.parametrize("channels", [65544, 2 ** 31, 2 ** 32 + 8])
+def test_too_many_channels_are_refused(channels):
+    """2^32 + 8 channels must not pass for 8."""
+    x = torch.zeros(1).expand(1, channels)
+    with pytest.raises(RuntimeError, match="C <= 65536"):
+        group_norm_act(x, 8)
+    with pytest.raises(RuntimeError, match="C <= 65536"):
+        group_norm_act(x[..., None].requires_grad_(), channels)
