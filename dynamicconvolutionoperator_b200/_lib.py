@@ -141,6 +141,7 @@ _SIGNATURES: dict[str, tuple[object, list[object]]] = {
     ),
     "ddpm_test_skip_arrive": (_c_int, [_c_int]),
     "ddpm_test_disable_tma": (_c_int, [_c_int]),
+    "ddpm_test_linear_choice": (_c_int, [_c_i64] + [_c_int] * 5 + [ctypes.POINTER(_c_int)]),
     "ddpm_umma_selftest": (
         _c_int, [_c_int, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_ptr]
     ),

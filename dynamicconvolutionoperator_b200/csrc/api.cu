@@ -102,6 +102,7 @@ int dropout(const void* x, const void* residual, void* out, long long n, double 
             cudaStream_t st);
 size_t linear_workspace_bytes(long long m, int n, int k, long long ldx, int act, int dt, int bwd,
                               int aligned);
+int linear_choice(long long m, int n, int k, int act, int dt, int product, int* out);
 int linear_fwd(const void* x, long long ldx, const void* w, const void* bias, const void* res,
                void* out, void* ws, size_t ws_bytes, long long m, int n, int k, int act, int dt,
                cudaStream_t st);
@@ -421,6 +422,11 @@ int ddpm_linear_bwd(const void* x, long long ldx, const void* weight, const void
   ddpm::clear_error();
   return ddpm::linear_bwd(x, ldx, weight, bias, grad_out, grad_x, grad_weight, grad_bias, workspace,
                           workspace_bytes, m, n, k, act, dtype, static_cast<cudaStream_t>(stream));
+}
+
+int ddpm_test_linear_choice(long long m, int n, int k, int act, int dtype, int product, int* out) {
+  ddpm::clear_error();
+  return ddpm::linear_choice(m, n, k, act, dtype, product, out);
 }
 
 }  // extern "C"

@@ -1075,32 +1075,50 @@ Tile pick_tile(long long m, int n, long long k, int parts, int splits) {
         least = t;
         // a short K loop leaves the epilogue as the longest part of a tile: twice
         // the warps there (65536 x 64 -> 1728: 94 -> 72 us), which a long one
-        // would pay for with a stage
-        best = Tile{bn, cg, bn == 256 && kb <= kShortK ? 16 : 8};
+        // would pay for with a stage. A block on its own has no room for them
+        // beside two stages, and with one a copy waits for the product before it
+        // (64 x 512 -> 25600: 14.2 us, with 8 warps 9.5 us).
+        best = Tile{bn, cg, cg == 2 && kb <= kShortK ? 16 : 8};
       }
     }
   return best;
 }
 
+int smem_limit() { return gencat::max_smem_optin() - 2048; }  // less the static shared memory
+
+// Stages and boxes of a block, and their bytes. `es`: bytes of a value of out.
+// As many stages as the K loop can use, at least two; what is left goes to the
+// epilogue's boxes, eight a warp at most, two at least.
+struct Rings {
+  int stages, nbuf, smem;
+};
+Rings pick_rings(Tile t, int parts, int es, long long kblocks, int splits) {
+  const int limit = smem_limit(), row = box_row(t.bn, es);
+  auto total = [&](int s, int b) {
+    return (int)smem_layout(t.cg, parts, t.bn, t.ew, row, s, b).total;
+  };
+  // a persistent block streams several tiles through the ring: twice a tile's
+  // steps is as far ahead as it needs to look
+  const long long tiles_k = (kblocks + splits - 1) / splits;
+  Rings r{tiles_k * 2 < kMaxStages ? (int)tiles_k * 2 : kMaxStages, 2, 0};
+  while (r.stages > 2 && total(r.stages, r.nbuf) > limit) --r.stages;
+  while (r.nbuf < kMaxBufs && total(r.stages, r.nbuf + 1) <= limit) ++r.nbuf;
+  r.smem = total(r.stages, r.nbuf);
+  return r;
+}
+
 template <typename T, int BN, int PARTS, Epi kEpi, int CG, int EW>
 int launch_gemm_as(GemmParams& p, cudaStream_t st) {
   auto fn = linear_gemm_kernel<T, BN, PARTS, kEpi, CG, EW>;
-  constexpr int kRow = box_row(BN, kEpi == kPartial ? 4 : (int)sizeof(T));
-  const int tiles_k = (p.kblocks + p.splits - 1) / p.splits;
-  const int limit = gencat::max_smem_optin() - 2048;  // static shared memory
-  // As many stages as the K loop can use, at least two; what is left goes to
-  // the epilogue's boxes, eight a warp at most, two at least.
-  p.nbuf = 2;
-  int stages = kMaxStages;
-  auto total = [&](int s, int b) { return (int)smem_layout(CG, PARTS, BN, EW, kRow, s, b).total; };
-  // a persistent block streams several tiles through the ring: twice a tile's
-  // steps is as far ahead as it needs to look
-  const int useful = tiles_k * 2 < 2 ? 2 : tiles_k * 2;
-  if (stages > useful) stages = useful;
-  while (stages > 1 && total(stages, p.nbuf) > limit) --stages;
-  while (p.nbuf < kMaxBufs && total(stages, p.nbuf + 1) <= limit) ++p.nbuf;
-  p.stages = stages;
-  const int smem = total(stages, p.nbuf);
+  const int limit = smem_limit();
+  const Rings r = pick_rings(Tile{BN, CG, EW}, PARTS, kEpi == kPartial ? 4 : (int)sizeof(T),
+                             p.kblocks, p.splits);
+  if (r.smem > limit)
+    return set_error(DDPM_ERR_UNSUPPORTED, "linear: %d bytes of shared memory, %d needed", limit,
+                     r.smem);
+  p.stages = r.stages;
+  p.nbuf = r.nbuf;
+  const int smem = r.smem;
   static std::atomic<unsigned long long> ready{0};  // devices whose limit is raised
   int dev = 0;
   DDPM_CUDA_TRY(cudaGetDevice(&dev));
@@ -1135,11 +1153,9 @@ int launch_gemm(GemmParams& p, Tile t, cudaStream_t st) {
   if constexpr (sizeof(T) == 4) {
     return t.bn == 128 ? launch_gemm_as<T, 128, 3, kEpi, 1, 8>(p, st)
                        : launch_gemm_as<T, 64, 3, kEpi, 1, 8>(p, st);
-  } else if (t.bn == 256 && t.ew == 16) {
-    return t.cg == 2 ? launch_gemm_as<T, 256, 1, kEpi, 2, 16>(p, st)
-                     : launch_gemm_as<T, 256, 1, kEpi, 1, 16>(p, st);
   } else {
-    return t.cg == 2     ? launch_gemm_as<T, 256, 1, kEpi, 2, 8>(p, st)
+    return t.ew == 16    ? launch_gemm_as<T, 256, 1, kEpi, 2, 16>(p, st)
+           : t.cg == 2   ? launch_gemm_as<T, 256, 1, kEpi, 2, 8>(p, st)
            : t.bn == 256 ? launch_gemm_as<T, 256, 1, kEpi, 1, 8>(p, st)
            : t.bn == 128 ? launch_gemm_as<T, 128, 1, kEpi, 1, 8>(p, st)
                          : launch_gemm_as<T, 64, 1, kEpi, 1, 8>(p, st);
@@ -1554,6 +1570,23 @@ size_t linear_workspace_bytes(long long m, int n, int k, long long ldx, int act,
   const int rc = check_linear(m, n, k, ldx, act, dt);
   if (rc || m == 0) return 0;
   return plan_linear(LinearShape{m, n, k, ldx, act, dt, aligned != 0}, bwd != 0).total;
+}
+
+// For the tests: how a product runs (0 forward or dz, 1 dx, 2 dweight).
+int linear_choice(long long m, int n, int k, int act, int dt, int product, int* out) {
+  const int rc = check_linear(m, n, k, k, act, dt);
+  if (rc) return rc;
+  DDPM_CHECK_ARG(m >= 1 && product >= 0 && product <= 2 && out, "unknown product");
+  const LinearPlan q = plan_linear(LinearShape{m, n, k, k, act, dt, true}, true);
+  const Tile t = product == 0 ? q.tile_z : product == 1 ? q.tile_x : q.tile_w;
+  const int splits = product == 0 ? q.splits_z : product == 1 ? q.splits_x : q.splits_w;
+  const long long terms = product == 0 ? k : product == 1 ? n : m;
+  const int bk = block_k(q.parts);
+  const Rings r = pick_rings(t, q.parts, splits > 1 ? 4 : dtype_size(dt), (terms + bk - 1) / bk,
+                             splits);
+  const int got[6] = {t.bn, t.cg, t.ew, splits, r.stages, r.smem <= smem_limit()};
+  for (int i = 0; i < 6; ++i) out[i] = got[i];
+  return DDPM_OK;
 }
 
 int linear_fwd(const void* x, long long ldx, const void* w, const void* bias, const void* res,

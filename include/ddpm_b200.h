@@ -470,6 +470,15 @@ DDPM_API int ddpm_test_skip_arrive(int enable);
 DDPM_API int ddpm_test_disable_tma(int disabled);
 
 /*
+ * For the tests of ddpm_linear_*: how a product of an aligned call runs on the current
+ * device (148 SMs without one). product: 0 the forward or dz, 1 grad_x, 2 grad_weight.
+ * out[6]: tile columns, blocks that share a tile, epilogue warps, splits of the sum,
+ * stages of the operands' ring, whether the block's shared memory fits.
+ */
+DDPM_API int ddpm_test_linear_choice(long long m, int n, int k, int act, int dtype, int product,
+                                     int* out);
+
+/*
  * Diagnostic (test-only; no reference counterpart): one 128 x n x k bf16 tcgen05 UMMA
  * on a single CTA with the operand layouts the fused kernels use.
  * a: [128 + shift, k] row-major bf16, b: [n, k] row-major bf16,

@@ -145,3 +145,17 @@ def linear(x, w, b, name, res, dy=None):
         "weight": (dz.t() @ xd, dzs.t() @ xd.abs(), dz.abs().t() @ xd.abs()),
         "bias": (dz.sum(0), dzs.sum(0), torch.zeros_like(dz.sum(0))),
     }
+
+
+def linear_choice(m, n, k, dtype, product, name=None):
+    """How a product of ``linear_act`` runs: {"forward", "x", "weight"} as (tile
+    columns, blocks, epilogue warps, splits, stages, fits)."""
+    import ctypes
+
+    from dynamicconvolutionoperator_b200 import _lib
+    from dynamicconvolutionoperator_b200._op import activation_code
+
+    out = (ctypes.c_int * 6)()
+    _lib.call("ddpm_test_linear_choice", m, n, k, activation_code(name), _lib.dtype_code(dtype),
+              ["forward", "x", "weight"].index(product), out)
+    return tuple(out)

@@ -248,3 +248,19 @@ def test_too_many_channels_are_refused(channels):
         group_norm_act(x, 8)
     with pytest.raises(RuntimeError, match="C <= 65536"):
         group_norm_act(x[..., None].requires_grad_(), channels)
+
+
+@pytest.mark.parametrize("dtype", ops.DTYPES)
+def test_every_product_has_a_ring_of_two_stages(dtype):
+    """With one stage a copy would wait for the product before it."""
+    sizes = (1, 16, 64, 200, 512, 1024, 4000, 19_000, 25_600, 40_000, 300_000)
+    seen = set()
+    for m in sizes:
+        for n in sizes:
+            for k in sizes:
+                for product in ("forward", "x", "weight"):
+                    bn, cg, ew, splits, stages, fits = ops.linear_choice(m, n, k, dtype, product)
+                    assert stages >= 2 and fits and splits >= 1, (m, n, k, product)
+                    seen.add((bn, cg, ew))
+    assert seen == ({(64, 1, 8), (128, 1, 8)} if dtype == torch.float32 else
+                    {(64, 1, 8), (128, 1, 8), (256, 1, 8), (256, 2, 8), (256, 2, 16)})
