@@ -140,6 +140,14 @@ class DDPM(nn.Module):
         self.norm = nn.GroupNorm(norm_groups, dim) if norm_groups is not None else None
         self.project = nn.Conv2d(dim, out_dim, 1) if out_dim is not None else None
 
+    def __setstate__(self, state: dict) -> None:
+        """A module pickled before it could have a head has none."""
+        super().__setstate__(state)
+        for name, value in (("norm", None), ("project", None), ("activation", None),
+                            ("dropout", 0.0), ("residual", False)):
+            if name not in self._modules:
+                self.__dict__.setdefault(name, value)
+
     # ------------------------------------------------------------ dispatch --
     def _fused_generator_ok(self, x: torch.Tensor, y: torch.Tensor,
                             weight: torch.Tensor, bias: torch.Tensor | None) -> bool:

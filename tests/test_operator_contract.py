@@ -264,3 +264,20 @@ def test_every_product_has_a_ring_of_two_stages(dtype):
                     seen.add((bn, cg, ew))
     assert seen == ({(64, 1, 8), (128, 1, 8)} if dtype == torch.float32 else
                     {(64, 1, 8), (128, 1, 8), (256, 1, 8), (256, 2, 8), (256, 2, 16)})
+
+
+def test_modules_pickled_without_a_head_load():
+    import pickle
+
+    from dynamicconvolutionoperator_b200 import DDPM
+
+    m = DDPM(4, 3)
+    for name in ("norm", "project", "activation", "dropout", "residual"):
+        del m.__dict__[name]
+    old = pickle.loads(pickle.dumps(m))
+    old._body = lambda x, y: x + y
+    x = torch.ones(1, 4, 2, 2)
+    assert torch.equal(old(x, x), 2 * x)
+    assert set(old.state_dict()) == set(m.state_dict())
+    new = pickle.loads(pickle.dumps(DDPM(4, 3, norm_groups=2, activation="silu", out_dim=4)))
+    assert new.norm.num_groups == 2 and new.project.out_channels == 4 and new.activation == "silu"
