@@ -7,7 +7,8 @@ a plain C-ABI shared object (see ``include/ddpm_b200.h``); Python loads it with
 ctypes, so no torch headers or torch ABI are involved.
 
 ``csrc/torch/*.cpp`` (the operators' autograd side, against torch's headers) goes
-into ``_operators.so`` beside it, which links the library.
+into ``_operators.so`` beside it, which links the library; another torch than the
+one it was built with builds it again.
 
 Usage: ``python -m dynamicconvolutionoperator_b200._build [--force] [--debug]``.
 """
@@ -83,9 +84,15 @@ def _build_operators(force: bool, verbose: bool) -> None:
 
     cxx = os.environ.get("CXX") or shutil.which("g++") or "g++"
     objs = []
+    (BUILD_DIR / "torch").mkdir(parents=True, exist_ok=True)
+    # the module fits the torch it was compiled against only: another one (or other
+    # flags) has to compile it again, which no file's time shows
+    stamp = BUILD_DIR / "torch" / "built_with"
+    with_ = "\n".join([torch.__version__, sys.version, cxx, *flags])
+    if not stamp.exists() or stamp.read_text() != with_:
+        force = True
     for src in sorted((CSRC / "torch").glob("*.cpp")):
         obj = BUILD_DIR / "torch" / (src.stem + ".o")
-        obj.parent.mkdir(exist_ok=True)
         if force or _stale(obj, src, sorted(INCLUDE.glob("*.h"))):
             run([cxx, *flags, "-c", str(src), "-o", str(obj)], f"compiling {src.name}")
         objs.append(obj)
@@ -100,6 +107,7 @@ def _build_operators(force: bool, verbose: bool) -> None:
              *libs, "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch", "-ltorch_python",
              "-l:libstdc++.so.6", "-Wl,-rpath,$ORIGIN"], "linking _operators.so")
         os.replace(tmp, OPERATORS_PATH)
+    stamp.write_text(with_)
 
 
 def build(force: bool = False, debug: bool = False, verbose: bool = False) -> Path:

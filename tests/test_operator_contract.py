@@ -281,3 +281,33 @@ def test_modules_pickled_without_a_head_load():
     assert set(old.state_dict()) == set(m.state_dict())
     new = pickle.loads(pickle.dumps(DDPM(4, 3, norm_groups=2, activation="silu", out_dim=4)))
     assert new.norm.num_groups == 2 and new.project.out_channels == 4 and new.activation == "silu"
+
+
+def test_another_torch_builds_the_operators_again(tmp_path, monkeypatch):
+    """_operators.so fits one torch; file times do not show a change of it."""
+    import subprocess
+
+    from dynamicconvolutionoperator_b200 import _build
+
+    made = []
+
+    def run(cmd, **kwargs):
+        out = _build.Path(cmd[cmd.index("-o") + 1])
+        out.write_text("")
+        made.append(out.name)
+        return subprocess.CompletedProcess(cmd, 0, "", "")
+
+    monkeypatch.setattr(_build.subprocess, "run", run)
+    monkeypatch.setattr(_build, "BUILD_DIR", tmp_path)
+    monkeypatch.setattr(_build, "OPERATORS_PATH", tmp_path / "_operators.so")
+
+    def build():
+        made.clear()
+        _build._build_operators(False, False)
+        return list(made)
+
+    assert build() == ["operators.o", "_operators.so.tmp"]
+    assert build() == []
+    monkeypatch.setattr(torch, "__version__", "0.0.0")
+    assert build() == ["operators.o", "_operators.so.tmp"]
+    assert build() == []
