@@ -26,6 +26,10 @@
 
 namespace ddpm {
 
+namespace gencat {
+int num_sms();
+}  // namespace gencat
+
 namespace {
 
 struct DropParams {
@@ -143,7 +147,7 @@ __global__ void __launch_bounds__(256) dropout_any_kernel(const DropParams p) {
 template <typename T, bool kRes, bool kAll>
 int launch_dropout_as(const DropParams& p, bool vec, cudaStream_t st) {
   const long long items = vec ? (p.n + 16 / sizeof(T) - 1) / (16 / sizeof(T)) : (p.n + 6) / 4;
-  const long long most = 148LL * 8 * 4;
+  const long long most = gencat::num_sms() * 32LL;  // four rounds of eight blocks an SM
   const long long want = (items + 255) / 256;
   const int grid = (int)(want < most ? want : most);
   if (vec) dropout_vec_kernel<T, kRes, kAll><<<grid, 256, 0, st>>>(p);

@@ -13,8 +13,9 @@
 // the second time comes from L2. One persistent launch walks chunks (R pixels
 // of one sample) in order: a block sums chunk t (phase 1), and L steps later,
 // when every block has passed the end of that chunk's sample, writes it
-// (phase 2). L = ceil((chunks of a sample - 1) / grid), 0 or 1 for samples up
-// to 16 MB, so what lies between the two phases is a few tens of MB.
+// (phase 2). L = ceil((chunks of a sample - 1) / grid), where a step of all blocks is
+// up to 21 MB of x (backward: 7): 1 for a sample of 16 MB, 3 in the backward. The
+// ring kernel adds two steps. So what lies between the phases is a few tens of MB.
 //
 // The blocks of a sample meet through a counter: the last one to add its
 // partial sums folds the sample's partials in their fixed order (no floating
@@ -448,7 +449,7 @@ __global__ void __launch_bounds__(kThreads, kBwd ? 2 : 3) norm_kernel(const Norm
           __nanosleep(32);
           if (tc::globaltimer_ns() - began > kWaitLimitNs) {
             sh_abort = 1;
-            atomicExch(p.status, 90);
+            atomicCAS(p.status, 0, 90);
             break;
           }
         }
@@ -600,7 +601,7 @@ struct RingShared {
   float2 sums[2][kWork];
   float2 stat1[kMaxSlots][kRingGroups];  // backward, phase 1: mean, rstd
   float4 stat2[2][kRingGroups];          // phase 2: mean, rstd, A, B
-  int abort, last;
+  int abort;
 };
 
 // The row loop of a phase, specialised for the activation.
@@ -721,7 +722,7 @@ __global__ void __launch_bounds__(kRingThreads, 1) norm_ring_kernel(const RingPa
     if (rp.resident || !write) keep = drop;  // read once
     auto fetch = [&](Walk& walk, uint64_t policy) {
       if (!ring_wait(&sh.empty[s], turn ^ 1, abort_flag)) {
-        fail(96);
+        fail(102);
         ok = false;
         return;
       }

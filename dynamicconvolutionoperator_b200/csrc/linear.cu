@@ -1030,7 +1030,7 @@ template <typename T> struct OpOf { using type = T; };
 template <> struct OpOf<float> { using type = __nv_bfloat16; };
 
 int small_grid(long long items) {
-  const long long want = (items + 255) / 256, most = 148 * 8;
+  const long long want = (items + 255) / 256, most = gencat::num_sms() * 8;
   return (int)(want < 1 ? 1 : want < most ? want : most);
 }
 

@@ -311,3 +311,17 @@ def test_another_torch_builds_the_operators_again(tmp_path, monkeypatch):
     monkeypatch.setattr(torch, "__version__", "0.0.0")
     assert build() == ["operators.o", "_operators.so.tmp"]
     assert build() == []
+
+
+def test_each_wait_of_the_operators_has_its_own_status_code():
+    """A code names the wait that ran out, so no two kernels may record the same one."""
+    import re
+    from collections import Counter
+
+    from dynamicconvolutionoperator_b200 import _build
+
+    codes = Counter()
+    for name in ("groupnorm.cu", "linear.cu"):
+        text = (_build.CSRC / name).read_text()
+        codes.update(re.findall(r"(?:fail\(|status, 0, |p\.status, )(\d+)\)", text))
+    assert len(codes) == 13 and max(codes.values()) == 1, codes
