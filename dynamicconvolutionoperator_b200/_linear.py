@@ -19,8 +19,10 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None 
     """``act(x weight^T + bias) + residual`` with one rounding.
 
     Sums are held in FP32; float32 data keeps its 24 bits (it is multiplied in
-    three bf16 parts, an infinity in it gives a NaN). 16-bit gradients round
-    ``dz = grad * act'`` once, as an operand of the two products it enters.
+    three bf16 parts; an infinity in it gives a NaN in the row or column that it
+    belongs to, but for the forward of up to eight rows, which multiplies in FP32
+    and gives the infinity). 16-bit gradients round ``dz = grad * act'`` once, as an
+    operand of the two products it enters.
 
     Args:
         x: CUDA tensor (float32, bfloat16 or float16) [..., k]. Rows may lie

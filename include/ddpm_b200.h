@@ -413,7 +413,8 @@ DDPM_API int ddpm_group_norm_bwd(const void* x, const void* grad_out, const void
  * x [m][k] (rows `ldx` >= k elements apart), weight [n][k], bias [n] or NULL,
  * residual [m][n] or NULL, out [m][n]; one dtype, FP32 accumulation, one
  * rounding. FP32 data is multiplied as three bf16 parts with the six products
- * above 2^-24 (an infinity in it gives a NaN). Workspace: 256-byte aligned, at
+ * above 2^-24 (an infinity in it gives a NaN; the forward of up to eight rows multiplies
+ * in FP32 and gives the infinity). Workspace: 256-byte aligned, at
  * least the returned bytes; `bwd` selects the entry point, `aligned` says that
  * every pointer of the call is on a 16-byte boundary (0 is always enough).
  * `out` must not overlap the inputs, except that it may be `residual`.

@@ -384,3 +384,23 @@ def test_forward_mode_is_refused(requires_grad):
             out = linear_act(x, w, None, "silu")
             with pytest.raises(RuntimeError, match="forward-mode"):
                 torch.autograd.grad(out, x, forward_ad.make_dual(dy, torch.ones_like(dy)))
+
+
+@pytest.mark.parametrize("dtype", ops.DTYPES)
+@pytest.mark.parametrize("m", [3, 8, 9, 300])
+def test_infinities_stay_in_their_row_or_column(m, dtype):
+    from dynamicconvolutionoperator_b200 import linear_act
+
+    x, w, b, res, _ = _case(m, 40, 24, dtype)
+    want = linear_act(x, w, b, "silu", res)
+    x[1, 5], w[7, 3] = float("inf"), float("-inf")
+    got = linear_act(x, w, b, "silu", res)
+    hit = torch.zeros(m, 40, dtype=torch.bool, device="cuda")
+    hit[1], hit[:, 7] = True, True
+    assert torch.equal(got[~hit], want[~hit]) and not got[hit].isfinite().all()
+    z = linear_act(x, w, b)[1]
+    keep = torch.arange(40, device="cuda") != 7
+    if dtype == torch.float32 and m > 8:  # three bf16 parts: as documented
+        assert z.isnan().all()
+    else:
+        assert torch.equal(z[keep], float("inf") * w[keep, 5].sign())
