@@ -194,15 +194,19 @@ class DDPM(nn.Module):
         return _kernels.fused_dynamic_cat(x, kernels, self.kernel_size, self.dilations)
 
     def forward(self, x: torch.Tensor, y: torch.Tensor,
-                seed: int | torch.Tensor | None = None) -> torch.Tensor:
-        """``seed``: key of the head's dropout (see ``dropout``); None draws one
-        from torch's default CPU generator, which a captured graph cannot do."""
+                seed: int | torch.Tensor | None = None, offset: int = 0) -> torch.Tensor:
+        """``seed`` and ``offset``: key and first position of the head's dropout
+        (see ``dropout``; values are numbered in [N, H, W, C] order). No seed
+        draws one from torch's default CPU generator, which a captured graph
+        cannot do. Ranks with one seed draw one mask: a shard of a batch passes
+        the position of its first value, ``samples before it * H * W * dim``, to
+        draw its part of the whole batch's mask."""
         out = self._body(x, y)
         if self.norm is None and self.project is None and not self.residual and not self.dropout:
             return out
-        return self._head(out, x, seed)
+        return self._head(out, x, seed, offset)
 
-    def _head(self, out: torch.Tensor, x: torch.Tensor, seed) -> torch.Tensor:
+    def _head(self, out: torch.Tensor, x: torch.Tensor, seed, offset: int) -> torch.Tensor:
         dt = out.dtype
         caller = torch.get_autocast_dtype("cuda") if _autocast_enabled() else None
         with torch.autocast("cuda", enabled=False):
@@ -223,7 +227,7 @@ class DDPM(nn.Module):
                         raise RuntimeError("a captured DDPM with dropout needs a seed tensor")
                     seed = int(torch.randint(1 << 62, ()))
                 # numbered in channel-last order; the last step adds the residual
-                out = _dropout(out, self.dropout, seed,
+                out = _dropout(out, self.dropout, seed, offset,
                                residual=res if self.project is None else None)
             elif self.project is None and res is not None:
                 out = out + res

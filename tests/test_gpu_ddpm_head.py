@@ -238,3 +238,15 @@ def test_replaced_projections_run_their_own_forward(layer):
     assert out.dtype == torch.bfloat16 and out.shape == want.shape
     with torch.autocast("cuda", dtype=torch.float16):
         assert m.float()(x, y).dtype == torch.float16
+
+
+def test_shards_draw_the_whole_batchs_mask():
+    from dynamicconvolutionoperator_b200 import DDPM
+
+    m = DDPM(16, 3, norm_groups=4, dropout=0.5).cuda()
+    x, y = torch.randn(2, 4, 16, 9, 7, device="cuda")
+    whole = m(x, y, seed=3) != 0
+    for first, last in ((0, 1), (1, 4)):
+        part = m(x[first:last], y[first:last], seed=3, offset=first * 9 * 7 * 16)
+        assert torch.equal(part != 0, whole[first:last])
+    assert not torch.equal(m(x[1:], y[1:], seed=3) != 0, whole[1:])
