@@ -73,9 +73,10 @@ class DDPM(nn.Module):
             TF32). ``False`` keeps the reference's cuDNN call.
 
     The remaining arguments add a head behind ``fuse``, on the library's
-    channel-last operators; without them the module is the reference's. Its
-    output has channel-last memory, and it is
-    ``project(dropout(act(norm(fuse(...))))) + x`` with the parts asked for:
+    channel-last operators; without them the module is the reference's. The
+    output is ``project(dropout(act(norm(fuse(...))))) + x`` with the parts asked
+    for, in channel-last memory where an operator wrote it (all but ``residual``
+    on its own, and ``dropout`` without the others in evaluation mode):
 
         norm_groups: Group norm over this many groups (``norm.weight``,
             ``norm.bias``), then ``activation``.

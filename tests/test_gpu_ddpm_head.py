@@ -250,3 +250,14 @@ def test_shards_draw_the_whole_batchs_mask():
         part = m(x[first:last], y[first:last], seed=3, offset=first * 9 * 7 * 16)
         assert torch.equal(part != 0, whole[first:last])
     assert not torch.equal(m(x[1:], y[1:], seed=3) != 0, whole[1:])
+
+
+@pytest.mark.parametrize("training", [True, False])
+@pytest.mark.parametrize("head", HEADS)
+def test_memory_of_the_output(head, training):
+    from dynamicconvolutionoperator_b200 import DDPM
+
+    m = DDPM(16, 3, **head).cuda().train(training)
+    x, y = torch.randn(2, 2, 16, 9, 7, device="cuda")
+    wrote = "norm_groups" in head or "out_dim" in head or ("dropout" in head and training)
+    assert m(x, y, seed=1).is_contiguous(memory_format=torch.channels_last) == wrote
