@@ -48,7 +48,8 @@
 // of the sum an addition (16 values of k). Same-sign fp16 data measured -3.9e-4 of
 // the sum at 65536 values and -6.2e-3 at 2^20, more than half a step of bf16. An
 // accumulator takes kChain values of k at most (-1.0e-4); longer sums are split, and
-// their FP32 partials added (and the epilogue applied) by a kernel of its own.
+// their FP32 partials added (and the epilogue applied) by a kernel of its own
+// (dweight of 65536 rows, 4096 x 1024 bf16: 387 -> 437 us; of 262144: 1611, 1605).
 //
 // Measured (bf16): 16384 x 1024 -> 4096 107 us (1280 TFLOP/s, 0.76 of the
 // measured peak; without its copies 98 us), with gelu 118 us; 8192^3 760 us (1450
@@ -1541,7 +1542,10 @@ int backward(const LinearShape& s, const LinearPlan& q, const void* x, const voi
   }
   if (gw && q.splits_w > 1) {
     fw = Fold{part, s.n, pitch4(s.k), q.splits_w, s.k, 0, gw};
-    if (q.splits_w < 16) {
+    // 4096 values: 64 partials 8.5 us by warps that share them, 12.7 a thread a value;
+    // 16384: 12.4 and 14.2; 65536: 22.2 and 15.8 (the whole gradient). Equal at about
+    // 600 values a partial (32 partials of 16384: 11.7 both).
+    if (fw.rows * fw.cols > 512LL * q.splits_w) {
       linear_fold_kernel<T><<<small_grid(fw.rows * fw.cols), 256, 0, st>>>(fw);
       DDPM_CHECK_LAUNCH("linear_fold_kernel");
     } else {
