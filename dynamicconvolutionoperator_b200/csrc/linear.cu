@@ -89,7 +89,7 @@ __host__ __device__ constexpr int gemm_threads(int parts, int ew) {
 constexpr int kMaxStages = 8, kMaxBufs = 8;
 constexpr uint64_t kWaitNs = 2000000000ull;
 constexpr int kGemvRows = 8;
-constexpr int kShortK = 8;  // K blocks
+constexpr int kShortK = 4;  // K blocks
 constexpr int kChain = 16384;  // values of k an accumulator sums (16-bit data)
 
 enum Epi { kOut, kDz, kPartial };
@@ -1075,8 +1075,9 @@ Tile pick_tile(long long m, int n, long long k, int parts, int splits) {
       if (least == 0 || t < least) {
         least = t;
         // a short K loop leaves the epilogue as the longest part of a tile: twice
-        // the warps there (65536 x 64 -> 1728: 94 -> 72 us), which a long one
-        // would pay for with a stage. A block on its own has no room for them
+        // the warps there (65536 x k -> 1728, k = 64: 94 -> 72 us, 128: 95 -> 75, 256:
+        // 97 both), which a longer one pays for with stages (384: 110 -> 121 us, 512:
+        // 122 -> 155). A block on its own has no room for them
         // beside two stages, and with one a copy waits for the product before it
         // (64 x 512 -> 25600: 14.2 us, with 8 warps 9.5 us).
         best = Tile{bn, cg, cg == 2 && kb <= kShortK ? 16 : 8};

@@ -19,7 +19,7 @@ HALF = [
     ((100, 25601, 512), "forward", (256, 1, 8)),
     ((100, 25600, 512), "weight", (256, 2, 16)),
     ((128, 30_000, 1000), "forward", (256, 1, 8)),
-    ((5001, 1504, 304), "forward", (256, 2, 16)),
+    ((5001, 1504, 240), "forward", (256, 2, 16)),
     ((20_000, 256, 264), "x", (256, 2, 16)),
     ((4000, 1200, 1104), "weight", (256, 1, 8)),
     ((1000, 2304, 700), "forward", (128, 1, 8)),

@@ -262,6 +262,9 @@ def test_every_product_has_a_ring_of_two_stages(dtype):
                     bn, cg, ew, splits, stages, fits = ops.linear_choice(m, n, k, dtype, product)
                     assert stages >= 2 and fits and splits >= 1, (m, n, k, product)
                     seen.add((bn, cg, ew))
+    # 16 epilogue warps for a short K loop only
+    assert ops.linear_choice(65536, 1728, 256, torch.bfloat16, "forward")[:3] == (256, 2, 16)
+    assert ops.linear_choice(65536, 1728, 320, torch.bfloat16, "forward")[:3] == (256, 2, 8)
     assert seen == ({(64, 1, 8), (128, 1, 8)} if dtype == torch.float32 else
                     {(64, 1, 8), (128, 1, 8), (256, 1, 8), (256, 2, 8), (256, 2, 16)})
 
