@@ -589,7 +589,13 @@ constexpr int kRingThreads = kWork + 32 * (kMergeWarps + kFoldWarps + 1);
 constexpr int kMaxSlots = 8, kRingGroups = 64;
 constexpr int kRingSmem = 196608;     // bytes of the ring
 constexpr int kSlack = 2;             // steps
-constexpr double kRingBytes = 4e6;    // least size of x
+// Least size of x, and the largest sample that goes to a cluster first. Measured,
+// bf16 with silu, forward / backward, ring and other kernel: one sample of 1 MB (FP32)
+// 13.6 / 14.4 and 16.4 / 14.3 us, of 2 MB 14.4 / 14.5 and 19.0 / 16.2; 32 samples of
+// 128 KB 18.4 / 16.4 and (clusters) 10.3 / 10.7, 65 of 256 KB 23.5 / 26.7 and
+// 20.3 / 24.6, 50 of 512 KB 26.7 / 34.9 and 38.4 / 48.5; 16357 of 8 KB 845 / 582 and
+// 282 / 366: a step of the ring is a microsecond however little it holds.
+constexpr double kRingBytes = 1e6, kClusterFirst = 262144.0;
 
 struct RingParams {
   NormParams n;
@@ -1127,15 +1133,8 @@ bool plan_ring(Plan* q, long long n, long long P, int C, int G, int es, bool bwd
   return true;
 }
 
-// `align`: the largest power of two (in elements, at most 16 bytes' worth)
-// that divides every tensor's address.
-int make_plan(Plan* q, long long n, long long P, int C, int G, int dt, bool bwd, int align) {
-  const int es = dtype_size(dt);
-  *q = Plan{};
-  if (plan_ring(q, n, P, C, G, es, bwd, align)) {
-    place(q, n, G, C, bwd);
-    return DDPM_OK;
-  }
+// Columns of a block of the other kernels.
+void plan_tile(Plan* q, int C, int G, int align) {
   // four channels a thread: eight spill (80 registers, three blocks an SM)
   q->V = gcd_pow2(C, align < 4 ? align : 4);
   const int cols = C / q->V;
@@ -1145,27 +1144,44 @@ int make_plan(Plan* q, long long n, long long P, int C, int G, int dt, bool bwd,
   q->TY = kThreads / q->TX;
   q->U = q->CT == 1 ? G : C;
   q->uw = q->CT == 1 ? C / G : 1;
-  // Small samples: a cluster each (a single block that takes several in turn
-  // where there are many), at least a row of pixels for every thread row and at
-  // most 64 KB of x a block: 16 x 16 x 64 FP32 forward 9.0 -> 7.5 us, and two
-  // calls fewer on the host.
-  if (q->CT == 1) {
-    const int blocks = 3 * gencat::num_sms();
-    for (int cl = 8; cl >= 1 && !q->cluster; cl /= 2) {
-      const long long r = (P + cl - 1) / cl;
-      if (cl > 1 && ((cl - 1) * r >= P || n * cl > blocks || r < q->TY)) continue;
-      if ((double)r * C * es > 65536.0) break;
-      q->cluster = true;
-      q->R = (int)r;
-      q->S = cl;
-      q->chunks = n * cl;
-      q->grid = (int)(q->chunks < blocks ? q->chunks : blocks);
-      q->lag = 0;
-    }
-    if (q->cluster) {
-      place(q, n, G, C, bwd);
-      return DDPM_OK;
-    }
+}
+
+// Small samples: a cluster each (a single block that takes several in turn where
+// there are many), at least a row of pixels for every thread row and at most 64 KB
+// of x a block: 16 x 16 x 64 FP32 forward 9.0 -> 7.5 us, and two calls fewer on the
+// host. (One sample of 512 KB, so at that limit: 17.2 us forward, 19.4 backward, the
+// blocks that wait for one another 14.4 and 12.4; eight of them 17.4 and 19.5, and
+// 19.0 and 16.5; fifty 38 and 48, and 50 and 56.)
+bool plan_cluster(Plan* q, long long n, long long P, int C, int es) {
+  if (q->CT != 1) return false;
+  const int blocks = 3 * gencat::num_sms();
+  for (int cl = 8; cl >= 1; cl /= 2) {
+    const long long r = (P + cl - 1) / cl;
+    if (cl > 1 && ((cl - 1) * r >= P || n * cl > blocks || r < q->TY)) continue;
+    if ((double)r * C * es > 65536.0) break;
+    q->cluster = true;
+    q->R = (int)r;
+    q->S = cl;
+    q->chunks = n * cl;
+    q->grid = (int)(q->chunks < blocks ? q->chunks : blocks);
+    q->lag = 0;
+    return true;
+  }
+  return false;
+}
+
+// `align`: the largest power of two (in elements, at most 16 bytes' worth)
+// that divides every tensor's address.
+int make_plan(Plan* q, long long n, long long P, int C, int G, int dt, bool bwd, int align) {
+  const int es = dtype_size(dt);
+  Plan tile{}, ring{};
+  plan_tile(&tile, C, G, align);
+  const bool cluster = plan_cluster(&tile, n, P, C, es);
+  const bool first = cluster && (double)P * C * es <= kClusterFirst;
+  *q = !first && plan_ring(&ring, n, P, C, G, es, bwd, align) ? ring : tile;
+  if (q->ring || cluster) {
+    place(q, n, G, C, bwd);
+    return DDPM_OK;
   }
   // Two (backward) or three (forward) blocks an SM are resident by the launch
   // bounds; the launch checks it.

@@ -329,3 +329,18 @@ def test_forward_mode_is_refused(requires_grad):
             out = group_norm_act(x, 2)
             with pytest.raises(RuntimeError, match="forward-mode"):
                 torch.autograd.grad(out, x, forward_ad.make_dual(torch.ones_like(x), x.detach()))
+
+
+@pytest.mark.parametrize("dtype", ops.DTYPES)
+@pytest.mark.parametrize("shape,groups", [
+    ((5000, 64, 4, 4), 8),     # many small samples
+    ((70_000, 64), 8),
+    ((2000, 24, 7, 9), 3),
+    ((129, 64, 32, 32), 8),    # clusters of fewer blocks than eight
+    ((300, 64, 48, 48), 8),    # the ring: more samples than blocks
+    ((1, 64, 100, 103), 8),    # and one small sample
+    ((2, 512, 33, 32), 32),
+])
+def test_small_and_many_samples(shape, groups, dtype):
+    x, w, b, dy = _case(shape, dtype, groups, seed=15)
+    _run(x, groups, w, b, dy, "silu", steps=256)

@@ -328,3 +328,14 @@ def test_each_wait_of_the_operators_has_its_own_status_code():
         text = (_build.CSRC / name).read_text()
         codes.update(re.findall(r"(?:fail\(|status, 0, |p\.status, )(\d+)\)", text))
     assert len(codes) == 13 and max(codes.values()) == 1, codes
+
+
+def test_small_samples_need_no_workspace_however_many_there_are():
+    """They go to the kernel without counters in global memory: a step of the other
+    ones costs a microsecond however little it holds."""
+    size = _lib.load().ddpm_group_norm_workspace_bytes
+    for n, pixels, c in ((16_357, 64, 64), (1_000_000, 1, 64), (129, 1024, 64), (64, 256, 512)):
+        for dtype in (1, 2):
+            assert size(n, pixels, c, 8, dtype, 0, 1) == 0, (n, pixels, c)
+    for n, pixels, c in ((32, 4096, 64), (1, 10_300, 64), (64, 65536, 64)):
+        assert size(n, pixels, c, 8, 1, 0, 1) > 0
