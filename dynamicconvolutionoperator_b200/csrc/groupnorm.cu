@@ -576,7 +576,7 @@ __global__ void __launch_bounds__(256) norm_param_kernel(const float2* __restric
 // order. A slot holds a chunk of x (backward: of x and dy).
 //
 // Measured, 64 x 256 x 256 x 64 bf16 with silu: forward 271 us (4.0 TB/s of the
-// 1.07 GB it has to move), backward 527 us (3.1 TB/s); the other kernel took 908
+// 1.07 GB it has to move), backward 517 us (3.1 TB/s); the other kernel took 908
 // and 2306. Neither a unit nor HBM is the limit but the steps' chains (copy, sums,
 // merge, count, fold, write): larger slots (three of 64 KB instead of four of 48:
 // 335 -> 290 us) help, fewer work warps (12 instead of 20) cost nothing, and a

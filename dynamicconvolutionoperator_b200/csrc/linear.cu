@@ -60,7 +60,8 @@
 //
 // Up to eight rows, forward: a dot-product kernel reads the weight once at the
 // memory's rate; a tensor-core tile would be 15/16 empty and its K loop serial (1024 -> 4096
-// bf16: 3.2 us, 2.6 TB/s).
+// bf16: 3.2 us, 2.6 TB/s). Both at 4, 6 and 8 rows: 1024 -> 4096 bf16 6.0, 8.4, 9.8 and
+// (tile) 10.3 us, 4096 -> 4096 18, 26, 32 and 25; FP32 14, 23, 26 and 126.
 #include <atomic>
 #include <type_traits>
 
@@ -1362,7 +1363,9 @@ LinearPlan plan_linear(const LinearShape& s, bool bwd) {
     }
     q.colsum_off = take((size_t)q.colsum_rows * s.n * 4);
     // dweight: the rows are split over the SMs that have no tile, at least four
-    // K blocks a split
+    // K blocks a split (with two, four and eight of them: 4096 rows 256 x 256 bf16
+    // 12.1, 11.3 and 12.1 us, 1024 rows 64 x 64 6.8, 7.7 and 9.6, 4096 rows
+    // 256 x 256 FP32 16.9, 15.6 and 18.3)
     const int bk = block_k(q.parts);
     const long long kb = (s.m + bk - 1) / bk;
     q.tile_w = pick_tile(s.n, s.k, s.m, q.parts, 1);
