@@ -1261,33 +1261,65 @@ int run_gemm(const Gemm& g, cudaStream_t st) {
 
 long long pitch4(int n) { return (n + 3) / 4 * 4; }
 
+// Rows of a split product that are done at a time, so that its partials take no
+// more than kPartBytes (or 256 rows' worth).
+constexpr size_t kPartBytes = 1ull << 30;
+long long part_rows(int splits, long long rows, int cols) {
+  const long long fit = (long long)(kPartBytes / ((size_t)splits * pitch4(cols) * 4)) / 256 * 256;
+  return rows <= fit ? rows : fit < 256 ? 256 : fit;
+}
+size_t part_bytes(int splits, long long rows, int cols) {
+  if (splits == 1) return 0;
+  const long long at_once = part_rows(splits, rows, cols);
+  return (size_t)splits * (at_once < rows ? at_once : rows) * pitch4(cols) * 4;
+}
+
+// Rows m0 .. m0 + rows of a split product, into `part`.
+template <typename T>
+int run_partials(const Gemm& g, long long m0, long long rows, float* part, cudaStream_t st) {
+  Gemm sub = g;
+  const uint8_t* a = static_cast<const uint8_t*>(g.a.ptr);
+  if (g.a_mn) {
+    sub.a.ptr = a + m0 * sizeof(T);
+    sub.a.cols = (int)rows;
+  } else {
+    sub.a.ptr = a + m0 * g.a.pitch * sizeof(T);
+    sub.a.rows = rows;
+  }
+  sub.M = rows;
+  sub.out = part;
+  sub.ld_out = pitch4(g.N);
+  sub.bias = sub.in = nullptr;
+  sub.colsum = nullptr;
+  return run_gemm<T, kPartial>(sub, st);
+}
+
 // A product with an epilogue, over `part` (FP32 partials) where it is split.
 template <typename T, Epi kEpi>
-int run_product(Gemm g, float* part, cudaStream_t st) {
+int run_product(const Gemm& g, float* part, cudaStream_t st) {
   if constexpr (sizeof(T) == 2) {  // FP32 data needs no splits here
     if (g.splits > 1) {
-      Finish f{};
-      f.part = part;
-      f.M = g.M;
-      f.pitch = pitch4(g.N);
-      f.splits = g.splits;
-      f.N = g.N;
-      f.tiles_n = (g.N + 255) / 256;
-      f.act = g.act;
-      f.bias = g.bias;
-      f.in = g.in;
-      f.out = g.out;
-      f.ld_out = g.ld_out;
-      f.colsum = g.colsum;
-      g.out = part;
-      g.ld_out = f.pitch;
-      g.bias = g.in = nullptr;
-      g.colsum = nullptr;
-      const int rc = run_gemm<T, kPartial>(g, st);
-      if (rc) return rc;
-      const long long blocks = (g.M + 31) / 32 * f.tiles_n;
-      linear_finish_kernel<T, kEpi><<<(unsigned)blocks, 256, 0, st>>>(f);
-      DDPM_CHECK_LAUNCH("linear_finish_kernel");
+      const long long step = part_rows(g.splits, g.M, g.N);
+      for (long long m0 = 0; m0 < g.M; m0 += step) {
+        Finish f{};
+        f.part = part;
+        f.M = g.M - m0 < step ? g.M - m0 : step;
+        f.pitch = pitch4(g.N);
+        f.splits = g.splits;
+        f.N = g.N;
+        f.tiles_n = (g.N + 255) / 256;
+        f.act = g.act;
+        f.bias = g.bias;
+        f.in = g.in ? static_cast<const T*>(g.in) + m0 * g.N : nullptr;
+        f.out = static_cast<T*>(g.out) + m0 * g.ld_out;
+        f.ld_out = g.ld_out;
+        f.colsum = g.colsum ? g.colsum + m0 / 32 * g.N : nullptr;  // m0: a multiple of 256
+        const int rc = run_partials<T>(g, m0, f.M, part, st);
+        if (rc) return rc;
+        const long long blocks = (f.M + 31) / 32 * f.tiles_n;
+        linear_finish_kernel<T, kEpi><<<(unsigned)blocks, 256, 0, st>>>(f);
+        DDPM_CHECK_LAUNCH("linear_finish_kernel");
+      }
       return DDPM_OK;
     }
   }
@@ -1337,7 +1369,7 @@ LinearPlan plan_linear(const LinearShape& s, bool bwd) {
   q.tile_z = pick_tile(s.m, s.n, s.k, q.parts, q.splits_z);
   size_t part = 0;  // the products use the partials' memory one after the other
   auto partials = [&](int splits, long long rows, int cols) {
-    const size_t bytes = splits > 1 ? (size_t)splits * rows * pitch4(cols) * 4 : 0;
+    const size_t bytes = part_bytes(splits, rows, cols);
     if (bytes > part) part = bytes;
   };
   if (!q.rows_path && (!bwd || s.act != DDPM_ACT_NONE)) partials(q.splits_z, s.m, s.n);
@@ -1517,6 +1549,7 @@ int backward(const LinearShape& s, const LinearPlan& q, const void* x, const voi
     g.tile = q.tile_x;
     if ((rc = run_product<T, kOut>(g, part, st))) return rc;
   }
+  bool fold_w = gw && q.splits_w > 1;
   if (gw) {
     Gemm g{};
     g.a = zo;
@@ -1527,10 +1560,19 @@ int backward(const LinearShape& s, const LinearPlan& q, const void* x, const voi
     g.K = s.m;
     g.splits = q.splits_w;
     g.tile = q.tile_w;
-    if (q.splits_w > 1) {
-      g.out = part;
-      g.ld_out = pitch4(s.k);
-      if ((rc = run_gemm<T, kPartial>(g, st))) return rc;
+    const long long step = part_rows(q.splits_w, s.n, s.k);
+    if (q.splits_w > 1 && step < s.n) {  // partials in several parts, each added up at once
+      for (long long m0 = 0; m0 < s.n; m0 += step) {
+        const long long rows = s.n - m0 < step ? s.n - m0 : step;
+        if ((rc = run_partials<T>(g, m0, rows, part, st))) return rc;
+        const Fold f{part, rows, pitch4(s.k), q.splits_w, s.k, 0,
+                     static_cast<T*>(gw) + m0 * s.k};
+        linear_fold_kernel<T><<<small_grid(f.rows * f.cols), 256, 0, st>>>(f);
+        DDPM_CHECK_LAUNCH("linear_fold_kernel");
+      }
+      fold_w = false;
+    } else if (q.splits_w > 1) {
+      if ((rc = run_partials<T>(g, 0, s.n, part, st))) return rc;
     } else {
       g.out = gw;
       g.ld_out = s.k;
@@ -1544,7 +1586,7 @@ int backward(const LinearShape& s, const LinearPlan& q, const void* x, const voi
     fb = Fold{colsum, 1, s.n, (int)q.colsum_rows, s.n, 0, gb};
     fb.blocks = blocks(fb);
   }
-  if (gw && q.splits_w > 1) {
+  if (fold_w) {
     fw = Fold{part, s.n, pitch4(s.k), q.splits_w, s.k, 0, gw};
     // 4096 values: 64 partials 8.5 us by warps that share them, 12.7 a thread a value;
     // 16384: 12.4 and 14.2; 65536: 22.2 and 15.8 (the whole gradient). Equal at about

@@ -11,7 +11,7 @@ import pytest
 import torch
 
 from tests import _operators as ops
-from tests.test_gpu_linear_act import _case, _run
+from tests.test_gpu_linear_act import _case, _run, _steps
 
 pytestmark = pytest.mark.gpu
 
@@ -101,3 +101,56 @@ def test_split_sums_captured_and_repeated():
         graph.replay()
     torch.cuda.synchronize()
     assert all(torch.equal(a, e) for a, e in zip(held, once()))
+
+
+def test_partials_of_a_weight_gradient_in_several_parts():
+    """64 splits of 5000 x 1024 partials would take 1.3 GB: 4096 rows of them at a time."""
+    from dynamicconvolutionoperator_b200 import linear_act
+
+    if torch.cuda.mem_get_info()[0] < 32 << 30:
+        pytest.skip("needs 32 GB")
+    rows, n, k = (1 << 20) - 5, 5000, 1024
+    x = _positive(rows, k, torch.bfloat16, 1.0, 11)
+    dy = _positive(rows, n, torch.bfloat16, 2.0 ** -10, 12)
+    w = torch.zeros(n, k, dtype=torch.bfloat16, device="cuda", requires_grad=True)
+    out = linear_act(x, w)
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    gw, = torch.autograd.grad(out, w, dy)
+    assert torch.cuda.max_memory_allocated() - before < 1.1 * 2 ** 30
+    for cols in (slice(0, 20), slice(4086, 4106), slice(n - 20, n)):
+        ref = sum(dy[i:i + (1 << 16), cols].double().t() @ x[i:i + (1 << 16)].double()
+                  for i in range(0, rows, 1 << 16))
+        _close("weight", gw[cols], ref, rows)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_partials_of_a_forward_in_several_parts(dtype):
+    """Two splits of 33001 x 4096 partials: 32768 rows at a time, in the forward and in
+    the product that makes dz."""
+    from dynamicconvolutionoperator_b200 import linear_act
+
+    if torch.cuda.mem_get_info()[0] < 32 << 30:
+        pytest.skip("needs 32 GB")
+    m, n, k = 33_001, 4096, 16_400
+    x, w, b, res, dy = _case(m, n, k, dtype, seed=13)
+    leaves = [t.requires_grad_() for t in (x, w, b)]
+    out = linear_act(*leaves, "silu", res)
+    gx, gw, gb = torch.autograd.grad(out, leaves, dy)
+    half = torch.finfo(dtype).eps / 2
+    for cols in (slice(0, 24), slice(n - 24, n)):
+        ref, scale, _, grads = ops.linear(x.detach(), w.detach()[cols], b.detach()[cols], "silu",
+                                          res[:, cols], dy[:, cols])
+        ops.check("out", out.detach()[:, cols], ref, ops.bound(ref, scale, _steps(k, dtype), dtype))
+        for key, got in (("weight", gw[cols]), ("bias", gb[cols])):
+            r, s, rounded = grads[key]
+            tol = ops.bound(r, s, _steps(m, dtype) + _steps(k, dtype), dtype)
+            tol = tol + half * rounded * (1 + half) + torch.finfo(dtype).tiny * half * m * 8
+            ops.check(key, got, r, tol)
+    # the rows around the seam as a call of their own: the same sums in the same order
+    seam = slice(32_700, m)
+    part = x.detach()[seam].requires_grad_()
+    again = linear_act(part, w.detach(), b.detach(), "silu", res[seam])
+    assert torch.equal(again, out[seam])
+    gp, = torch.autograd.grad(again, part, dy[seam])
+    assert torch.equal(gp, gx[seam])

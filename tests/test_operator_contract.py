@@ -339,3 +339,12 @@ def test_small_samples_need_no_workspace_however_many_there_are():
             assert size(n, pixels, c, 8, dtype, 0, 1) == 0, (n, pixels, c)
     for n, pixels, c in ((32, 4096, 64), (1, 10_300, 64), (64, 65536, 64)):
         assert size(n, pixels, c, 8, 1, 0, 1) > 0
+
+
+def test_partials_of_long_sums_take_a_gigabyte_at_most():
+    size = _lib.load().ddpm_linear_workspace_bytes
+    m, n, k = 1 << 20, 16_384, 16_400  # two splits of it: 137 GB
+    assert size(m, n, k, k, 0, 1, 0, 1) <= 1 << 30
+    extra = -(-m // 64) * n  # column sums for the bias
+    assert size(m, n, k, k, 0, 1, 1, 1) <= (1 << 30) + extra * 4
+    assert size(300, 520, 16_400, 16_400, 0, 1, 0, 1) == -(-2 * 300 * 520 * 4 // 256) * 256
